@@ -325,6 +325,59 @@ int pa_search_reduced_noalloc(int64_t *output_I, float *output_D,
                               int n_neighbors, int n_routers, int n_leaves,
                               int ef_search, void *stream);
 
+/* ---- products of grouped rows, 4-bit tables -----------------------------------
+ * No counterpart upstream.  Rows that were sent to routers (pa_route) put in group
+ * order, every row times the matrix of its own group with the gradients, and tables
+ * held in four bits a value.  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
+ * [1, PA_MAX_GROUPS], a row has at most PA_MAX_WIDTH values, rows < 2^31. */
+#define PA_F32 0
+#define PA_BF16 1
+#define PA_F16 2
+#define PA_MXFP4 0
+#define PA_NVFP4 1
+#define PA_MAX_GROUPS 1024
+#define PA_MAX_WIDTH 65536
+
+/* Stable sort of rows by group: offsets [n_groups + 1], order [rows]; ids outside
+ * [0, n_groups) go behind offsets[n_groups].  workspace: the bytes the first call
+ * says (may be 0, then NULL will do). */
+int64_t pa_group_rows_workspace_bytes(int64_t rows, int n_groups);
+int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *router, int64_t rows,
+                  int n_groups, void *workspace, void *stream);
+
+/* out[i, :] = VT[g] query[i, :] for offsets[g] <= i < offsets[g + 1]; query [rows, d]
+ * with row stride ld_query, VT [n_groups, d_out, d], out [rows, d_out] with row
+ * stride ld_out.  fp32 sums.  Rows of no group become zeros.  offsets are clamped to
+ * [0, rows]; if they do not ascend the result is unspecified, the accesses are not. */
+int pa_project_grouped(void *out, const void *query, const void *VT, const int64_t *offsets,
+                       int64_t rows, int n_groups, int d, int d_out, int64_t ld_query,
+                       int64_t ld_out, int dtype, void *stream);
+/* Gradients: grad_query[i, :] = VT[g]^T grad[i, :], grad_VT[g] = sum of grad[i, :]
+ * query[i, :]^T over the rows of g (zeros without rows).  Either may be NULL. */
+int pa_project_grouped_backward(void *grad_query, void *grad_VT, const void *grad,
+                                const void *query, const void *VT, const int64_t *offsets,
+                                int64_t rows, int n_groups, int d, int d_out, int64_t ld_grad,
+                                int64_t ld_query, int64_t ld_grad_query, int dtype,
+                                void *stream);
+
+/* Rows of d values to 4-bit blocks.  P = d rounded up to a multiple of 32; codes
+ * [rows, P / 2] (E2M1, even value in the low half, zero codes behind d; 16-byte
+ * aligned), scales [rows, P / 32] (PA_MXFP4: E8M0 of blocks of 32) or [rows, P / 16]
+ * (PA_NVFP4: E4M3 of blocks of 16), row_scale [rows] fp32 (PA_NVFP4 only, a power of
+ * two).  NaN or infinity makes the block (PA_MXFP4) or row (PA_NVFP4) NaN. */
+int pa_quantize_fp4(uint8_t *codes, uint8_t *scales, float *row_scale, const void *x,
+                    int64_t rows, int d, int64_t ldx, int dtype, int method, void *stream);
+int pa_dequantize_fp4(float *out, const uint8_t *codes, const uint8_t *scales,
+                      const float *row_scale, int64_t rows, int d, int method, void *stream);
+
+/* out[i, n] = sum_k q(i, k) t(g, n, k) over 4-bit rows [rows, d] and a 4-bit table
+ * [n_groups, d_out, d]; offsets as above, or NULL with n_groups = 1.  fp32 sums, out
+ * [rows, d_out] of out_dtype.  n_groups * d_out < 2^31. */
+int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8_t *query_scales,
+                   const float *query_row_scale, const uint8_t *codes, const uint8_t *scales,
+                   const float *row_scale, const int64_t *offsets, int64_t rows, int n_groups,
+                   int d, int64_t d_out, int out_dtype, int method, void *stream);
+
 /* Kernels launched by this library on behalf of the calling process. */
 int64_t pa_launch_count(void);
 

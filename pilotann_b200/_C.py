@@ -25,6 +25,8 @@ SYMBOLS = (
     "pa_visited_pool_destroy", "pa_visited_pool_slots", "pa_cpu_heap_size_for", "pa_refine_ctas_per_sm",
     "pa_pack_fullgraph", "pa_refine", "pa_stage_attach_refine", "pa_stage_search_ex",
     "pa_stage_search_device_ex", "pa_stage_slot_rows", "pa_stage_submit", "pa_stage_wait",
+    "pa_group_rows_workspace_bytes", "pa_group_rows", "pa_project_grouped",
+    "pa_project_grouped_backward", "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4",
 )
 
 PA_OUT_HANDOFF, PA_OUT_STAGE2, PA_OUT_TOPK = 0, 1, 2
@@ -119,6 +121,20 @@ def lib() -> ctypes.CDLL:
     L.pa_search_reduced_noalloc.argtypes = [P, P, P, P, P, P, P, P, P, c_int64, c_int64, c_int64,
                                             c_int, c_int, c_int, c_int, c_int, P]
     L.pa_search_reduced_noalloc.restype = c_int
+    L.pa_group_rows_workspace_bytes.argtypes = [c_int64, c_int]
+    L.pa_group_rows_workspace_bytes.restype = c_int64
+    L.pa_group_rows.argtypes = [P, P, P, c_int64, c_int, P, P]
+    L.pa_project_grouped.argtypes = [P, P, P, P, c_int64, c_int, c_int, c_int, c_int64, c_int64,
+                                     c_int, P]
+    L.pa_project_grouped_backward.argtypes = [P, P, P, P, P, P, c_int64, c_int, c_int, c_int,
+                                              c_int64, c_int64, c_int64, c_int, P]
+    L.pa_quantize_fp4.argtypes = [P, P, P, P, c_int64, c_int, c_int64, c_int, c_int, P]
+    L.pa_dequantize_fp4.argtypes = [P, P, P, P, c_int64, c_int, c_int, P]
+    L.pa_project_fp4.argtypes = [P, P, P, P, P, P, P, P, c_int64, c_int, c_int, c_int64, c_int,
+                                 c_int, P]
+    for name in ("pa_group_rows", "pa_project_grouped", "pa_project_grouped_backward",
+                 "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4"):
+        getattr(L, name).restype = c_int
     for name in ("pa_traverse_csr", "pa_pack_graph", "pa_traverse_packed", "pa_route",
                  "pa_project", "pa_stage_create", "pa_stage_search", "pa_stage_search_device",
                  "pa_stage_synchronize", "pa_heap_size_for"):

@@ -1,0 +1,33 @@
+// Conversions and the segments of grouped rows, shared by the products.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "pa_common.cuh"
+
+namespace pa {
+namespace grouped {
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);  // round to nearest even
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// The rows as n_groups + 2 segments: those before the first group, the groups, those behind
+// the last.  Edge i (0 .. n_groups + 2) is where segment i starts.
+__device__ __forceinline__ int64_t edge(const int64_t *offsets, int n_groups, int64_t rows, int i) {
+    if (i == 0) return 0;
+    if (i == n_groups + 2) return rows;
+    const int64_t e = offsets[i - 1];
+    return e < 0 ? 0 : (e > rows ? rows : e);
+}
+
+}  // namespace grouped
+}  // namespace pa

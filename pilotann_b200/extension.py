@@ -3,7 +3,8 @@ GPU search stage (``extension/entry.cpp:65-86``): same function names, argument
 order and error behaviour (``RuntimeError``), implemented as ctypes calls into
 the C-ABI library.  Hot names: ``traverse_cuda``, ``routing_cuda``; plus the
 entry points that have no upstream counterpart because upstream keeps its
-tensors in CSR form (``pack_graph``, ``traverse_packed``, ``project``).
+tensors in CSR form (``pack_graph``, ``traverse_packed``, ``project``), and the
+products of grouped rows and 4-bit tables (``products.py``).
 
 Tensors are checked exactly as ``CHECK_CUDA`` does (``extension/inc/common.h:
 23-29``): CUDA device, rank, dtype, contiguity.  Work is enqueued on the
@@ -17,6 +18,8 @@ import threading
 import torch
 
 from . import _C
+from .products import (Fp4Table, dequantize_fp4, group_rows, project_fp4,  # noqa: F401
+                       project_grouped, project_grouped_backward, quantize_fp4)
 
 BEAM_WIDTH = 4
 
