@@ -329,7 +329,7 @@ int pa_search_reduced_noalloc(int64_t *output_I, float *output_D,
  * No counterpart upstream.  Rows that were sent to routers (pa_route) put in group
  * order, every row times the matrix of its own group with the gradients, and tables
  * held in four bits a value.  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
- * [1, PA_MAX_GROUPS], a row has at most PA_MAX_WIDTH values, rows < 2^31. */
+ * [1, PA_MAX_GROUPS], a row has at most PA_MAX_WIDTH values, at most PA_MAX_ROWS rows. */
 #define PA_F32 0
 #define PA_BF16 1
 #define PA_F16 2
@@ -337,6 +337,7 @@ int pa_search_reduced_noalloc(int64_t *output_I, float *output_D,
 #define PA_NVFP4 1
 #define PA_MAX_GROUPS 1024
 #define PA_MAX_WIDTH 65536
+#define PA_MAX_ROWS 0x7fff0000
 
 /* Stable sort of rows by group: offsets [n_groups + 1], order [rows]; ids outside
  * [0, n_groups) go behind offsets[n_groups].  workspace: the bytes the first call

@@ -124,7 +124,7 @@ int quantize_launch(uint8_t *codes, uint8_t *scales, float *row_scale, const voi
 }
 
 int check_table(int64_t rows, int64_t d, int method) {
-    PA_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "rows out of range");
+    PA_REQUIRE(rows >= 0 && rows <= PA_MAX_ROWS, "rows out of range");
     PA_REQUIRE(d >= 1 && d <= PA_MAX_WIDTH, "d must be in [1, %d]", PA_MAX_WIDTH);
     PA_REQUIRE(method == PA_MXFP4 || method == PA_NVFP4, "unknown 4-bit method %d", method);
     return PA_OK;

@@ -114,7 +114,7 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
                               const int64_t *offsets, int64_t rows, int n_groups, int d,
                               int64_t d_out, int out_dtype, int method, void *stream) {
     using namespace pa;
-    PA_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "rows out of range");
+    PA_REQUIRE(rows >= 0 && rows <= PA_MAX_ROWS, "rows out of range");
     PA_REQUIRE(d >= 1 && d <= PA_MAX_WIDTH, "d must be in [1, %d]", PA_MAX_WIDTH);
     PA_REQUIRE(method == PA_MXFP4 || method == PA_NVFP4, "unknown 4-bit method %d", method);
     PA_REQUIRE(out_dtype == PA_F32 || out_dtype == PA_BF16 || out_dtype == PA_F16,

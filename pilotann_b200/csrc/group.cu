@@ -167,7 +167,7 @@ extern "C" int64_t pa_group_rows_workspace_bytes(int64_t rows, int n_groups) {
 extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *router, int64_t rows,
                              int n_groups, void *workspace, void *stream) {
     using namespace pa;
-    PA_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "rows out of range");
+    PA_REQUIRE(rows >= 0 && rows <= PA_MAX_ROWS, "rows out of range");
     PA_REQUIRE(n_groups >= 1 && n_groups <= PA_MAX_GROUPS, "n_groups must be in [1, %d]",
                PA_MAX_GROUPS);
     PA_REQUIRE(offsets && (rows == 0 || (order && router)), "null pointer");

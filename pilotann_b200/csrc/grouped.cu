@@ -120,10 +120,19 @@ matrices_kernel(T *__restrict__ dw, const T *__restrict__ dy, const T *__restric
         }
 }
 
+// rows of 16-bit values that a bulk-tensor copy can start at
+bool ldi_ok(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
 template <typename T>
 int rows_launch(void *out, const void *x, const void *w, const int64_t *offsets, int64_t rows,
                 int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
                 cudaStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        const int64_t ldw = transposed ? d_out : d_sum;
+        if (ldi_ok(x, ldx) && ldi_ok(w, ldw))
+            return rows_mma<T>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo,
+                               transposed, s);
+    }
     dim3 grid(static_cast<unsigned>(rows / kT + n_groups + 2),
               static_cast<unsigned>((d_out + kT - 1) / kT));
     if (transposed)
@@ -142,6 +151,10 @@ int rows_launch(void *out, const void *x, const void *w, const int64_t *offsets,
 template <typename T>
 int matrices_launch(void *dw, const void *dy, const void *x, const int64_t *offsets, int64_t rows,
                     int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (rows > 0 && ldi_ok(dy, ldy) && ldi_ok(x, ldx))
+            return matrices_mma<T>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
+    }
     dim3 grid(static_cast<unsigned>((d + kT - 1) / kT), static_cast<unsigned>((d_out + kT - 1) / kT),
               static_cast<unsigned>(n_groups));
     matrices_kernel<T><<<grid, 256, 0, s>>>(static_cast<T *>(dw), static_cast<const T *>(dy),
@@ -153,7 +166,7 @@ int matrices_launch(void *dw, const void *dy, const void *x, const int64_t *offs
 }
 
 int check(int64_t rows, int n_groups, int d, int d_out, int dtype) {
-    PA_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "rows out of range");
+    PA_REQUIRE(rows >= 0 && rows <= PA_MAX_ROWS, "rows out of range");
     PA_REQUIRE(n_groups >= 1 && n_groups <= PA_MAX_GROUPS, "n_groups must be in [1, %d]",
                PA_MAX_GROUPS);
     PA_REQUIRE(d >= 1 && d <= PA_MAX_WIDTH && d_out >= 1 && d_out <= PA_MAX_WIDTH,

@@ -1,0 +1,455 @@
+// The grouped products of grouped.cu on the tensor cores, for 16-bit values whose rows start on
+// 16 bytes.  All three have the form
+//   D[m, c] = sum_t A(m, t) B(c, t)
+// with m along the axis that is contiguous in the result (128 of them a tile: the lanes of
+// TMEM) and c along its rows:
+//   forward   m = n of y,   c = rows i of a group, t = k:  A = w[g] (t contiguous), B = x
+//   rows      m = k of dx,  c = rows i of a group, t = n:  A = w[g] (m contiguous), B = dy
+//   matrices  m = k of dw,  c = n of dw,           t = i:  A = x, B = dy (m and c contiguous)
+// The rows of a group are on the narrow side of the tile (16 to 256 columns), so that groups
+// of a few rows do not multiply 128; the result is stored lane by lane, 32 neighbours of a row at a
+// time, and columns behind the group's last row are left out, so a tile may hang over into the next
+// group: those columns are computed and dropped.  In `matrices` t runs over rows: the tail of
+// the last slice belongs to the next group and is cleared in shared memory, in both operands,
+// so that a NaN there stays there.
+//
+// Persistent CTAs; warp 0 keeps bulk-tensor copies ahead, warp 1 issues the MMAs, warps 4-7 store
+// the tile before while the next is multiplied (two accumulators in TMEM).  Every wait is
+// bounded.
+#include "grouped.cuh"
+#include "tc05.cuh"
+#include "tmap.cuh"
+
+namespace pa {
+namespace grouped {
+
+namespace mma {
+constexpr int BM = 128, BK = 64;
+constexpr int THREADS = 256;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+enum { FORWARD = 0, ROWS = 1, MATRICES = 2 };
+__host__ __device__ constexpr int b_bytes(int bn) { return bn * BK * 2; }
+__host__ __device__ constexpr int stages(int bn) {
+    return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : 10;
+}
+__host__ __device__ constexpr int smem_bytes(int bn) {
+    return stages(bn) * (A_BYTES + b_bytes(bn)) + 1024;
+}
+}  // namespace mma
+
+struct Shape {
+    int rows, n_groups;
+    int m_size;       // of D: contiguous axis
+    int c_size;       // MATRICES: rows of one matrix
+    int t_size;       // FORWARD, ROWS: summed axis
+    int64_t ldo;
+};
+
+struct Tile {
+    int g;            // group, or -1: rows of no group, zeros
+    int m0;           // first of 128 along the contiguous axis
+    int c0, c_end;    // rows of the result: c0 .. min(c0 + BN, c_end)
+    int t0, t_end;    // summed axis
+    int64_t out_row;  // row of the result that column 0 is
+};
+
+// inclusive prefix over the CTA's threads (all call it): maximum or sum; *all is over all of them
+template <bool MAX>
+__device__ __forceinline__ int cta_scan(int v, int *warp_part_s, int *all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = MAX ? max(v, y) : v + y;
+    }
+    if (lane == 31) warp_part_s[warp] = v;
+    __syncthreads();
+    int before = 0, total = 0;  // the values are not negative
+    for (int w = 0; w < mma::THREADS / 32; ++w) {
+        const int p = warp_part_s[w];
+        if (w < warp) before = MAX ? max(before, p) : before + p;
+        total = MAX ? max(total, p) : total + p;
+    }
+    __syncthreads();
+    *all = total;
+    return MAX ? max(before, v) : before + v;
+}
+
+template <typename T, int MODE, int BN>
+__global__ void __launch_bounds__(mma::THREADS, 1)
+mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
+           const __grid_constant__ CUtensorMap map_b, const int64_t *__restrict__ offsets, Shape sh,
+           int *__restrict__ status) {
+    using namespace mma;
+    constexpr int STAGES = stages(BN), B_BYTES = b_bytes(BN), STAGE_BYTES = A_BYTES + B_BYTES;
+    constexpr bool A_MN = MODE != FORWARD, B_MN = MODE == MATRICES;
+    constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // TMEM columns: a power of two
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
+        quit_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_s;
+    __shared__ int edge_s[PA_MAX_GROUPS + 3];
+    __shared__ int tiles_s[PA_MAX_GROUPS + 3];  // row tiles before segment i
+    __shared__ int warp_part_s[THREADS / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
+
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&full_bar[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&empty_bar[s]), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&acc_full[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 4);
+        }
+        tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
+        abort_s = 0;
+        tc05::fence_barrier_init();
+        tc05::tma_prefetch_desc(&map_a);
+        tc05::tma_prefetch_desc(&map_b);
+    }
+    if (warp == 0) tc05::tmem_alloc(tc05::smem_u32(&tmem_slot), COLS);
+    // segments, made to ascend, and the tiles before each
+    const int segs = sh.n_groups + 2;
+    int carry = 0;
+    for (int i0 = 0; i0 <= segs; i0 += THREADS) {
+        const int i = i0 + tid;
+        const int e = i <= segs ? static_cast<int>(edge(offsets, sh.n_groups, sh.rows, i)) : 0;
+        int all;
+        const int v = cta_scan<true>(e, warp_part_s, &all);
+        if (i <= segs) edge_s[i] = max(carry, v);
+        carry = max(carry, all);
+    }
+    __syncthreads();
+    carry = 0;
+    for (int i0 = 0; i0 < segs; i0 += THREADS) {
+        const int i = i0 + tid;
+        const int own = i < segs ? (static_cast<unsigned>(edge_s[i + 1] - edge_s[i]) + BN - 1) / BN : 0;
+        int all;
+        const int v = cta_scan<false>(own, warp_part_s, &all);
+        if (i < segs) tiles_s[i] = carry + v - own;
+        carry += all;
+    }
+    if (tid == 0) tiles_s[segs] = carry;
+    tc05::fence_before_sync();
+    __syncthreads();
+    tc05::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+
+    const int m_tiles = (sh.m_size + BM - 1) / BM;
+    const int c_tiles = (sh.c_size + BN - 1) / BN;
+    const int64_t n_tiles = MODE == MATRICES
+                                ? static_cast<int64_t>(sh.n_groups) * c_tiles * m_tiles
+                                : static_cast<int64_t>(tiles_s[segs]) * m_tiles;
+    auto tile_at = [&](int64_t t) {
+        Tile r;
+        const int row = static_cast<int>(t / m_tiles);
+        r.m0 = static_cast<int>(t - static_cast<int64_t>(row) * m_tiles) * BM;
+        if (MODE == MATRICES) {
+            r.g = row / c_tiles;
+            r.c0 = (row - r.g * c_tiles) * BN;
+            r.c_end = sh.c_size;
+            r.t0 = edge_s[r.g + 1];
+            r.t_end = max(r.t0, edge_s[r.g + 2]);
+            r.out_row = static_cast<int64_t>(r.g) * sh.c_size + r.c0;
+        } else {
+            int lo = 0, hi = segs;  // the segment with tiles_s[lo] <= row < tiles_s[lo + 1]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (tiles_s[mid] <= row) lo = mid; else hi = mid;
+            }
+            r.g = lo >= 1 && lo <= sh.n_groups ? lo - 1 : -1;
+            r.c0 = edge_s[lo] + (row - tiles_s[lo]) * BN;
+            r.c_end = edge_s[lo + 1];
+            r.t0 = 0;
+            r.t_end = r.g >= 0 ? sh.t_size : 0;
+            r.out_row = r.c0;
+        }
+        return r;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+                const Tile tile = tile_at(t);
+                for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
+                    const int s = it % STAGES;
+                    if (it >= STAGES &&
+                        !tc05::mbar_wait_bounded(tc05::smem_u32(&empty_bar[s]),
+                                                 (it / STAGES - 1) & 1, WAIT_LIMIT)) {
+                        abort_s = 1;
+                        break;
+                    }
+                    const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                    const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+                    tc05::mbar_expect_tx(bar, STAGE_BYTES);
+                    if (MODE == FORWARD) {
+                        tc05::tma_load_3d(a, &map_a, t0, tile.m0, tile.g, bar);
+                        tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
+                    } else if (MODE == ROWS) {
+                        tc05::tma_load_3d(a, &map_a, tile.m0, t0, tile.g, bar);
+                        tc05::tma_load_3d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, tile.g, bar);
+                        tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
+                    } else {
+                        tc05::tma_load_2d(a, &map_a, tile.m0, t0, bar);
+                        tc05::tma_load_2d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, bar);
+#pragma unroll
+                        for (int j = 0; j < BN / 64; ++j)
+                            tc05::tma_load_2d(b + j * 8192, &map_b, tile.c0 + 64 * j, t0, bar);
+                    }
+                }
+            }
+            if (abort_s) {  // no copy is left in flight behind the CTA
+                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                    tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]),
+                                            (i / STAGES) & 1, WAIT_LIMIT);
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc =
+            tc05::idesc_f16(sizeof(T) == 2 && is_bf16<T>(), A_MN, B_MN, BM, BN);
+        uint32_t it = 0, acc_it = 0;
+        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+            const Tile tile = tile_at(t);
+            if (tile.t0 >= tile.t_end) continue;
+            const int slot = acc_it & 1;
+            if (acc_it >= 2 &&
+                !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[slot]), (acc_it / 2 - 1) & 1,
+                                         WAIT_LIMIT)) {
+                abort_s = 1;
+                break;
+            }
+            tc05::fence_after_sync();
+            const uint32_t d = tmem + slot * BN;
+            for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
+                const int s = it % STAGES;
+                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
+                                             WAIT_LIMIT)) {
+                    abort_s = 1;
+                    break;
+                }
+                const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                const int live = MODE == MATRICES ? min(BK, tile.t_end - t0) : BK;
+                if (MODE == MATRICES && live % 16 != 0) {
+                    // rows of the next group up to the end of the last k step: 128 bytes each
+                    const int dead = 16 - live % 16;
+                    for (int i = lane; i < dead * 8 * (2 + BN / 64); i += 32) {
+                        const int chunk = i / (dead * 8), rest = i - chunk * dead * 8;
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                         a + chunk * 8192 + live * 128 + rest * 16),
+                                     "r"(0)
+                                     : "memory");
+                    }
+                    tc05::fence_proxy_async_smem();
+                }
+                __syncwarp();
+                tc05::fence_after_sync();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k) {
+                        if (16 * k < live) {
+                            const uint64_t da =
+                                A_MN ? tc05::smem_desc_mn_sw128(a + k * 2048, A_BYTES / 2)
+                                     : tc05::smem_desc_sw128(a + k * 32);
+                            const uint64_t db = B_MN ? tc05::smem_desc_mn_sw128(b + k * 2048, 8192)
+                                                     : tc05::smem_desc_sw128(b + k * 32);
+                            tc05::mma_f16(d, da, db, idesc, t0 > tile.t0 || k > 0);
+                        }
+                    }
+                    tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
+                    if (t0 + BK >= tile.t_end) tc05::mma_commit(tc05::smem_u32(&acc_full[slot]));
+                }
+                __syncwarp();
+            }
+            ++acc_it;
+        }
+        if (abort_s && lane == 0) {  // nor does a product read on
+            tc05::mma_commit(tc05::smem_u32(&quit_bar));
+            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
+        }
+    } else if (warp >= 4) {
+        const int w = warp - 4;
+        uint32_t acc_it = 0;
+        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+            const Tile tile = tile_at(t);
+            const bool some = tile.t0 < tile.t_end;
+            const int slot = acc_it & 1;
+            if (some) {
+                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
+                                             WAIT_LIMIT)) {
+                    abort_s = 1;
+                    break;
+                }
+                tc05::fence_after_sync();
+            }
+            const int m = tile.m0 + 32 * w + lane;
+            const int live = min(BN, tile.c_end - tile.c0);
+            T *dst = out + tile.out_row * sh.ldo + m;
+            constexpr int STEP = BN < 32 ? BN : 32;
+#pragma unroll 1
+            for (int c0 = 0; c0 < live; c0 += STEP) {
+                uint32_t r[STEP];
+                if (some) {
+                    const uint32_t at = tmem + ((32u * w) << 16) + slot * BN + c0;
+                    if constexpr (STEP == 32) tc05::tmem_ld_32x32(at, r);
+                    else tc05::tmem_ld_32x16(at, r);
+                    tc05::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j) r[j] = 0;
+                }
+                if (m < sh.m_size) {
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j)
+                        if (c0 + j < live)
+                            dst[(c0 + j) * sh.ldo] = from_f32<T>(__uint_as_float(r[j]));
+                }
+            }
+            if (some) {
+                tc05::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&acc_empty[slot]));
+                ++acc_it;
+            }
+        }
+    }
+    __syncwarp();
+    tc05::fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && abort_s) atomicExch(status, 1);
+    if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
+}
+
+// ---- host -------------------------------------------------------------------------
+template <typename T, int MODE, int BN>
+int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
+           const Shape &sh, int64_t most_tiles, cudaStream_t s) {
+    static bool configured[64] = {};
+    int dev = 0, sms = 0;
+    PA_CUDA_TRY(cudaGetDevice(&dev));
+    PA_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64 && !configured[dev]) {
+        PA_CUDA_TRY(cudaFuncSetAttribute(mma_kernel<T, MODE, BN>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         mma::smem_bytes(BN)));
+        configured[dev] = true;
+    }
+    int *status = const_cast<int *>(gemm_status_address());
+    PA_REQUIRE(status != nullptr, "status word not found");
+    const unsigned grid = static_cast<unsigned>(most_tiles < sms ? most_tiles : sms);
+    mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, offsets, sh,
+                                                                            status);
+    count_launch();
+    PA_CUDA_TRY(cudaGetLastError());
+    return PA_OK;
+}
+
+template <typename T> constexpr CUtensorMapDataType map_type() {
+    return is_bf16<T>() ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+template <typename T>
+static int map_rows(CUtensorMap *map, const void *x, int64_t width, int64_t rows, int64_t ld,
+                    int box_rows) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(width), static_cast<uint64_t>(rows)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(ld) * 2};
+    const uint32_t box[2] = {64, static_cast<uint32_t>(box_rows)};
+    return tensor_map(map, map_type<T>(), x, 2, dims, strides, box);
+}
+
+template <typename T>
+static int map_matrices(CUtensorMap *map, const void *w, int64_t d, int64_t d_out, int64_t n_groups,
+                        int box_rows) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(d_out),
+                              static_cast<uint64_t>(n_groups)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(d) * 2, static_cast<uint64_t>(d) * d_out * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(box_rows), 1};
+    return tensor_map(map, map_type<T>(), w, 3, dims, strides, box);
+}
+
+template <typename T, int MODE, int BN>
+static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
+                       int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo,
+                       cudaStream_t s) {
+    CUtensorMap a, b;
+    const bool fwd = MODE == mma::FORWARD;
+    int rc = map_matrices<T>(&a, w, fwd ? d_sum : d_out, fwd ? d_out : d_sum, n_groups,
+                             fwd ? 128 : 64);
+    if (rc != PA_OK) return rc;
+    rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN);
+    if (rc != PA_OK) return rc;
+    const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum, ldo};
+    const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
+    return launch<T, MODE, BN>(out, a, b, offsets, sh, most, s);
+}
+
+template <typename T, int MODE>
+static int rows_mma_mode(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
+                         int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo,
+                         cudaStream_t s) {
+    const int64_t each = (rows + n_groups - 1) / n_groups;  // on average
+#define PA_GO(BN) \
+    return rows_mma_bn<T, MODE, BN>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldo, s)
+    if (each <= 16) PA_GO(16);
+    if (each <= 32) PA_GO(32);
+    if (each <= 64) PA_GO(64);
+    if (each <= 128) PA_GO(128);
+    PA_GO(256);
+#undef PA_GO
+}
+
+template <typename T>
+int rows_mma(void *out, const void *in, const void *w, const int64_t *offsets, int64_t rows,
+             int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo, bool transposed,
+             cudaStream_t s) {
+    T *o = static_cast<T *>(out);
+    const T *i = static_cast<const T *>(in), *m = static_cast<const T *>(w);
+    if (transposed)
+        return rows_mma_mode<T, mma::ROWS>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
+                                           s);
+    return rows_mma_mode<T, mma::FORWARD>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
+                                          s);
+}
+
+template <typename T, int BN>
+static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offsets, int64_t rows,
+                           int n_groups, int d, int d_out, int64_t ldy, int64_t ldx,
+                           cudaStream_t s) {
+    CUtensorMap a, b;
+    int rc = map_rows<T>(&a, x, d, rows, ldx, 64);
+    if (rc != PA_OK) return rc;
+    rc = map_rows<T>(&b, dy, d_out, rows, ldy, 64);
+    if (rc != PA_OK) return rc;
+    const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0, d};
+    const int64_t most =
+        static_cast<int64_t>(n_groups) * ((d + 127) / 128) * ((d_out + BN - 1) / BN);
+    return launch<T, mma::MATRICES, BN>(dw, a, b, offsets, sh, most, s);
+}
+
+template <typename T>
+int matrices_mma(void *dw, const void *dy, const void *x, const int64_t *offsets, int64_t rows,
+                 int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
+    T *o = static_cast<T *>(dw);
+    const T *y = static_cast<const T *>(dy), *i = static_cast<const T *>(x);
+#define PA_GO(BN) return matrices_mma_bn<T, BN>(o, y, i, offsets, rows, n_groups, d, d_out, ldy, ldx, s)
+    if (d_out <= 64) PA_GO(64);
+    if (d_out <= 128) PA_GO(128);
+    PA_GO(256);
+#undef PA_GO
+}
+
+template int rows_mma<__half>(void *, const void *, const void *, const int64_t *, int64_t, int, int,
+                              int, int64_t, int64_t, bool, cudaStream_t);
+template int rows_mma<__nv_bfloat16>(void *, const void *, const void *, const int64_t *, int64_t,
+                                     int, int, int, int64_t, int64_t, bool, cudaStream_t);
+template int matrices_mma<__half>(void *, const void *, const void *, const int64_t *, int64_t, int,
+                                  int, int, int64_t, int64_t, cudaStream_t);
+template int matrices_mma<__nv_bfloat16>(void *, const void *, const void *, const int64_t *,
+                                         int64_t, int, int, int, int64_t, int64_t, cudaStream_t);
+
+}  // namespace grouped
+}  // namespace pa

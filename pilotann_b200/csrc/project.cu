@@ -1,10 +1,9 @@
 // Query projection: rotated = query @ VT^T (upstream runs this on the CPU,
 // pilot_ann/layers/staged.py:198).  out[b, j] = sum_k query[b, k] * VT[j, k].
 // Both operands are K-major, the natural "TN" contraction.
-#include <cuda.h>
-
 #include "pa_common.cuh"
 #include "tc05.cuh"
+#include "tmap.cuh"
 
 namespace pa {
 
@@ -363,6 +362,34 @@ static EncodeTiledFn encode_tiled_fn() {
             fn = reinterpret_cast<EncodeTiledFn>(p);
     }
     return fn;
+}
+
+// A tensor map over `base`: dims and box innermost first, strides in bytes of the axes above the
+// innermost, tiles with the 128-byte swizzle, zeros outside the tensor.
+int tensor_map(CUtensorMap *map, CUtensorMapDataType type, const void *base, int rank,
+               const uint64_t *dims, const uint64_t *strides, const uint32_t *box) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t d[3], st[2];
+    cuuint32_t b[3], elem[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+    for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
+    auto encode = [&]() {
+        return fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, b,
+                  elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult rc = encode();
+    if (rc == CUDA_ERROR_INVALID_CONTEXT || rc == CUDA_ERROR_NOT_INITIALIZED) {
+        // a thread whose first GPU call this is (autograd's): bind the device's context
+        int dev = 0;
+        PA_CUDA_TRY(cudaGetDevice(&dev));
+        PA_CUDA_TRY(cudaSetDevice(dev));
+        rc = encode();
+    }
+    if (rc != CUDA_SUCCESS)
+        return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
+    return PA_OK;
 }
 
 // K-major fp32 matrix [rows, K] with row stride ld, tiles of box_rows x 32 floats

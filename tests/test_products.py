@@ -598,6 +598,34 @@ def test_a_captured_step_while_an_eager_graph_lives():
 
 
 @pytest.mark.gpu
+def test_first_call_of_a_thread():
+    """A thread that has made no GPU call yet has no context bound: a child process, so that
+    the library itself is fresh too."""
+    import subprocess
+    import sys
+    code = """
+import threading, torch
+from pilotann_b200 import extension as e
+x = torch.randn(40, 64, device="cuda").bfloat16()
+w = torch.randn(2, 32, 64, device="cuda").bfloat16()
+o = torch.tensor([0, 10, 40], device="cuda")
+dy = torch.randn(40, 32, device="cuda").bfloat16()
+t = e.quantize_fp4(w)
+torch.cuda.synchronize()
+got = []
+for call in (lambda: e.project_grouped_backward(dy, x, w, o), lambda: e.project_fp4(x, t, o)):
+    thread = threading.Thread(target=lambda: got.append(call()))
+    thread.start(); thread.join()
+assert len(got) == 2, got
+want = e.project_grouped_backward(dy, x, w, o)
+assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1])
+assert torch.equal(got[1], e.project_fp4(x, t, o))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_tensors_on_another_device_than_the_current():
     if torch.cuda.device_count() < 2:
         pytest.skip("one device")
