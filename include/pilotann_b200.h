@@ -373,7 +373,7 @@ int pa_dequantize_fp4(float *out, const uint8_t *codes, const uint8_t *scales,
 
 /* out[i, n] = sum_k q(i, k) t(g, n, k) over 4-bit rows [rows, d] and a 4-bit table
  * [n_groups, d_out, d]; offsets as above, or NULL with n_groups = 1.  fp32 sums, out
- * [rows, d_out] of out_dtype.  n_groups * d_out < 2^31. */
+ * [rows, d_out] of out_dtype.  n_groups * d_out <= PA_MAX_ROWS. */
 int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8_t *query_scales,
                    const float *query_row_scale, const uint8_t *codes, const uint8_t *scales,
                    const float *row_scale, const int64_t *offsets, int64_t rows, int n_groups,

@@ -1,108 +1,454 @@
 // Products of 4-bit rows with a 4-bit table, dense or with one table per group of rows:
 //   out[i, n] = sum_k q(i, k) t(g, n, k)
-// fp32 sums; the segments of rows are those of grouped.cu.
+// on the block-scaled tensor-core instructions (kind::mxf4: E8M0 per 32 values, kind::mxf4nvf4:
+// E4M3 per 16), fp32 sums in TMEM.  The table is the wide side of the tile (128 rows, the
+// lanes of TMEM), the queries the narrow one (16 to 192 columns), as in grouped_mma.cu: few
+// queries do not multiply 128, and a result row is stored 32 neighbours at a time.
+//
+// Codes come by bulk-tensor copies, 256 values (128 bytes) of every row a stage.  Scales are
+// row-major bytes in memory, while the instruction wants, for 128 rows and four bytes each,
+// word (r % 32, r / 32) in TMEM: a loader warp takes 16 bytes of rows l, l + 32, l + 64,
+// l + 96 per lane (512 values of mxfp4, 256 of nvfp4), which is a 4 x 4 transpose in its
+// registers, stores four 16-byte rows without bank conflicts, and tcgen05.cp spreads them.
+// nvfp4's row scales, powers of two, multiply the finished sum.
 #include "fp4.cuh"
 #include "grouped.cuh"
+#include "segments.cuh"
+#include "tc05.cuh"
+#include "tmap.cuh"
 
 namespace pa {
 namespace fp4 {
 
-using grouped::edge;
 using grouped::from_f32;
+using grouped::Segments;
 
-constexpr int kT = 64, kK = 32;
+namespace mma {
+constexpr int BM = 128, BK = 256;        // values; 128 bytes of codes
+constexpr int A_BYTES = BM * BK / 2;
+constexpr int SCALE_SLOTS = 4;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+__host__ __device__ constexpr int b_blocks(int bn) { return bn > 128 ? 2 : 1; }
+__host__ __device__ constexpr int threads(int bn) { return 32 * (7 + b_blocks(bn)); }
+__host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK / 2; }
+__host__ __device__ constexpr int scale_bytes(int bn) { return (1 + b_blocks(bn)) * 2048; }
+__host__ __device__ constexpr int stages(int bn) {
+    return bn >= 192 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 7 : bn >= 32 ? 9 : 10;
+}
+__host__ __device__ constexpr int smem_bytes(int bn) {
+    return stages(bn) * stage_bytes(bn) + SCALE_SLOTS * scale_bytes(bn) + 1024;
+}
+}  // namespace mma
 
-template <int METHOD>
-__device__ __forceinline__ void load_slice(float (*t_s)[kT + 4], const uint8_t *codes,
-                                           const uint8_t *scales, int64_t r0, int n_r, int64_t k0,
-                                           int64_t dp) {
-    // 64 rows x 32 values; a thread has eight of one row
-    const int r = threadIdx.x >> 2, k = 8 * (threadIdx.x & 3);
-    uint32_t code = 0;
-    float b = 0.0f;
-    if (r < n_r) {
-        code = *reinterpret_cast<const uint32_t *>(codes + (r0 + r) * (dp / 2) + (k0 + k) / 2);
-        const uint32_t byte = scales[(r0 + r) * (dp / block_of(METHOD)) + (k0 + k) / block_of(METHOD)];
-        b = METHOD == PA_MXFP4 ? e8m0_value(byte) : e4m3_value(byte);
+struct Args {
+    void *out;
+    const uint8_t *q_scales, *t_scales;
+    const float *q_row_scale, *t_row_scale;
+    const int64_t *offsets;
+    int64_t d_out;
+    int rows, n_groups, values;          // values of a row, padded to 32
+    int q_pitch, t_pitch;                // bytes of scales from row to row
+    int out_dtype;
+    int *status;
+};
+
+// Bytes [at, at + 16) of a row of `pitch` scale bytes, zero behind its end.  Only aligned 16-byte
+// pieces that hold a byte of the row are read.
+struct Piece { uint4 v0, v1; };
+__device__ __forceinline__ Piece scales_fetch(const uint8_t *row, int at, int pitch, bool live) {
+    Piece p = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    const int have = min(16, pitch - at);
+    if (live && have > 0) {
+        const uint8_t *src = row + at;
+        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 15u);
+        const uint4 *base = reinterpret_cast<const uint4 *>(src - shift);
+        p.v0 = __ldg(base);
+        if (shift + have > 16) p.v1 = __ldg(base + 1);
     }
+    return p;
+}
+__device__ __forceinline__ uint4 scales_take(const Piece &p, const uint8_t *row, int at, int pitch) {
+    const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + at) & 15u);
+    uint32_t w[8] = {p.v0.x, p.v0.y, p.v0.z, p.v0.w, p.v1.x, p.v1.y, p.v1.z, p.v1.w};
+    if (shift & 8u) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t_s[k + j][r] = r < n_r ? code_value((code >> (4 * j)) & 15u) * b : 0.0f;
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 4u) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const uint32_t bits = 8u * (shift & 3u);
+    uint32_t r[4];
+    const int have = pitch - at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = __funnelshift_r(w[i], w[i + 1], bits);
+        const int left = have - 4 * i;  // bytes of this word that are the row's
+        if (left < 4) r[i] = left <= 0 ? 0u : r[i] & ((1u << (8 * left)) - 1u);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <int METHOD, typename O>
-__global__ void __launch_bounds__(256)
-project_kernel(O *__restrict__ out, const uint8_t *__restrict__ q_codes,
-               const uint8_t *__restrict__ q_scales, const float *__restrict__ q_row_scale,
-               const uint8_t *__restrict__ t_codes, const uint8_t *__restrict__ t_scales,
-               const float *__restrict__ t_row_scale, const int64_t *__restrict__ offsets,
-               int64_t rows, int n_groups, int d, int64_t d_out) {
-    __shared__ __align__(16) float p_s[kK][kT + 4], q_s[kK][kT + 4];
-    const int64_t dp = padded(d), slot = blockIdx.y;
-    int64_t lo = 0, hi = rows, r0 = slot * kT;
-    int seg = 1;
-    if (offsets != nullptr) {
-        int below = 0;
-        for (int i0 = 0; i0 < n_groups + 2; i0 += 256) {
-            const int i = i0 + threadIdx.x;
-            below += __syncthreads_count(i < n_groups + 2 &&
-                                         edge(offsets, n_groups, rows, i) / kT + i <= slot);
+template <int METHOD, int BN>
+__global__ void __launch_bounds__(mma::threads(BN), 1)
+project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_q,
+               const __grid_constant__ Args args) {
+    using namespace mma;
+    constexpr int THREADS = threads(BN), STAGES = stages(BN), STAGE_BYTES = stage_bytes(BN);
+    constexpr int NB = b_blocks(BN), SLOT_BYTES = scale_bytes(BN);
+    constexpr int GROUP = METHOD == PA_MXFP4 ? 2 : 1;   // stages that 16 scale bytes last
+    constexpr int SCALE_COLS = 16 * (1 + NB);
+    constexpr int ACC_COLS = 2 * BN;
+    constexpr uint32_t COLS = ACC_COLS + 2 * SCALE_COLS <= 128 ? 128
+                              : ACC_COLS + 2 * SCALE_COLS <= 256 ? 256 : 512;
+    static_assert(ACC_COLS + 2 * SCALE_COLS <= 512, "TMEM has 512 columns");
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], sc_full[SCALE_SLOTS],
+        sc_empty[SCALE_SLOTS], acc_full[2], acc_empty[2], quit_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_s;
+    __shared__ Segments segs;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
+    const uint32_t scale_ring = ring + STAGES * STAGE_BYTES;
+
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&full_bar[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&empty_bar[s]), 1);
         }
-        seg = below - 1;
-        lo = edge(offsets, n_groups, rows, seg);
-        hi = edge(offsets, n_groups, rows, seg + 1);
-        r0 = lo + (slot - (lo / kT + seg)) * kT;
-    }
-    if (r0 < lo || r0 >= hi) return;
-    const int n_r = static_cast<int>(min(static_cast<int64_t>(kT), hi - r0));
-    const int64_t c0 = blockIdx.x * static_cast<int64_t>(kT);
-    const int n_c = static_cast<int>(min(static_cast<int64_t>(kT), d_out - c0));
-    const bool grouped_row = seg >= 1 && seg <= n_groups;
-    const int64_t t0 = (seg - 1) * d_out + c0;  // first table row of this tile
-    float acc[4][4] = {};
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int64_t k0 = 0; grouped_row && k0 < dp; k0 += kK) {
-        load_slice<METHOD>(p_s, q_codes, q_scales, r0, n_r, k0, dp);
-        load_slice<METHOD>(q_s, t_codes, t_scales, t0, n_c, k0, dp);
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < kK; ++t) {
-            const float4 a = *reinterpret_cast<const float4 *>(&p_s[t][4 * ty]);
-            const float4 b = *reinterpret_cast<const float4 *>(&q_s[t][4 * tx]);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(av[i], bv[j], acc[i][j]);
+        for (int s = 0; s < SCALE_SLOTS; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&sc_full[s]), 1 + NB);
+            tc05::mbar_init(tc05::smem_u32(&sc_empty[s]), 1);
         }
-        __syncthreads();
+        for (int s = 0; s < 2; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&acc_full[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 4);
+        }
+        tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
+        abort_s = 0;
+        tc05::fence_barrier_init();
+        tc05::tma_prefetch_desc(&map_t);
+        tc05::tma_prefetch_desc(&map_q);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = 4 * ty + i, c = 4 * tx + j;
-            if (r < n_r && c < n_c) {
-                float v = acc[i][j];
-                if (METHOD == PA_NVFP4 && grouped_row) v *= q_row_scale[r0 + r] * t_row_scale[t0 + c];
-                out[(r0 + r) * d_out + c0 + c] = from_f32<O>(v);
+    if (warp == 0) tc05::tmem_alloc(tc05::smem_u32(&tmem_slot), COLS);
+    grouped::segs_make<THREADS>(segs, args.offsets, args.n_groups, args.rows, BN);
+    tc05::fence_before_sync();
+    __syncthreads();
+    tc05::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+
+    const int m_tiles = static_cast<int>((args.d_out + BM - 1) / BM);
+    const int64_t n_tiles = static_cast<int64_t>(segs.tiles[args.n_groups + 2]) * m_tiles;
+    const int n_stages = (args.values + BK - 1) / BK;
+    struct Tile { int g, m0, c0, c_end; };
+    auto tile_at = [&](int64_t t) {
+        Tile r;
+        const int row = static_cast<int>(t / m_tiles);
+        r.m0 = static_cast<int>(t - static_cast<int64_t>(row) * m_tiles) * BM;
+        const int seg = grouped::segs_find(segs, args.n_groups, row);
+        r.g = seg >= 1 && seg <= args.n_groups ? seg - 1 : -1;  // -1: rows of no group, zeros
+        r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
+        r.c_end = segs.edge[seg + 1];
+        return r;
+    };
+
+    if (warp == 0) {
+        // ---- codes ----
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+                const Tile tile = tile_at(t);
+                if (tile.g < 0) continue;
+                for (int k = 0; k < n_stages; ++k, ++it) {
+                    const int s = it % STAGES;
+                    if (it >= STAGES &&
+                        !tc05::mbar_wait_bounded(tc05::smem_u32(&empty_bar[s]),
+                                                 (it / STAGES - 1) & 1, WAIT_LIMIT)) {
+                        abort_s = 1;
+                        break;
+                    }
+                    const uint32_t a = ring + s * STAGE_BYTES;
+                    const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+                    tc05::mbar_expect_tx(bar, STAGE_BYTES);
+                    tc05::tma_load_3d(a, &map_t, k * (BK / 2), tile.m0, tile.g, bar);
+                    tc05::tma_load_2d(a + A_BYTES, &map_q, k * (BK / 2), tile.c0, bar);
+                }
+            }
+            if (abort_s) {  // no copy is left in flight behind the CTA
+                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                    tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]),
+                                            (i / STAGES) & 1, WAIT_LIMIT);
             }
         }
+    } else if (warp == 1) {
+        // ---- products ----
+        if (lane == 0) {
+            uint32_t it = 0, sg = 0, acc_it = 0;
+            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+                const Tile tile = tile_at(t);
+                if (tile.g < 0) continue;
+                const int acc = acc_it & 1;
+                if (acc_it >= 2 && !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[acc]),
+                                                            (acc_it / 2 - 1) & 1, WAIT_LIMIT)) {
+                    abort_s = 1;
+                    break;
+                }
+                tc05::fence_after_sync();
+                const uint32_t d = tmem + acc * BN;
+                uint32_t sa = 0, sb = 0;
+                for (int k = 0; k < n_stages; ++k, ++it) {
+                    const int s = it % STAGES, slot = sg % SCALE_SLOTS;
+                    if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
+                                                 WAIT_LIMIT)) {
+                        abort_s = 1;
+                        break;
+                    }
+                    if (k % GROUP == 0) {
+                        if (!tc05::mbar_wait_bounded(tc05::smem_u32(&sc_full[slot]),
+                                                     (sg / SCALE_SLOTS) & 1, WAIT_LIMIT)) {
+                            abort_s = 1;
+                            break;
+                        }
+                        tc05::fence_after_sync();
+                        sa = tmem + ACC_COLS + (sg & 1) * SCALE_COLS;
+                        sb = sa + 16;
+                        const uint32_t from = scale_ring + slot * SLOT_BYTES;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            tc05::tmem_cp_scales(sa + 4 * w,
+                                                 tc05::smem_desc_rows16(from + 512 * w));
+#pragma unroll
+                            for (int j = 0; j < NB; ++j)
+                                tc05::tmem_cp_scales(
+                                    sb + 4 * (NB * w + j),
+                                    tc05::smem_desc_rows16(from + 2048 * (1 + j) + 512 * w));
+                        }
+                    }
+                    tc05::fence_after_sync();
+                    const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (k * BK + 64 * j < args.values) {
+                            // 64 values: two bytes of a scale word (mxfp4) or all four (nvfp4)
+                            const int word = METHOD == PA_MXFP4 ? 2 * (k % GROUP) + j / 2 : j;
+                            const uint32_t idesc = tc05::idesc_mxf4(
+                                METHOD == PA_MXFP4, BN, METHOD == PA_MXFP4 ? 2 * (j & 1) : 0);
+                            tc05::mma_fp4<METHOD == PA_MXFP4>(
+                                d, tc05::smem_desc_sw128(a + 32 * j),
+                                tc05::smem_desc_sw128(b + 32 * j), idesc, sa + 4 * word,
+                                sb + 4 * NB * word, k > 0 || j > 0);
+                        }
+                    }
+                    tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
+                    if (k % GROUP == GROUP - 1 || k + 1 == n_stages) {
+                        tc05::mma_commit(tc05::smem_u32(&sc_empty[slot]));
+                        ++sg;
+                    }
+                }
+                if (!abort_s) tc05::mma_commit(tc05::smem_u32(&acc_full[acc]));
+                ++acc_it;
+            }
+            if (abort_s) {  // nor does a product read on
+                tc05::mma_commit(tc05::smem_u32(&quit_bar));
+                tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
+            }
+        }
+    } else if (warp < 4 || warp >= 8) {
+        // ---- scales: warp 2 the table's 128 rows, warps 3 and 8 the queries' ----
+        const int block = warp == 2 ? 0 : warp == 3 ? 1 : 2;
+        const int pitch = block == 0 ? args.t_pitch : args.q_pitch;
+        const int n_pieces = (n_stages + GROUP - 1) / GROUP;
+        int64_t t = blockIdx.x;
+        int piece = 0;
+        Tile tile = {};
+        const uint8_t *row[4];
+        bool live[4];
+        auto rows_of_tile = [&]() {  // skips tiles without a group; false at the end
+            while (t < n_tiles) {
+                tile = tile_at(t);
+                if (tile.g >= 0) break;
+                t += gridDim.x;
+            }
+            if (t >= n_tiles) return false;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int r = 32 * b + lane;
+                if (block == 0) {
+                    live[b] = tile.m0 + r < args.d_out;
+                    row[b] = args.t_scales +
+                             (tile.g * args.d_out + tile.m0 + r) * static_cast<int64_t>(pitch);
+                } else {
+                    const int c = 128 * (block - 1) + r;
+                    live[b] = c < BN && tile.c0 + c < tile.c_end;
+                    row[b] = args.q_scales + (tile.c0 + c) * static_cast<int64_t>(pitch);
+                }
+            }
+            return true;
+        };
+        bool more = rows_of_tile();
+        Piece next[4];
+        if (more) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], 0, pitch, live[b]);
+        }
+        for (uint32_t sg = 0; more && !abort_s; ++sg) {
+            uint4 v[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) v[b] = scales_take(next[b], row[b], 16 * piece, pitch);
+            if (++piece == n_pieces) {
+                piece = 0;
+                t += gridDim.x;
+                more = rows_of_tile();
+            }
+            if (more) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    next[b] = scales_fetch(row[b], 16 * piece, pitch, live[b]);
+            }
+            const int slot = sg % SCALE_SLOTS;
+            if (sg >= SCALE_SLOTS &&
+                !tc05::mbar_wait_bounded(tc05::smem_u32(&sc_empty[slot]),
+                                         (sg / SCALE_SLOTS - 1) & 1, WAIT_LIMIT)) {
+                abort_s = 1;
+                break;
+            }
+            const uint32_t to = scale_ring + slot * SLOT_BYTES + 2048 * block + 16 * lane;
+            const uint32_t w[4][4] = {{v[0].x, v[1].x, v[2].x, v[3].x},
+                                      {v[0].y, v[1].y, v[2].y, v[3].y},
+                                      {v[0].z, v[1].z, v[2].z, v[3].z},
+                                      {v[0].w, v[1].w, v[2].w, v[3].w}};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512 * i),
+                             "r"(w[i][0]), "r"(w[i][1]), "r"(w[i][2]), "r"(w[i][3])
+                             : "memory");
+            tc05::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&sc_full[slot]));
+        }
+    } else {
+        // ---- results: warp w has lanes 32 (w - 4) .. of the accumulator ----
+        const int w = warp - 4;
+        uint32_t acc_it = 0;
+        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+            const Tile tile = tile_at(t);
+            const bool some = tile.g >= 0;
+            const int acc = acc_it & 1;
+            const int m = tile.m0 + 32 * w + lane;
+            const bool mine = m < args.d_out;
+            float t_scale = 1.0f;
+            if (METHOD == PA_NVFP4 && some && mine)
+                t_scale = __ldg(args.t_row_scale + tile.g * args.d_out + m);
+            if (some) {
+                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
+                                             WAIT_LIMIT)) {
+                    abort_s = 1;
+                    break;
+                }
+                tc05::fence_after_sync();
+            }
+            const int live = min(BN, tile.c_end - tile.c0);
+            const int64_t at = tile.c0 * args.d_out + m;
+            constexpr int STEP = BN < 32 ? BN : 32;
+#pragma unroll 1
+            for (int c0 = 0; c0 < live; c0 += STEP) {
+                uint32_t r[STEP];
+                float q_scale = 1.0f;
+                if (METHOD == PA_NVFP4 && some && lane < STEP && c0 + lane < live)
+                    q_scale = __ldg(args.q_row_scale + tile.c0 + c0 + lane);
+                if (some) {
+                    const uint32_t col = tmem + ((32u * w) << 16) + acc * BN + c0;
+                    if constexpr (STEP == 32) tc05::tmem_ld_32x32(col, r);
+                    else tc05::tmem_ld_32x16(col, r);
+                    tc05::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j) r[j] = 0;
+                }
+                if (METHOD == PA_NVFP4) {
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j)
+                        r[j] = __float_as_uint(__uint_as_float(r[j]) *
+                                               (t_scale * __shfl_sync(0xffffffffu, q_scale, j)));
+                }
+                auto store = [&](auto *out) {
+                    using O = typename std::remove_pointer<decltype(out)>::type;
+                    O *dst = out + at + c0 * args.d_out;
+#pragma unroll
+                    for (int j = 0; j < STEP; ++j)
+                        if (c0 + j < live) dst[j * args.d_out] = from_f32<O>(__uint_as_float(r[j]));
+                };
+                if (mine) {
+                    if (args.out_dtype == PA_F32) store(static_cast<float *>(args.out));
+                    else if (args.out_dtype == PA_BF16) store(static_cast<__nv_bfloat16 *>(args.out));
+                    else store(static_cast<__half *>(args.out));
+                }
+            }
+            if (some) {
+                tc05::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&acc_empty[acc]));
+                ++acc_it;
+            }
+        }
+    }
+    __syncwarp();
+    tc05::fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && abort_s) atomicExch(args.status, 1);
+    if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
 }
 
-template <int METHOD, typename O>
-int project_launch(void *out, const uint8_t *q_codes, const uint8_t *q_scales,
-                   const float *q_row_scale, const uint8_t *t_codes, const uint8_t *t_scales,
-                   const float *t_row_scale, const int64_t *offsets, int64_t rows, int n_groups,
-                   int d, int64_t d_out, cudaStream_t s) {
-    const int64_t slots = offsets ? rows / kT + n_groups + 2 : (rows + kT - 1) / kT;
-    PA_REQUIRE(slots <= 65535, "too many rows for one call");
-    dim3 grid(static_cast<unsigned>((d_out + kT - 1) / kT), static_cast<unsigned>(slots));
-    project_kernel<METHOD, O><<<grid, 256, 0, s>>>(static_cast<O *>(out), q_codes, q_scales,
-                                                   q_row_scale, t_codes, t_scales, t_row_scale,
-                                                   offsets, rows, n_groups, d, d_out);
+// ---- host -------------------------------------------------------------------------
+static int map_codes(CUtensorMap *map, const uint8_t *codes, int values, int64_t rows,
+                     int64_t n_groups, int box_rows) {
+    const uint64_t width = static_cast<uint64_t>(values) / 2;
+    const uint64_t dims[3] = {width, static_cast<uint64_t>(rows), static_cast<uint64_t>(n_groups)};
+    const uint64_t strides[2] = {width, width * rows};
+    const uint32_t box[3] = {128, static_cast<uint32_t>(box_rows), 1};
+    return tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, n_groups ? 3 : 2, dims, strides,
+                      box);
+}
+
+template <int METHOD, int BN>
+static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t_codes,
+                      cudaStream_t s) {
+    static bool configured[64] = {};
+    int dev = 0, sms = 0;
+    PA_CUDA_TRY(cudaGetDevice(&dev));
+    PA_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64 && !configured[dev]) {
+        PA_CUDA_TRY(cudaFuncSetAttribute(project_kernel<METHOD, BN>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         mma::smem_bytes(BN)));
+        configured[dev] = true;
+    }
+    CUtensorMap map_t, map_q;
+    int rc = map_codes(&map_t, t_codes, args.values, args.d_out, args.n_groups, mma::BM);
+    if (rc != PA_OK) return rc;
+    rc = map_codes(&map_q, q_codes, args.values, args.rows, 0, BN);
+    if (rc != PA_OK) return rc;
+    const int64_t most = (static_cast<int64_t>(args.rows) / BN + args.n_groups + 2) *
+                         ((args.d_out + mma::BM - 1) / mma::BM);
+    const unsigned grid = static_cast<unsigned>(most < sms ? most : sms);
+    project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q,
+                                                                                   args);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
+}
+
+template <int METHOD>
+static int project_method(const Args &args, const uint8_t *q_codes, const uint8_t *t_codes,
+                          cudaStream_t s) {
+    const int each = (args.rows + args.n_groups - 1) / args.n_groups;  // on average
+    if (each <= 16) return project_bn<METHOD, 16>(args, q_codes, t_codes, s);
+    if (each <= 32) return project_bn<METHOD, 32>(args, q_codes, t_codes, s);
+    if (each <= 64) return project_bn<METHOD, 64>(args, q_codes, t_codes, s);
+    if (each <= 128) return project_bn<METHOD, 128>(args, q_codes, t_codes, s);
+    return project_bn<METHOD, 192>(args, q_codes, t_codes, s);
 }
 
 }  // namespace fp4
@@ -122,22 +468,19 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     PA_REQUIRE(n_groups >= 1 && n_groups <= PA_MAX_GROUPS, "n_groups must be in [1, %d]",
                PA_MAX_GROUPS);
     PA_REQUIRE(offsets || n_groups == 1, "several groups need offsets");
-    PA_REQUIRE(d_out >= 0 && d_out * n_groups <= 0x7fffffff, "table rows out of range");
+    PA_REQUIRE(d_out >= 0 && d_out <= PA_MAX_ROWS / n_groups, "table rows out of range");
     if (rows == 0 || d_out == 0) return PA_OK;
     PA_REQUIRE(out && query_codes && query_scales && codes && scales, "null pointer");
     PA_REQUIRE(method == PA_MXFP4 || (query_row_scale && row_scale), "nvfp4 needs row scales");
     PA_REQUIRE(aligned16(query_codes) && aligned16(codes), "codes must be 16-byte aligned");
+    int *status = const_cast<int *>(gemm_status_address());
+    PA_REQUIRE(status != nullptr, "status word not found");
+    const int values = static_cast<int>(fp4::padded(d));
+    const int pitch = values / fp4::block_of(method);
+    const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,
+                         static_cast<int>(rows), n_groups, values, pitch, pitch, out_dtype, status};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define PA_GO(M, O)                                                                              \
-    return fp4::project_launch<M, O>(out, query_codes, query_scales, query_row_scale, codes,     \
-                                     scales, row_scale, offsets, rows, n_groups, d, d_out, s)
-    if (method == PA_MXFP4) {
-        if (out_dtype == PA_F32) PA_GO(PA_MXFP4, float);
-        if (out_dtype == PA_BF16) PA_GO(PA_MXFP4, __nv_bfloat16);
-        PA_GO(PA_MXFP4, __half);
-    }
-    if (out_dtype == PA_F32) PA_GO(PA_NVFP4, float);
-    if (out_dtype == PA_BF16) PA_GO(PA_NVFP4, __nv_bfloat16);
-    PA_GO(PA_NVFP4, __half);
-#undef PA_GO
+    return method == PA_MXFP4
+               ? fp4::project_method<PA_MXFP4>(args, query_codes, codes, s)
+               : fp4::project_method<PA_NVFP4>(args, query_codes, codes, s);
 }

@@ -17,6 +17,7 @@
 // the tile before while the next is multiplied (two accumulators in TMEM).  Every wait is
 // bounded.
 #include "grouped.cuh"
+#include "segments.cuh"
 #include "tc05.cuh"
 #include "tmap.cuh"
 
@@ -54,28 +55,6 @@ struct Tile {
     int64_t out_row;  // row of the result that column 0 is
 };
 
-// inclusive prefix over the CTA's threads (all call it): maximum or sum; *all is over all of them
-template <bool MAX>
-__device__ __forceinline__ int cta_scan(int v, int *warp_part_s, int *all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v = MAX ? max(v, y) : v + y;
-    }
-    if (lane == 31) warp_part_s[warp] = v;
-    __syncthreads();
-    int before = 0, total = 0;  // the values are not negative
-    for (int w = 0; w < mma::THREADS / 32; ++w) {
-        const int p = warp_part_s[w];
-        if (w < warp) before = MAX ? max(before, p) : before + p;
-        total = MAX ? max(total, p) : total + p;
-    }
-    __syncthreads();
-    *all = total;
-    return MAX ? max(before, v) : before + v;
-}
-
 template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(mma::THREADS, 1)
 mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
@@ -90,9 +69,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         quit_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_s;
-    __shared__ int edge_s[PA_MAX_GROUPS + 3];
-    __shared__ int tiles_s[PA_MAX_GROUPS + 3];  // row tiles before segment i
-    __shared__ int warp_part_s[THREADS / 32];
+    __shared__ Segments segs;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
 
@@ -112,28 +89,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         tc05::tma_prefetch_desc(&map_b);
     }
     if (warp == 0) tc05::tmem_alloc(tc05::smem_u32(&tmem_slot), COLS);
-    // segments, made to ascend, and the tiles before each
-    const int segs = sh.n_groups + 2;
-    int carry = 0;
-    for (int i0 = 0; i0 <= segs; i0 += THREADS) {
-        const int i = i0 + tid;
-        const int e = i <= segs ? static_cast<int>(edge(offsets, sh.n_groups, sh.rows, i)) : 0;
-        int all;
-        const int v = cta_scan<true>(e, warp_part_s, &all);
-        if (i <= segs) edge_s[i] = max(carry, v);
-        carry = max(carry, all);
-    }
-    __syncthreads();
-    carry = 0;
-    for (int i0 = 0; i0 < segs; i0 += THREADS) {
-        const int i = i0 + tid;
-        const int own = i < segs ? (static_cast<unsigned>(edge_s[i + 1] - edge_s[i]) + BN - 1) / BN : 0;
-        int all;
-        const int v = cta_scan<false>(own, warp_part_s, &all);
-        if (i < segs) tiles_s[i] = carry + v - own;
-        carry += all;
-    }
-    if (tid == 0) tiles_s[segs] = carry;
+    segs_make<THREADS>(segs, offsets, sh.n_groups, sh.rows, BN);
     tc05::fence_before_sync();
     __syncthreads();
     tc05::fence_after_sync();
@@ -143,7 +99,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     const int c_tiles = (sh.c_size + BN - 1) / BN;
     const int64_t n_tiles = MODE == MATRICES
                                 ? static_cast<int64_t>(sh.n_groups) * c_tiles * m_tiles
-                                : static_cast<int64_t>(tiles_s[segs]) * m_tiles;
+                                : static_cast<int64_t>(segs.tiles[sh.n_groups + 2]) * m_tiles;
     auto tile_at = [&](int64_t t) {
         Tile r;
         const int row = static_cast<int>(t / m_tiles);
@@ -152,18 +108,14 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             r.g = row / c_tiles;
             r.c0 = (row - r.g * c_tiles) * BN;
             r.c_end = sh.c_size;
-            r.t0 = edge_s[r.g + 1];
-            r.t_end = max(r.t0, edge_s[r.g + 2]);
+            r.t0 = segs.edge[r.g + 1];
+            r.t_end = max(r.t0, segs.edge[r.g + 2]);
             r.out_row = static_cast<int64_t>(r.g) * sh.c_size + r.c0;
         } else {
-            int lo = 0, hi = segs;  // the segment with tiles_s[lo] <= row < tiles_s[lo + 1]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (tiles_s[mid] <= row) lo = mid; else hi = mid;
-            }
+            const int lo = segs_find(segs, sh.n_groups, row);
             r.g = lo >= 1 && lo <= sh.n_groups ? lo - 1 : -1;
-            r.c0 = edge_s[lo] + (row - tiles_s[lo]) * BN;
-            r.c_end = edge_s[lo + 1];
+            r.c0 = segs.edge[lo] + (row - segs.tiles[lo]) * BN;
+            r.c_end = segs.edge[lo + 1];
             r.t0 = 0;
             r.t_end = r.g >= 0 ? sh.t_size : 0;
             r.out_row = r.c0;

@@ -1,0 +1,81 @@
+// Tiles of the rows of each group, worked out by every CTA of a persistent kernel from the
+// offsets on the device.
+#pragma once
+
+#include "grouped.cuh"
+
+namespace pa {
+namespace grouped {
+
+struct Segments {
+    int edge[PA_MAX_GROUPS + 3];   // first row of segment i, ascending
+    int tiles[PA_MAX_GROUPS + 3];  // row tiles before segment i
+    int part[32];                  // of the prefix sums
+};
+
+// inclusive prefix over the CTA's threads (all call it): maximum or sum; *all is over all of them
+template <int THREADS, bool MAX>
+__device__ __forceinline__ int cta_scan(int v, int *warp_part_s, int *all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = MAX ? max(v, y) : v + y;
+    }
+    if (lane == 31) warp_part_s[warp] = v;
+    __syncthreads();
+    int before = 0, total = 0;  // the values are not negative
+    for (int w = 0; w < THREADS / 32; ++w) {
+        const int p = warp_part_s[w];
+        if (w < warp) before = MAX ? max(before, p) : before + p;
+        total = MAX ? max(total, p) : total + p;
+    }
+    __syncthreads();
+    *all = total;
+    return MAX ? max(before, v) : before + v;
+}
+
+// All threads of the CTA; a barrier is still needed behind it.  offsets == nullptr: one group that
+// has all rows.
+template <int THREADS>
+__device__ __forceinline__ void segs_make(Segments &s, const int64_t *offsets, int n_groups,
+                                          int rows, int tile_rows) {
+    const int segs = n_groups + 2;
+    int carry = 0;
+    for (int i0 = 0; i0 <= segs; i0 += THREADS) {  // edges, made to ascend
+        const int i = i0 + threadIdx.x;
+        int e = 0;
+        if (i <= segs)
+            e = offsets ? static_cast<int>(edge(offsets, n_groups, rows, i)) : (i <= 1 ? 0 : rows);
+        int all;
+        const int v = cta_scan<THREADS, true>(e, s.part, &all);
+        if (i <= segs) s.edge[i] = max(carry, v);
+        carry = max(carry, all);
+    }
+    __syncthreads();
+    carry = 0;
+    for (int i0 = 0; i0 < segs; i0 += THREADS) {
+        const int i = i0 + threadIdx.x;
+        const int own =
+            i < segs ? (static_cast<unsigned>(s.edge[i + 1] - s.edge[i]) + tile_rows - 1) / tile_rows
+                     : 0;
+        int all;
+        const int v = cta_scan<THREADS, false>(own, s.part, &all);
+        if (i < segs) s.tiles[i] = carry + v - own;
+        carry += all;
+    }
+    if (threadIdx.x == 0) s.tiles[segs] = carry;
+}
+
+// the segment that has row tile `tile`
+__device__ __forceinline__ int segs_find(const Segments &s, int n_groups, int tile) {
+    int lo = 0, hi = n_groups + 2;  // tiles[lo] <= tile < tiles[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s.tiles[mid] <= tile) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+}  // namespace grouped
+}  // namespace pa

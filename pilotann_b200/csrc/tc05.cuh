@@ -124,6 +124,21 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t c
     d |= static_cast<uint64_t>(2) << 61;
     return d;
 }
+// 32 rows of 16 bytes, no swizzle: 8-row groups 128 bytes apart (for tcgen05.cp of block scales)
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
+}
+// kind::mxf4 and kind::mxf4nvf4, both operands E2M1 and K-major, tile 128 x N, K = 64; `id`: which
+// byte of a 4-byte scale word the step starts at (same for A and B)
+__host__ __device__ constexpr uint32_t idesc_mxf4(bool e8m0, int N, uint32_t id) {
+    return (id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+           ((e8m0 ? 1u : 0u) << 23) | (1u << 27) | (id << 29);
+}
 // kind::f16, fp32 accumulate; bf16 or fp16 operands, MN-major where said
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn, int M, int N) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
@@ -159,6 +174,37 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t desc_a, uint64
         "}\n" ::"r"(tmem_d),
         "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+// D[tmem] (+)= (A * scales)[128 x 64] (B * scales)^T; E8M0 per 32 values or E4M3 per 16
+template <bool E8M0>
+__device__ __forceinline__ void mma_fp4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                        uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb,
+                                        uint32_t accumulate) {
+    if (E8M0)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+            "[%5], p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, "
+            "[%4], [%5], p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+}
+// 32 rows x 16 bytes of shared memory to four TMEM columns, the same for each warp's 32 lanes
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
 }
 // The mbarrier gets one arrival when all MMAs issued so far by this thread finish.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
