@@ -42,15 +42,6 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
     return r;
 }
 
-// what a code (0..15) stands for: magnitude 0, 0.5, 1, 1.5, then (2 + m) 2^(e - 1)
-__device__ __forceinline__ float code_value(uint32_t code) {
-    const uint32_t m = code & 7u;
-    // exponent and mantissa bits moved to fp32's place are 2^-126 of the value, the smallest
-    // of them subnormal: one exact product brings both forms up
-    const float v = __uint_as_float(m << 22) * __uint_as_float(253u << 23);
-    return code & 8u ? -v : v;
-}
-
 __device__ __forceinline__ uint8_t e4m3_of(float v) {  // nearest even; callers keep v <= 448
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(v));

@@ -47,19 +47,24 @@ def _contiguous(name: str, x: torch.Tensor) -> None:
         raise RuntimeError(f"{name} custom kernel requires contiguous tensor")
 
 
-def _same_device(a: torch.Tensor, **others) -> None:
-    for name, x in others.items():
-        if x.device != a.device:
-            raise RuntimeError(f"{name} must be on {a.device}, got {x.device}")
+def _same_device(a: torch.Tensor, name: str, x: torch.Tensor) -> None:
+    if x.device != a.device:
+        raise RuntimeError(f"{name} must be on {a.device}, got {x.device}")
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream     # a number, without a Stream object around it
 
 
 def _call(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on the tensors' device and its current stream."""
-    if torch.cuda.current_device() == device.index:
-        _C.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _C.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _C.check(rc)
 
 
 # ---- rows by group -----------------------------------------------------------------
@@ -90,7 +95,8 @@ def _grouped_checks(query, VT, offsets) -> None:
     _check("offsets", offsets, 1, (torch.int64,))
     _contiguous("VT", VT)
     _contiguous("offsets", offsets)
-    _same_device(query, VT=VT, offsets=offsets)
+    _same_device(query, "VT", VT)
+    _same_device(query, "offsets", offsets)
     _require(VT.size(2) == query.size(1), "VT.size(2) == query.size(1)")
     _require(1 <= VT.size(0) <= MAX_GROUPS, f"1 <= VT.size(0) <= {MAX_GROUPS}")
     _require(offsets.size(0) == VT.size(0) + 1, "offsets.size(0) == VT.size(0) + 1")
@@ -128,8 +134,9 @@ class _ProjectGrouped(torch.autograd.Function):
         return _grouped_forward(query, VT, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        if torch.is_grad_enabled():       # create_graph: the gradients have none themselves
+            raise RuntimeError("project_grouped can be differentiated only once")
         query, VT, offsets = ctx.saved_tensors
         if not grad.is_contiguous() and (grad.stride(1) != 1 or grad.stride(0) < grad.size(1)):
             grad = grad.contiguous()      # an expanded gradient, as of a sum
@@ -170,7 +177,7 @@ def project_grouped_backward(grad: torch.Tensor, query: torch.Tensor, VT: torch.
     ``grad_VT[g] = grad[g's rows].T @ query[g's rows]`` (zeros for a group without rows)."""
     _grouped_checks(query, VT, offsets)
     _check("grad", grad, 2, (query.dtype,))
-    _same_device(query, grad=grad)
+    _same_device(query, "grad", grad)
     _require(tuple(grad.shape) == (query.size(0), VT.size(1)), "grad.shape == (rows, d_out)")
     return _grouped_backward(grad, query, VT, offsets, want_query, want_VT)
 
@@ -206,8 +213,8 @@ class Fp4Table:
             _check("row_scale", row_scale, dim - 1, (torch.float32,))
             _contiguous("row_scale", row_scale)
             _require(row_scale.shape == codes.shape[:-1], "row_scale.shape == codes.shape[:-1]")
-            _same_device(codes, row_scale=row_scale)
-        _same_device(codes, scales=scales)
+            _same_device(codes, "row_scale", row_scale)
+        _same_device(codes, "scales", scales)
         _require(codes.data_ptr() % 16 == 0, "codes 16-byte aligned")
         self.codes, self.scales, self.row_scale = codes, scales, row_scale
         self.d, self.method = d, method
@@ -244,7 +251,7 @@ def quantize_fp4(x: torch.Tensor, method: str = "mxfp4") -> Fp4Table:
         _contiguous("x", x)
     ld = d if dim == 3 else _row_stride("x", x)
     lead, dev = x.shape[:-1], x.device
-    rows = lead.numel()
+    rows = x.size(0) if dim == 2 else x.size(0) * x.size(1)
     padded = -(-d // 32) * 32
     codes = torch.empty(*lead, padded // 2, dtype=torch.uint8, device=dev)
     scales = torch.empty(*lead, padded // _BLOCK[method], dtype=torch.uint8, device=dev)
@@ -252,7 +259,10 @@ def quantize_fp4(x: torch.Tensor, method: str = "mxfp4") -> Fp4Table:
     _call(dev, _C.lib().pa_quantize_fp4, codes.data_ptr(), scales.data_ptr(),
           0 if row_scale is None else row_scale.data_ptr(), x.data_ptr(), rows, d, ld,
           _DTYPE[x.dtype], _METHOD[method])
-    return Fp4Table(codes, scales, row_scale, d, method)
+    table = Fp4Table.__new__(Fp4Table)       # parts made here need no checks
+    table.codes, table.scales, table.row_scale = codes, scales, row_scale
+    table.d, table.method = d, method
+    return table
 
 
 def dequantize_fp4(table: Fp4Table) -> torch.Tensor:
@@ -286,7 +296,7 @@ def project_fp4(query, table: Fp4Table, offsets: torch.Tensor | None = None,
         _require(codes.dim() == 3, "table of [n_groups, d_out, d] with offsets")
         _check("offsets", offsets, 1, (torch.int64,))
         _contiguous("offsets", offsets)
-        _same_device(codes, offsets=offsets)
+        _same_device(codes, "offsets", offsets)
         n_groups, d_out = codes.size(0), codes.size(1)
         _require(1 <= n_groups <= MAX_GROUPS, f"1 <= n_groups <= {MAX_GROUPS}")
         _require(offsets.size(0) == n_groups + 1, "offsets.size(0) == n_groups + 1")
@@ -296,14 +306,14 @@ def project_fp4(query, table: Fp4Table, offsets: torch.Tensor | None = None,
         _require(query.codes.dim() == 2, "query of [rows, d]")
         _require(query.method == method, "query.method == table.method")
         _require(query.d == d, "query.size(1) == table.d")
-        _same_device(codes, query=query.codes)
+        _same_device(codes, "query", query.codes)
         rows = query.codes.size(0)
         q = (query.codes.data_ptr(), query.scales.data_ptr(),
              0 if query.row_scale is None else query.row_scale.data_ptr())
     else:
         _check("query", query, 2, tuple(_DTYPE))
         _require(query.size(1) == d, "query.size(1) == table.d")
-        _same_device(codes, query=query)
+        _same_device(codes, "query", query)
         rows = query.size(0)
         ld = _row_stride("query", query)
         # scratch: codes, row scales, block scales of the quantised queries

@@ -289,6 +289,15 @@ def test_gradient_of_a_sum_is_expanded():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = torch.randn(20, 24, device="cuda", requires_grad=True)
+    w = torch.randn(2, 8, 24, device="cuda", requires_grad=True)
+    y = ext().project_grouped(x, w, torch.tensor([0, 5, 20], device="cuda"))
+    with pytest.raises(RuntimeError, match="only once"):
+        torch.autograd.grad(y.square().sum(), x, create_graph=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [[0, 40, 20, 64], [-5, 10, 20, 1000], [64, 32, 16, 0],
                                  [1 << 62, -(1 << 62), 7, 1 << 40]])
 @pytest.mark.parametrize("dtype", [F32, BF16])
