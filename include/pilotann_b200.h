@@ -349,17 +349,27 @@ int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *router, int64
 /* out[i, :] = VT[g] query[i, :] for offsets[g] <= i < offsets[g + 1]; query [rows, d]
  * with row stride ld_query, VT [n_groups, d_out, d], out [rows, d_out] with row
  * stride ld_out.  fp32 sums.  Rows of no group become zeros.  offsets are clamped to
- * [0, rows]; if they do not ascend the result is unspecified, the accesses are not. */
+ * [0, rows]; if they do not ascend the result is unspecified, the accesses are not.
+ * workspace: 16-byte aligned, of the bytes that the first call says for the same
+ * operands (0 where their rows start on 16 bytes, then NULL will do). */
+int64_t pa_project_grouped_workspace_bytes(const void *query, const void *VT, int64_t rows,
+                                           int n_groups, int d, int d_out, int64_t ld_query,
+                                           int dtype);
 int pa_project_grouped(void *out, const void *query, const void *VT, const int64_t *offsets,
                        int64_t rows, int n_groups, int d, int d_out, int64_t ld_query,
-                       int64_t ld_out, int dtype, void *stream);
+                       int64_t ld_out, int dtype, void *workspace, void *stream);
 /* Gradients: grad_query[i, :] = VT[g]^T grad[i, :], grad_VT[g] = sum of grad[i, :]
  * query[i, :]^T over the rows of g (zeros without rows).  Either may be NULL. */
+int64_t pa_project_grouped_backward_workspace_bytes(const void *grad, const void *query,
+                                                    const void *VT, int64_t rows, int n_groups,
+                                                    int d, int d_out, int64_t ld_grad,
+                                                    int64_t ld_query, int dtype, int want_query,
+                                                    int want_VT);
 int pa_project_grouped_backward(void *grad_query, void *grad_VT, const void *grad,
                                 const void *query, const void *VT, const int64_t *offsets,
                                 int64_t rows, int n_groups, int d, int d_out, int64_t ld_grad,
                                 int64_t ld_query, int64_t ld_grad_query, int dtype,
-                                void *stream);
+                                void *workspace, void *stream);
 
 /* Rows of d values to 4-bit blocks.  P = d rounded up to a multiple of 32; codes
  * [rows, P / 2] (E2M1, even value in the low half, zero codes behind d; 16-byte

@@ -26,7 +26,8 @@ SYMBOLS = (
     "pa_pack_fullgraph", "pa_refine", "pa_stage_attach_refine", "pa_stage_search_ex",
     "pa_stage_search_device_ex", "pa_stage_slot_rows", "pa_stage_submit", "pa_stage_wait",
     "pa_group_rows_workspace_bytes", "pa_group_rows", "pa_project_grouped",
-    "pa_project_grouped_backward", "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4",
+    "pa_project_grouped_backward", "pa_project_grouped_workspace_bytes",
+    "pa_project_grouped_backward_workspace_bytes", "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4",
 )
 
 PA_OUT_HANDOFF, PA_OUT_STAGE2, PA_OUT_TOPK = 0, 1, 2
@@ -125,9 +126,15 @@ def lib() -> ctypes.CDLL:
     L.pa_group_rows_workspace_bytes.restype = c_int64
     L.pa_group_rows.argtypes = [P, P, P, c_int64, c_int, P, P]
     L.pa_project_grouped.argtypes = [P, P, P, P, c_int64, c_int, c_int, c_int, c_int64, c_int64,
-                                     c_int, P]
+                                     c_int, P, P]
     L.pa_project_grouped_backward.argtypes = [P, P, P, P, P, P, c_int64, c_int, c_int, c_int,
-                                              c_int64, c_int64, c_int64, c_int, P]
+                                              c_int64, c_int64, c_int64, c_int, P, P]
+    L.pa_project_grouped_workspace_bytes.argtypes = [P, P, c_int64, c_int, c_int, c_int, c_int64,
+                                                     c_int]
+    L.pa_project_grouped_workspace_bytes.restype = c_int64
+    L.pa_project_grouped_backward_workspace_bytes.argtypes = [
+        P, P, P, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int, c_int, c_int]
+    L.pa_project_grouped_backward_workspace_bytes.restype = c_int64
     L.pa_quantize_fp4.argtypes = [P, P, P, P, c_int64, c_int, c_int64, c_int, c_int, P]
     L.pa_dequantize_fp4.argtypes = [P, P, P, P, c_int64, c_int, c_int, P]
     L.pa_project_fp4.argtypes = [P, P, P, P, P, P, P, P, c_int64, c_int, c_int, c_int64, c_int,

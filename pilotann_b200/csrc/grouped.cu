@@ -120,46 +120,106 @@ matrices_kernel(T *__restrict__ dw, const T *__restrict__ dy, const T *__restric
         }
 }
 
-// rows of 16-bit values that a bulk-tensor copy can start at
-bool ldi_ok(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+// ---- 16-bit operands that a bulk-tensor copy cannot read --------------------------
+// Rows that do not start on 16 bytes (an odd width, a slice of a wider tensor) are copied into
+// the workspace with a pitch of whole 16 bytes first; the products then run on that.  A copy
+// reads and writes the operand once (of the matrices only those whose group has rows), which the
+// tensor cores win back many times over plain loads: 4099 rows x 13 matrices of 333 x 200, all
+// gradients, 178 us with the 64 x 64 tiles above.
+constexpr int kCopyRows = 32;  // per CTA
 
-template <typename T>
-int rows_launch(void *out, const void *x, const void *w, const int64_t *offsets, int64_t rows,
-                int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
-                cudaStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        const int64_t ldw = transposed ? d_out : d_sum;
-        if (ldi_ok(x, ldx) && ldi_ok(w, ldw))
-            return rows_mma<T>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo,
-                               transposed, s);
+__global__ void __launch_bounds__(256)
+repitch_kernel(uint4 *__restrict__ out, const uint16_t *__restrict__ in, int64_t rows, int width,
+               int64_t ld, const int64_t *__restrict__ offsets, int n_groups, int64_t n_rows) {
+    const int pieces = (width + 7) / 8, g = blockIdx.y;
+    if (offsets && edge(offsets, n_groups, n_rows, g + 1) >= edge(offsets, n_groups, n_rows, g + 2))
+        return;
+    out += g * rows * pieces;
+    in += g * rows * ld;
+    const int64_t r0 = blockIdx.x * static_cast<int64_t>(kCopyRows);
+    const int n = static_cast<int>(min(static_cast<int64_t>(kCopyRows), rows - r0)) * pieces;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int r = i / pieces, p = i - r * pieces;
+        const uint16_t *src = in + (r0 + r) * ld + 8 * p;
+        // aligned words that hold one of the piece's values, shifted by half a word if need be
+        const uint32_t half = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src) >> 1) & 1u;
+        const uint32_t *base = reinterpret_cast<const uint32_t *>(src - half);
+        const int have = min(8, width - 8 * p) + half;  // 16-bit values from base on
+        uint32_t w[5];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) w[j] = 2 * j < have ? __ldg(base + j) : 0u;
+        uint4 v;
+        v.x = __funnelshift_r(w[0], w[1], 16 * half);
+        v.y = __funnelshift_r(w[1], w[2], 16 * half);
+        v.z = __funnelshift_r(w[2], w[3], 16 * half);
+        v.w = __funnelshift_r(w[3], w[4], 16 * half);
+        out[(r0 + r) * pieces + p] = v;
     }
-    dim3 grid(static_cast<unsigned>(rows / kT + n_groups + 2),
-              static_cast<unsigned>((d_out + kT - 1) / kT));
-    if (transposed)
-        rows_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<T *>(out), static_cast<const T *>(x),
-                                                   static_cast<const T *>(w), offsets, rows,
-                                                   n_groups, d_sum, d_out, ldx, ldo);
-    else
-        rows_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<T *>(out), static_cast<const T *>(x),
-                                                  static_cast<const T *>(w), offsets, rows,
-                                                  n_groups, d_sum, d_out, ldx, ldo);
+}
+
+int64_t pitched(int width) { return (width + 7) / 8 * 8; }
+
+// rows of 16-bit values that a bulk-tensor copy can start at
+bool rows_ok(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+int64_t copy_bytes(const void *p, int64_t rows, int width, int64_t ld) {
+    return rows_ok(p, ld) ? 0 : rows * pitched(width) * 2;
+}
+
+int repitch(uint8_t *to, const void *p, int64_t ld, int64_t rows, int width, int n_groups,
+            const int64_t *offsets, int64_t n_rows, cudaStream_t s) {
+    dim3 grid(static_cast<unsigned>((rows + kCopyRows - 1) / kCopyRows),
+              static_cast<unsigned>(n_groups));
+    repitch_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<uint4 *>(to),
+                                        static_cast<const uint16_t *>(p), rows, width, ld, offsets,
+                                        n_groups, n_rows);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
 }
 
-template <typename T>
-int matrices_launch(void *dw, const void *dy, const void *x, const int64_t *offsets, int64_t rows,
-                    int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        if (rows > 0 && ldi_ok(dy, ldy) && ldi_ok(x, ldx))
-            return matrices_mma<T>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
-    }
+// *p and *ld on exit: the operand itself, or its copy, with *ws moved behind it
+int rows_make_ok(const void **p, int64_t *ld, int64_t rows, int width, uint8_t **ws,
+                 cudaStream_t s) {
+    if (rows_ok(*p, *ld)) return PA_OK;
+    int rc = repitch(*ws, *p, *ld, rows, width, 1, nullptr, 0, s);
+    *p = *ws;
+    *ld = pitched(width);
+    *ws += rows * pitched(width) * 2;
+    return rc;
+}
+
+int matrices_make_ok(const void **w, int64_t *ld, int n_groups, int d, int d_out,
+                     const int64_t *offsets, int64_t n_rows, uint8_t **ws, cudaStream_t s) {
+    if (rows_ok(*w, *ld)) return PA_OK;
+    int rc = repitch(*ws, *w, *ld, d_out, d, n_groups, offsets, n_rows, s);
+    *w = *ws;
+    *ld = pitched(d);
+    *ws += static_cast<int64_t>(n_groups) * d_out * pitched(d) * 2;
+    return rc;
+}
+
+int rows_f32(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
+             int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
+             cudaStream_t s) {
+    dim3 grid(static_cast<unsigned>(rows / kT + n_groups + 2),
+              static_cast<unsigned>((d_out + kT - 1) / kT));
+    if (transposed)
+        rows_kernel<float, false><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
+                                                       d_out, ldx, ldo);
+    else
+        rows_kernel<float, true><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
+                                                      d_out, ldx, ldo);
+    count_launch();
+    PA_CUDA_TRY(cudaGetLastError());
+    return PA_OK;
+}
+
+int matrices_f32(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
+                 int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
     dim3 grid(static_cast<unsigned>((d + kT - 1) / kT), static_cast<unsigned>((d_out + kT - 1) / kT),
               static_cast<unsigned>(n_groups));
-    matrices_kernel<T><<<grid, 256, 0, s>>>(static_cast<T *>(dw), static_cast<const T *>(dy),
-                                            static_cast<const T *>(x), offsets, rows, n_groups, d,
-                                            d_out, ldy, ldx);
+    matrices_kernel<float><<<grid, 256, 0, s>>>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy,
+                                                ldx);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
@@ -175,65 +235,123 @@ int check(int64_t rows, int n_groups, int d, int d_out, int dtype) {
     return PA_OK;
 }
 
-int project_rows(void *out, const void *in, const void *w, const int64_t *offsets, int64_t rows,
-                 int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo, int dtype,
-                 bool transposed, cudaStream_t s) {
-    if (dtype == PA_F32)
-        return rows_launch<float>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
-                                  transposed, s);
+// forward, or with `transposed` the gradient of the rows, of 16-bit values
+int rows_16(void *out, const void *in, int64_t ldi, const void *w, int64_t ldw,
+            const int64_t *offsets, int64_t rows, int n_groups, int d_sum, int d_out, int64_t ldo,
+            int dtype, bool transposed, cudaStream_t s) {
     if (dtype == PA_BF16)
-        return rows_launch<__nv_bfloat16>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi,
-                                          ldo, transposed, s);
-    return rows_launch<__half>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
-                               transposed, s);
+        return rows_mma<__nv_bfloat16>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
+                                       ldo, transposed, s);
+    return rows_mma<__half>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldw, ldo,
+                            transposed, s);
 }
 
 }  // namespace grouped
 }  // namespace pa
 
+extern "C" int64_t pa_project_grouped_workspace_bytes(const void *query, const void *VT,
+                                                      int64_t rows, int n_groups, int d, int d_out,
+                                                      int64_t ld_query, int dtype) {
+    using namespace pa::grouped;
+    if (dtype == PA_F32) return 0;
+    return copy_bytes(query, rows, d, ld_query) +
+           copy_bytes(VT, static_cast<int64_t>(n_groups) * d_out, d, d);
+}
+
 extern "C" int pa_project_grouped(void *out, const void *query, const void *VT,
                                   const int64_t *offsets, int64_t rows, int n_groups, int d,
                                   int d_out, int64_t ld_query, int64_t ld_out, int dtype,
-                                  void *stream) {
+                                  void *workspace, void *stream) {
     using namespace pa;
     int rc = grouped::check(rows, n_groups, d, d_out, dtype);
     if (rc != PA_OK) return rc;
     PA_REQUIRE(ld_query >= d && ld_out >= d_out, "row strides must cover the rows");
     if (rows == 0) return PA_OK;
     PA_REQUIRE(out && query && VT && offsets, "null pointer");
-    return grouped::project_rows(out, query, VT, offsets, rows, n_groups, d, d_out, ld_query,
-                                 ld_out, dtype, false, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == PA_F32)
+        return grouped::rows_f32(static_cast<float *>(out), static_cast<const float *>(query),
+                                 static_cast<const float *>(VT), offsets, rows, n_groups, d, d_out,
+                                 ld_query, ld_out, false, s);
+    PA_REQUIRE(workspace || !pa_project_grouped_workspace_bytes(query, VT, rows, n_groups, d, d_out,
+                                                               ld_query, dtype),
+               "workspace missing (pa_project_grouped_workspace_bytes)");
+    PA_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    int64_t ldw = d;
+    rc = grouped::rows_make_ok(&query, &ld_query, rows, d, &ws, s);
+    if (rc != PA_OK) return rc;
+    rc = grouped::matrices_make_ok(&VT, &ldw, n_groups, d, d_out, offsets, rows, &ws, s);
+    if (rc != PA_OK) return rc;
+    return grouped::rows_16(out, query, ld_query, VT, ldw, offsets, rows, n_groups, d, d_out,
+                            ld_out, dtype, false, s);
+}
+
+extern "C" int64_t pa_project_grouped_backward_workspace_bytes(
+    const void *grad, const void *query, const void *VT, int64_t rows, int n_groups, int d,
+    int d_out, int64_t ld_grad, int64_t ld_query, int dtype, int want_query, int want_VT) {
+    using namespace pa::grouped;
+    if (dtype == PA_F32) return 0;
+    return copy_bytes(grad, rows, d_out, ld_grad) +
+           (want_query ? copy_bytes(VT, static_cast<int64_t>(n_groups) * d_out, d, d) : 0) +
+           (want_VT ? copy_bytes(query, rows, d, ld_query) : 0);
 }
 
 extern "C" int pa_project_grouped_backward(void *grad_query, void *grad_VT, const void *grad,
                                            const void *query, const void *VT,
                                            const int64_t *offsets, int64_t rows, int n_groups,
                                            int d, int d_out, int64_t ld_grad, int64_t ld_query,
-                                           int64_t ld_grad_query, int dtype, void *stream) {
+                                           int64_t ld_grad_query, int dtype, void *workspace,
+                                           void *stream) {
     using namespace pa;
     int rc = grouped::check(rows, n_groups, d, d_out, dtype);
     if (rc != PA_OK) return rc;
     PA_REQUIRE(ld_grad >= d_out, "row strides must cover the rows");
     PA_REQUIRE(!grad_query || ld_grad_query >= d, "row strides must cover the rows");
     PA_REQUIRE(!grad_VT || ld_query >= d, "row strides must cover the rows");
+    if (!grad_query && !grad_VT) return PA_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (grad_query && rows > 0) {
-        PA_REQUIRE(grad && VT && offsets, "null pointer");
-        rc = grouped::project_rows(grad_query, grad, VT, offsets, rows, n_groups, d_out, d, ld_grad,
-                                   ld_grad_query, dtype, true, s);
-        if (rc != PA_OK) return rc;
+    if (rows == 0) {  // no products: the matrices' gradients are zero
+        if (grad_VT)
+            PA_CUDA_TRY(cudaMemsetAsync(grad_VT, 0, static_cast<size_t>(n_groups) * d_out * d *
+                                                        (dtype == PA_F32 ? 4 : 2), s));
+        return PA_OK;
     }
-    if (grad_VT) {
-        PA_REQUIRE(offsets && (rows == 0 || (grad && query)), "null pointer");
-        if (dtype == PA_F32)
-            rc = grouped::matrices_launch<float>(grad_VT, grad, query, offsets, rows, n_groups, d,
-                                                 d_out, ld_grad, ld_query, s);
-        else if (dtype == PA_BF16)
-            rc = grouped::matrices_launch<__nv_bfloat16>(grad_VT, grad, query, offsets, rows,
-                                                         n_groups, d, d_out, ld_grad, ld_query, s);
-        else
-            rc = grouped::matrices_launch<__half>(grad_VT, grad, query, offsets, rows, n_groups, d,
-                                                  d_out, ld_grad, ld_query, s);
+    PA_REQUIRE(grad && offsets && (!grad_query || VT) && (!grad_VT || query), "null pointer");
+    if (dtype == PA_F32) {
+        const float *dy = static_cast<const float *>(grad);
+        if (grad_query)
+            rc = grouped::rows_f32(static_cast<float *>(grad_query), dy,
+                                   static_cast<const float *>(VT), offsets, rows, n_groups, d_out,
+                                   d, ld_grad, ld_grad_query, true, s);
+        if (rc == PA_OK && grad_VT)
+            rc = grouped::matrices_f32(static_cast<float *>(grad_VT), dy,
+                                       static_cast<const float *>(query), offsets, rows, n_groups,
+                                       d, d_out, ld_grad, ld_query, s);
+        return rc;
+    }
+    PA_REQUIRE(workspace || !pa_project_grouped_backward_workspace_bytes(
+                                grad, query, VT, rows, n_groups, d, d_out, ld_grad, ld_query, dtype,
+                                grad_query != nullptr, grad_VT != nullptr),
+               "workspace missing (pa_project_grouped_backward_workspace_bytes)");
+    PA_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    rc = grouped::rows_make_ok(&grad, &ld_grad, rows, d_out, &ws, s);
+    if (rc == PA_OK && grad_query) {
+        int64_t ldw = d;
+        rc = grouped::matrices_make_ok(&VT, &ldw, n_groups, d, d_out, offsets, rows, &ws, s);
+        if (rc == PA_OK)
+            rc = grouped::rows_16(grad_query, grad, ld_grad, VT, ldw, offsets, rows, n_groups,
+                                  d_out, d, ld_grad_query, dtype, true, s);
+    }
+    if (rc == PA_OK && grad_VT) {
+        rc = grouped::rows_make_ok(&query, &ld_query, rows, d, &ws, s);
+        if (rc == PA_OK)
+            rc = dtype == PA_BF16
+                     ? grouped::matrices_mma<__nv_bfloat16>(grad_VT, grad, query, offsets, rows,
+                                                            n_groups, d, d_out, ld_grad, ld_query, s)
+                     : grouped::matrices_mma<__half>(grad_VT, grad, query, offsets, rows, n_groups,
+                                                     d, d_out, ld_grad, ld_query, s);
     }
     return rc;
 }

@@ -35,7 +35,8 @@ __device__ __forceinline__ int64_t edge(const int64_t *offsets, int n_groups, in
 // grouped_mma.cu: 16-bit values on the tensor cores, rows on 16 bytes
 template <typename T>
 int rows_mma(void *out, const void *in, const void *w, const int64_t *offsets, int64_t rows,
-             int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo, bool transposed,
+             int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw, int64_t ldo,
+             bool transposed,
              cudaStream_t s);
 template <typename T>
 int matrices_mma(void *dw, const void *dy, const void *x, const int64_t *offsets, int64_t rows,

@@ -315,22 +315,22 @@ static int map_rows(CUtensorMap *map, const void *x, int64_t width, int64_t rows
 
 template <typename T>
 static int map_matrices(CUtensorMap *map, const void *w, int64_t d, int64_t d_out, int64_t n_groups,
-                        int box_rows) {
+                        int64_t ld, int box_rows) {
     const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(d_out),
                               static_cast<uint64_t>(n_groups)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(d) * 2, static_cast<uint64_t>(d) * d_out * 2};
+    const uint64_t strides[2] = {static_cast<uint64_t>(ld) * 2, static_cast<uint64_t>(ld) * d_out * 2};
     const uint32_t box[3] = {64, static_cast<uint32_t>(box_rows), 1};
     return tensor_map(map, map_type<T>(), w, 3, dims, strides, box);
 }
 
 template <typename T, int MODE, int BN>
 static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
-                       int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo,
-                       cudaStream_t s) {
+                       int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw,
+                       int64_t ldo, cudaStream_t s) {
     CUtensorMap a, b;
     const bool fwd = MODE == mma::FORWARD;
     int rc = map_matrices<T>(&a, w, fwd ? d_sum : d_out, fwd ? d_out : d_sum, n_groups,
-                             fwd ? 128 : 64);
+                             ldw, fwd ? 128 : 64);
     if (rc != PA_OK) return rc;
     rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN);
     if (rc != PA_OK) return rc;
@@ -341,11 +341,12 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
 
 template <typename T, int MODE>
 static int rows_mma_mode(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
-                         int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo,
-                         cudaStream_t s) {
+                         int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw,
+                         int64_t ldo, cudaStream_t s) {
     const int64_t each = (rows + n_groups - 1) / n_groups;  // on average
 #define PA_GO(BN) \
-    return rows_mma_bn<T, MODE, BN>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldo, s)
+    return rows_mma_bn<T, MODE, BN>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldw, ldo, \
+                                   s)
     if (each <= 16) PA_GO(16);
     if (each <= 32) PA_GO(32);
     if (each <= 64) PA_GO(64);
@@ -356,15 +357,16 @@ static int rows_mma_mode(T *out, const T *in, const T *w, const int64_t *offsets
 
 template <typename T>
 int rows_mma(void *out, const void *in, const void *w, const int64_t *offsets, int64_t rows,
-             int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldo, bool transposed,
+             int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw, int64_t ldo,
+             bool transposed,
              cudaStream_t s) {
     T *o = static_cast<T *>(out);
     const T *i = static_cast<const T *>(in), *m = static_cast<const T *>(w);
     if (transposed)
-        return rows_mma_mode<T, mma::ROWS>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
-                                           s);
-    return rows_mma_mode<T, mma::FORWARD>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldo,
-                                          s);
+        return rows_mma_mode<T, mma::ROWS>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
+                                           ldo, s);
+    return rows_mma_mode<T, mma::FORWARD>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
+                                          ldo, s);
 }
 
 template <typename T, int BN>
@@ -395,9 +397,9 @@ int matrices_mma(void *dw, const void *dy, const void *x, const int64_t *offsets
 }
 
 template int rows_mma<__half>(void *, const void *, const void *, const int64_t *, int64_t, int, int,
-                              int, int64_t, int64_t, bool, cudaStream_t);
+                              int, int64_t, int64_t, int64_t, bool, cudaStream_t);
 template int rows_mma<__nv_bfloat16>(void *, const void *, const void *, const int64_t *, int64_t,
-                                     int, int, int, int64_t, int64_t, bool, cudaStream_t);
+                                     int, int, int, int64_t, int64_t, int64_t, bool, cudaStream_t);
 template int matrices_mma<__half>(void *, const void *, const void *, const int64_t *, int64_t, int,
                                   int, int, int64_t, int64_t, cudaStream_t);
 template int matrices_mma<__nv_bfloat16>(void *, const void *, const void *, const int64_t *,

@@ -107,23 +107,32 @@ def _grouped_checks(query, VT, offsets) -> None:
 def _grouped_forward(query, VT, offsets):
     rows, d = query.shape
     n_groups, d_out, _ = VT.shape
-    out = torch.empty(rows, d_out, dtype=query.dtype, device=query.device)
-    _call(query.device, _C.lib().pa_project_grouped, out.data_ptr(), query.data_ptr(),
-          VT.data_ptr(), offsets.data_ptr(), rows, n_groups, d, d_out,
-          _row_stride("query", query), d_out, _DTYPE[query.dtype])
+    dev, dtype = query.device, _DTYPE[query.dtype]
+    L = _C.lib()
+    q, w, ld = query.data_ptr(), VT.data_ptr(), _row_stride("query", query)
+    need = L.pa_project_grouped_workspace_bytes(q, w, rows, n_groups, d, d_out, ld, dtype)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    out = torch.empty(rows, d_out, dtype=query.dtype, device=dev)
+    _call(dev, L.pa_project_grouped, out.data_ptr(), q, w, offsets.data_ptr(), rows, n_groups, d,
+          d_out, ld, d_out, dtype, 0 if ws is None else ws.data_ptr())
     return out
 
 
 def _grouped_backward(grad, query, VT, offsets, want_query, want_VT):
     rows, d = query.shape
     n_groups, d_out, _ = VT.shape
-    dev = query.device
+    dev, dtype = query.device, _DTYPE[query.dtype]
+    L = _C.lib()
+    y, q, w = grad.data_ptr(), query.data_ptr(), VT.data_ptr()
+    ldy, ldq = _row_stride("grad", grad), _row_stride("query", query)
+    need = L.pa_project_grouped_backward_workspace_bytes(y, q, w, rows, n_groups, d, d_out, ldy, ldq,
+                                                         dtype, want_query, want_VT)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     dq = torch.empty(rows, d, dtype=query.dtype, device=dev) if want_query else None
-    dw = torch.empty_like(VT) if want_VT else None
-    _call(dev, _C.lib().pa_project_grouped_backward, 0 if dq is None else dq.data_ptr(),
-          0 if dw is None else dw.data_ptr(), grad.data_ptr(), query.data_ptr(), VT.data_ptr(),
-          offsets.data_ptr(), rows, n_groups, d, d_out, _row_stride("grad", grad),
-          _row_stride("query", query), d, _DTYPE[query.dtype])
+    dw = torch.empty(n_groups, d_out, d, dtype=query.dtype, device=dev) if want_VT else None
+    _call(dev, L.pa_project_grouped_backward, 0 if dq is None else dq.data_ptr(),
+          0 if dw is None else dw.data_ptr(), y, q, w, offsets.data_ptr(), rows, n_groups, d, d_out,
+          ldy, ldq, d, dtype, 0 if ws is None else ws.data_ptr())
     return dq, dw
 
 

@@ -42,13 +42,13 @@ def test_c_entry_points_refuse_bad_arguments():
     refused(L.pa_group_rows(0, 0, 0, 1 << 31, 4, 0, 0), b"rows")
     refused(L.pa_group_rows(0, 0, 0, 4, 4, 0, 0), b"null")
     refused(L.pa_group_rows(16, 16, 16, 100000, 4, 0, 0), b"workspace")
-    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 0, 8, 8, 8, 0, 0), b"d_out")
-    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 65537, 8, 65537, 0, 0), b"d_out")
-    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 7, 8, 0, 0), b"strides")
-    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 3, 0), b"dtype")
-    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 0, 0), b"null")
-    refused(L.pa_project_grouped_backward(16, 0, 0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 7, 0, 0), b"strides")
-    refused(L.pa_project_grouped_backward(0, 16, 0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 8, 0, 0), b"null")
+    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 0, 8, 8, 8, 0, 0, 0), b"d_out")
+    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 65537, 8, 65537, 0, 0, 0), b"d_out")
+    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 7, 8, 0, 0, 0), b"strides")
+    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 3, 0, 0), b"dtype")
+    refused(L.pa_project_grouped(0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 0, 0, 0), b"null")
+    refused(L.pa_project_grouped_backward(16, 0, 0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 7, 0, 0, 0), b"strides")
+    refused(L.pa_project_grouped_backward(0, 16, 0, 0, 0, 0, 4, 2, 8, 8, 8, 8, 8, 0, 0, 0), b"null")
     refused(L.pa_quantize_fp4(0, 0, 0, 0, 4, 0, 8, 0, 0, 0), b"d must")
     refused(L.pa_quantize_fp4(0, 0, 0, 0, 4, 8, 4, 0, 0, 0), b"stride")
     refused(L.pa_quantize_fp4(0, 0, 0, 0, 4, 8, 8, 0, 2, 0), b"method")
@@ -58,6 +58,12 @@ def test_c_entry_points_refuse_bad_arguments():
     refused(L.pa_project_fp4(0, 0, 0, 0, 0, 0, 0, 0, 4, 1, 8, 1 << 31, 0, 0, 0), b"table rows")
     refused(L.pa_project_fp4(0, 0, 0, 0, 0, 0, 0, 0, 4, 1, 8, 8, 7, 0, 0), b"dtype")
     refused(L.pa_project_fp4(16, 16, 16, 0, 16, 16, 0, 0, 4, 1, 8, 8, 0, 1, 0), b"row scales")
+    refused(L.pa_project_grouped(16, 16, 16, 16, 4, 2, 9, 8, 9, 8, 1, 0, 0), b"workspace")
+    refused(L.pa_project_grouped_backward(16, 0, 16, 0, 16, 16, 4, 2, 8, 9, 9, 8, 8, 1, 0, 0),
+            b"workspace")
+    assert L.pa_project_grouped_workspace_bytes(16, 16, 4, 2, 8, 8, 8, 1) == 0
+    assert L.pa_project_grouped_workspace_bytes(18, 16, 4, 2, 8, 8, 8, 1) == 4 * 8 * 2
+    assert L.pa_project_grouped_workspace_bytes(16, 16, 4, 2, 9, 8, 9, 1) == (4 + 2 * 8) * 16 * 2
     assert L.pa_group_rows_workspace_bytes(8192, 64) == 0
     assert L.pa_group_rows_workspace_bytes(8193, 64) == 2 * 65 * 4
 
@@ -312,7 +318,7 @@ def test_offsets_that_do_not_ascend_stay_inside(bad, dtype):
     offsets = torch.tensor(bad, device="cuda")
     _C.check(_C.lib().pa_project_grouped(out.data_ptr() + 128 * d_out * out.element_size(),
                                          x.data_ptr(), w.data_ptr(), offsets.data_ptr(), rows, 3,
-                                         d, d_out, d, d_out, 0 if dtype == F32 else 1,
+                                         d, d_out, d, d_out, 0 if dtype == F32 else 1, 0,
                                          torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert (out[:128] == 7).all() and (out[128 + rows:] == 7).all()
