@@ -1,0 +1,116 @@
+// Accumulator tiles to 16-bit results.  A tile in TMEM has 128 neighbours of a result row in
+// its lanes and rows in its columns: the transpose of what memory wants.  Four warps (32 lanes
+// each) take `COLS` columns at a time in the fragment layout of 8 x 8 matrices, round, and store
+// them transposed to shared memory (stmatrix), from where rows of 256 bytes go out 16 bytes a
+// thread.  Storing straight from the lanes, 2 bytes a thread, cost 20 instructions a column and
+// bound the products of short sums: 16384 rows x 32 matrices of 2048 x 768 took 115 us.
+#pragma once
+
+#include "grouped.cuh"
+#include "tc05.cuh"
+
+namespace pa {
+namespace epilogue {
+
+constexpr int kPitch = 272;  // bytes from row to row: 8 rows of 16 bytes fall into different banks
+constexpr int kThreads = 128;
+__host__ __device__ constexpr int cols(int bn) { return bn < 32 ? bn : 32; }
+__host__ __device__ constexpr int bytes(int bn) { return 2 * cols(bn) * kPitch; }  // two buffers
+
+__device__ __forceinline__ void sync() {
+    asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory");
+}
+// true if all four warps say so; they must agree before one leaves the others at a barrier
+__device__ __forceinline__ bool all_agree(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 q, %1, 0;\n"
+        "barrier.cta.red.and.aligned.pred p, 1, 128, q;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(ok))
+        : "memory");
+    return r != 0;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (grouped::is_bf16<T>())
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (nullptr-like: `some` false = zeros), the
+// first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).  `m_left`: lanes that exist.
+// scale(lane of the tile, column of the chunk) multiplies before rounding.  All 128 threads.
+template <typename T, int COLS, typename Scale>
+__device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, bool some, int live,
+                                            int m_left, bool vec, uint32_t buf, int w, int lane,
+                                            Scale scale) {
+    uint32_t p[2][COLS / 8][2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t r[COLS / 2];
+        if (some) {
+            const uint32_t at = tmem + ((32u * w + 16u * half) << 16);
+            if constexpr (COLS == 32) tc05::tmem_ld_16x256_x4(at, r);
+            else tc05::tmem_ld_16x256_x2(at, r);
+            tc05::tmem_ld_wait();
+        } else {
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) r[j] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < COLS / 8; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int m = 32 * w + 16 * half + 8 * h + lane / 4, c = 8 * i + 2 * (lane % 4);
+                p[half][i][h] = pack2<T>(scale(__uint_as_float(r[4 * i + 2 * h]), m, c),
+                                         scale(__uint_as_float(r[4 * i + 2 * h + 1]), m, c + 1));
+            }
+    }
+    // lane l names row l % 8 of matrix l / 8: column block l / 16, rows 8 (l / 8 % 2) on
+    const uint32_t row = buf + (8 * (lane / 16) + lane % 8) * kPitch + (32 * w + 8 * (lane / 8 % 2)) * 2;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < COLS / 8; i += 2)
+            asm volatile(
+                "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                    row + 8 * i * kPitch + 32 * half),
+                "r"(p[half][i][0]), "r"(p[half][i][1]), "r"(p[half][i + 1][0]),
+                "r"(p[half][i + 1][1])
+                : "memory");
+    sync();
+    const int tid = 32 * w + lane;
+    if (vec) {
+        const int m = 8 * (tid % 16);
+#pragma unroll
+        for (int c = tid / 16; c < COLS; c += 8) {
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(buf + c * kPitch + 2 * m)
+                         : "memory");
+            if (c < live && m < m_left) *reinterpret_cast<uint4 *>(dst + c * ld + m) = v;
+        }
+    } else {
+        const int rows = live < COLS ? live : COLS;
+        for (int c = w; c < rows; c += 4)
+#pragma unroll
+            for (int m = lane; m < 128; m += 32) {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + c * kPitch + 2 * m)
+                             : "memory");
+                if (m < m_left) *reinterpret_cast<uint16_t *>(dst + c * ld + m) = v;
+            }
+    }
+}
+
+}  // namespace epilogue
+}  // namespace pa

@@ -7,15 +7,15 @@
 //   rows      m = k of dx,  c = rows i of a group, t = n:  A = w[g] (m contiguous), B = dy
 //   matrices  m = k of dw,  c = n of dw,           t = i:  A = x, B = dy (m and c contiguous)
 // The rows of a group are on the narrow side of the tile (16 to 256 columns), so that groups
-// of a few rows do not multiply 128; the result is stored lane by lane, 32 neighbours of a row at a
-// time, and columns behind the group's last row are left out, so a tile may hang over into the next
-// group: those columns are computed and dropped.  In `matrices` t runs over rows: the tail of
+// of a few rows do not multiply 128; columns behind the group's last row are not stored, so a tile
+// may hang over into the next group: those columns are computed and dropped.  In `matrices` t runs over rows: the tail of
 // the last slice belongs to the next group and is cleared in shared memory, in both operands,
 // so that a NaN there stays there.
 //
 // Persistent CTAs; warp 0 keeps bulk-tensor copies ahead, warp 1 issues the MMAs, warps 4-7 store
 // the tile before while the next is multiplied (two accumulators in TMEM).  Every wait is
 // bounded.
+#include "epilogue.cuh"
 #include "grouped.cuh"
 #include "segments.cuh"
 #include "tc05.cuh"
@@ -35,7 +35,7 @@ __host__ __device__ constexpr int stages(int bn) {
     return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : 10;
 }
 __host__ __device__ constexpr int smem_bytes(int bn) {
-    return stages(bn) * (A_BYTES + b_bytes(bn)) + 1024;
+    return stages(bn) * (A_BYTES + b_bytes(bn)) + epilogue::bytes(bn) + 1024;
 }
 }  // namespace mma
 
@@ -45,6 +45,7 @@ struct Shape {
     int c_size;       // MATRICES: rows of one matrix
     int t_size;       // FORWARD, ROWS: summed axis
     int64_t ldo;
+    bool vec;         // result rows start on 16 bytes and are whole pieces of 16
 };
 
 struct Tile {
@@ -225,42 +226,30 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         }
     } else if (warp >= 4) {
         const int w = warp - 4;
-        uint32_t acc_it = 0;
-        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
+        const uint32_t buf = ring + STAGES * STAGE_BYTES;
+        constexpr int CHUNK = epilogue::cols(BN);
+        uint32_t acc_it = 0, chunk = 0;
+        for (int64_t t = blockIdx.x; t < n_tiles; t += gridDim.x) {
             const Tile tile = tile_at(t);
             const bool some = tile.t0 < tile.t_end;
             const int slot = acc_it & 1;
-            if (some) {
-                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT)) {
-                    abort_s = 1;
-                    break;
-                }
-                tc05::fence_after_sync();
+            bool ok = !abort_s;
+            if (some && ok)
+                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
+                                             WAIT_LIMIT);
+            if (!epilogue::all_agree(ok)) {
+                abort_s = 1;
+                break;
             }
-            const int m = tile.m0 + 32 * w + lane;
+            tc05::fence_after_sync();
             const int live = min(BN, tile.c_end - tile.c0);
-            T *dst = out + tile.out_row * sh.ldo + m;
-            constexpr int STEP = BN < 32 ? BN : 32;
+            T *dst = out + tile.out_row * sh.ldo + tile.m0;
 #pragma unroll 1
-            for (int c0 = 0; c0 < live; c0 += STEP) {
-                uint32_t r[STEP];
-                if (some) {
-                    const uint32_t at = tmem + ((32u * w) << 16) + slot * BN + c0;
-                    if constexpr (STEP == 32) tc05::tmem_ld_32x32(at, r);
-                    else tc05::tmem_ld_32x16(at, r);
-                    tc05::tmem_ld_wait();
-                } else {
-#pragma unroll
-                    for (int j = 0; j < STEP; ++j) r[j] = 0;
-                }
-                if (m < sh.m_size) {
-#pragma unroll
-                    for (int j = 0; j < STEP; ++j)
-                        if (c0 + j < live)
-                            dst[(c0 + j) * sh.ldo] = from_f32<T>(__uint_as_float(r[j]));
-                }
-            }
+            for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
+                epilogue::store_chunk<T, CHUNK>(
+                    dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
+                    sh.m_size - tile.m0, sh.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
+                    lane, [](float v, int, int) { return v; });
             if (some) {
                 tc05::fence_before_sync();
                 __syncwarp();
@@ -334,7 +323,8 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
     if (rc != PA_OK) return rc;
     rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN);
     if (rc != PA_OK) return rc;
-    const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum, ldo};
+    const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum, ldo,
+                   aligned16(out) && ldo % 8 == 0 && d_out % 8 == 0};
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
     return launch<T, MODE, BN>(out, a, b, offsets, sh, most, s);
 }
@@ -378,7 +368,7 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     if (rc != PA_OK) return rc;
     rc = map_rows<T>(&b, dy, d_out, rows, ldy, 64);
     if (rc != PA_OK) return rc;
-    const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0, d};
+    const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0, d, aligned16(dw) && d % 8 == 0};
     const int64_t most =
         static_cast<int64_t>(n_groups) * ((d + 127) / 128) * ((d_out + BN - 1) / BN);
     return launch<T, mma::MATRICES, BN>(dw, a, b, offsets, sh, most, s);
