@@ -7,6 +7,7 @@
 // quotients are those of the definition, up to fp32's own half step.  Rows are independent of
 // one another: a query's codes do not depend on the batch it comes in.
 #include "fp4.cuh"
+#include "grouped.cuh"
 
 namespace pa {
 namespace fp4 {
@@ -14,64 +15,83 @@ namespace fp4 {
 constexpr int kWarps = 8;  // rows per CTA, a warp each
 
 // A lane has eight consecutive values of a chunk of 256, a block is four lanes (mxfp4) or two;
-// kChunks chunks are loaded before any is worked on.  Rows are read once where they fit those
-// registers (or the method needs no maximum of the row), else a second time from the caches.
-constexpr int kChunks = 4;
+// CHUNKS (1 to 4) chunks are loaded before any is worked on.  Rows are read once where they fit
+// those registers (or the method needs no maximum of the row), else a second time from the caches.
+// Eight values as they are in memory: 32 bytes of fp32, 16 of the others.
+template <typename T> struct Raw { uint32_t w[2 * sizeof(T)]; };
 
-__device__ __forceinline__ void unpack8(float (&v)[8], const float *p) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)),
-                 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void unpack8(float (&v)[8], const __nv_bfloat16 *p) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <typename T>
+__device__ __forceinline__ void load8(Raw<T> &raw, const T *row, int64_t at, int64_t d, bool vec) {
+    if (vec && at + 8 <= d) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + at) + i);
+            raw.w[4 * i] = a.x; raw.w[4 * i + 1] = a.y; raw.w[4 * i + 2] = a.z; raw.w[4 * i + 3] = a.w;
+        }
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            raw.w[j] = at + j < d ? __ldg(reinterpret_cast<const uint32_t *>(row) + at + j) : 0u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h =
+                at + j < d ? __ldg(reinterpret_cast<const uint16_t *>(row) + at + j) : 0u;
+            raw.w[j / 2] = j % 2 ? raw.w[j / 2] | (h << 16) : h;
+        }
     }
 }
-__device__ __forceinline__ void unpack8(float (&v)[8], const __half *p) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+
+__device__ __forceinline__ void values8(float (&v)[8], const Raw<float> &raw) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw.w[j]);
+}
+__device__ __forceinline__ void values8(float (&v)[8], const Raw<__nv_bfloat16> &raw) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+        v[2 * j] = __uint_as_float(raw.w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(raw.w[j] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void values8(float (&v)[8], const Raw<__half> &raw) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&raw.w[j]));
         v[2 * j] = f.x;
         v[2 * j + 1] = f.y;
     }
 }
-template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T *row, int64_t at, int64_t d, bool vec) {
-    if (vec && at + 8 <= d) {
-        unpack8(v, row + at);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = at + j < d ? load_f32(row + at + j) : 0.0f;
-    }
-}
 
-__device__ __forceinline__ uint32_t top_bits(const float (&v)[8]) {
-    uint32_t t = 0;  // magnitudes order like their bits; NaN above infinity above the rest
+// Bits of the largest magnitude, as fp32: magnitudes order like their bits in every type, NaN above
+// infinity above the rest, so 16-bit ones are compared two at a time.
+__device__ __forceinline__ uint32_t top_bits(const Raw<float> &raw) {
+    uint32_t t = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t = max(t, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) t = max(t, raw.w[j] & 0x7fffffffu);
     return t;
+}
+template <typename T> __device__ __forceinline__ uint32_t top_bits(const Raw<T> &raw) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t = __vmaxu2(t, raw.w[j] & 0x7fff7fffu);
+    t = max(t & 0xffffu, t >> 16);
+    if (grouped::is_bf16<T>()) return t << 16;
+    const float f = __half2float(__ushort_as_half(static_cast<unsigned short>(t)));
+    return __float_as_uint(f);
 }
 
 // v / step as codes.  fp32 values are divided.  16-bit ones have at most 11 significant bits and
-// step has four, so that a quotient is a border between two codes exactly or at least 2^-12 of
-// its value away from it: a product with the reciprocal (off by 2^-23), rounded to 18 bits
-// behind the leading one, lands on the border in the first case and stays off it in the other,
-// at a third of the instructions.
+// step has four, so that a quotient is a border between two codes (a multiple of 1/4) exactly or at
+// least 2^-13 away from it: a product with the reciprocal, off by 2^-22 of its value, is rounded
+// to a multiple of 2^-14 by adding and subtracting 768, which lands on the border in the first case and stays
+// off it in the other, for two instructions a value.  (It loses the sign of what becomes 0.)
 template <typename T>
 __device__ __forceinline__ uint32_t codes_by(float (&v)[8], float step) {
     if (sizeof(T) == 2 && step >= 1.1754944e-38f) {  // a reciprocal that does not overflow
-        const float inv = __frcp_rn(step);
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));  // step < 2^126
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = __uint_as_float((__float_as_uint(__fmul_rn(v[j], inv)) + 16u) & ~31u);
+        for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(__fmaf_rn(v[j], inv, 768.0f), -768.0f);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = step > 0.0f ? __fdiv_rn(v[j], step) : 0.0f;
@@ -79,7 +99,18 @@ __device__ __forceinline__ uint32_t codes_by(float (&v)[8], float step) {
     return codes_of(v);
 }
 
-template <typename T, int METHOD>
+// E4M3 of top / 6: borders have five significant bits, so the same holds of a product with 1 / 6,
+// here rounded to 18 bits behind the leading one
+template <typename T> __device__ __forceinline__ uint32_t scale_of(float top) {
+    float ratio;
+    if (sizeof(T) == 2)
+        ratio = __uint_as_float((__float_as_uint(__fmul_rn(top, 1.0f / 6.0f)) + 16u) & ~31u);
+    else
+        ratio = __fdiv_rn(top, 6.0f);
+    return e4m3_of(fminf(ratio, 448.0f));
+}
+
+template <typename T, int METHOD, int CHUNKS>
 __global__ void __launch_bounds__(32 * kWarps)
 quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                 float *__restrict__ row_scale, const T *__restrict__ x, int64_t rows, int64_t d,
@@ -92,15 +123,15 @@ quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
     constexpr int kLanes = METHOD == PA_MXFP4 ? 4 : 2;  // lanes of a block
     uint32_t *to = reinterpret_cast<uint32_t *>(codes + r * (dp / 2)) + lane;
     uint8_t *to_scale = scales + r * (dp / (8 * kLanes)) + lane / kLanes;
-    float v[kChunks][8];
+    Raw<T> raw[CHUNKS];
     float s = 1.0f, s_inv = 1.0f;
     if (METHOD == PA_NVFP4) {
         uint32_t top = 0;
-        for (int64_t a0 = 0; a0 < dp; a0 += 256 * kChunks) {
+        for (int64_t a0 = 0; a0 < dp; a0 += 256 * CHUNKS) {
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) load8(v[c], row, a0 + 256 * c + 8 * lane, d, vec);
+            for (int c = 0; c < CHUNKS; ++c) load8(raw[c], row, a0 + 256 * c + 8 * lane, d, vec);
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) top = max(top, top_bits(v[c]));
+            for (int c = 0; c < CHUNKS; ++c) top = max(top, top_bits(raw[c]));
         }
         top = __reduce_max_sync(0xffffffffu, top);
         // 6 * 448 = 1.3125 * 2^11; the power is in [-126, 117]
@@ -111,32 +142,33 @@ quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
         s_inv = fine ? __uint_as_float(static_cast<uint32_t>(127 - power) << 23) : CUDART_NAN_F;
         if (lane == 0) row_scale[r] = s;
     }
-    for (int64_t a0 = 0; a0 < dp; a0 += 256 * kChunks) {
-        if (METHOD == PA_MXFP4 || dp > 256 * kChunks) {
+    for (int64_t a0 = 0; a0 < dp; a0 += 256 * CHUNKS) {
+        if (METHOD == PA_MXFP4 || dp > 256 * CHUNKS) {
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) load8(v[c], row, a0 + 256 * c + 8 * lane, d, vec);
+            for (int c = 0; c < CHUNKS; ++c) load8(raw[c], row, a0 + 256 * c + 8 * lane, d, vec);
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < CHUNKS; ++c) {
             const int64_t at = a0 + 256 * c + 8 * lane;
             if (a0 + 256 * c >= dp) break;  // uniform
-            uint32_t top = top_bits(v[c]);
+            uint32_t top = top_bits(raw[c]);
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1)
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float v[8];
+            values8(v, raw[c]);
             uint32_t byte, code;
             if (METHOD == PA_MXFP4) {
                 const uint32_t e = top >> 23;
                 byte = e > 2u ? e - 2u : 0u;
                 const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[c][j] = __fmul_rn(v[c][j], inv);
-                code = codes_of(v[c]);
+                for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], inv);
+                code = codes_of(v);
                 if (e == 255u) { byte = 255u; code = 0u; }
             } else {
-                const float ratio = __fdiv_rn(__fmul_rn(__uint_as_float(top), s_inv), 6.0f);
-                byte = e4m3_of(fminf(ratio, 448.0f));
-                code = codes_by<T>(v[c], __fmul_rn(e4m3_value(byte), s));
+                byte = scale_of<T>(__fmul_rn(__uint_as_float(top), s_inv));
+                code = codes_by<T>(v, __fmul_rn(e4m3_value(byte), s));
                 if (!(s > 0.0f)) { byte = 0u; code = 0u; }  // NaN: the row's scale says it
             }
             if (at < dp) {
@@ -147,25 +179,26 @@ quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
     }
 }
 
-// eight codes -> eight values of their block (exact: two significant bits times at most four)
-__device__ __forceinline__ void values_of(float (&v)[8], uint32_t code, float scale) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t h;
-        asm("{\n"
-            ".reg .b8 b;\n"
-            "cvt.u8.u32 b, %1;\n"
-            "cvt.rn.f16x2.e2m1x2 %0, b;\n"
-            "}\n"
-            : "=r"(h)
-            : "r"((code >> (8 * j)) & 0xffu));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-        v[2 * j] = __fmul_rn(f.x, scale);
-        v[2 * j + 1] = __fmul_rn(f.y, scale);
-    }
+// four codes -> four values of their block (exact: two significant bits times at most four)
+__device__ __forceinline__ float4 values_of(uint32_t code, float scale) {
+    uint32_t lo, hi;
+    asm("{\n"
+        ".reg .b8 b0, b1, b2, b3;\n"
+        "mov.b32 {b0, b1, b2, b3}, %2;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n"
+        "}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(code));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo)),
+                 b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return make_float4(__fmul_rn(a.x, scale), __fmul_rn(a.y, scale), __fmul_rn(b.x, scale),
+                       __fmul_rn(b.y, scale));
 }
 
-template <int METHOD>
+// A warp has a row; it loads 256 codes (4 bytes a lane) at a time and hands them around so that
+// the lanes store 16 bytes side by side.
+template <int METHOD, int CHUNKS>
 __global__ void __launch_bounds__(32 * kWarps)
 dequantize_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
                   const uint8_t *__restrict__ scales, const float *__restrict__ row_scale,
@@ -178,51 +211,69 @@ dequantize_kernel(float *__restrict__ out, const uint8_t *__restrict__ codes,
     const uint32_t *from = reinterpret_cast<const uint32_t *>(codes + r * (dp / 2)) + lane;
     const uint8_t *from_scale = scales + r * (dp / (8 * kLanes)) + lane / kLanes;
     const float s = METHOD == PA_NVFP4 ? row_scale[r] : 1.0f;
-    float *to = out + r * d + 8 * lane;
-    for (int64_t a0 = 0; a0 < d; a0 += 256 * kChunks) {
-        uint32_t code[kChunks], byte[kChunks];
+    float *to = out + r * d + 4 * lane;
+    for (int64_t a0 = 0; a0 < d; a0 += 256 * CHUNKS) {
+        uint32_t code[CHUNKS], byte[CHUNKS];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < CHUNKS; ++c) {
             const int64_t a = a0 + 256 * c;
-            const bool live = a + 8 * lane < d;
+            const bool live = a + 8 * lane < dp;
             code[c] = live ? __ldg(from + a / 8) : 0u;
             byte[c] = live ? __ldg(from_scale + a / (8 * kLanes)) : 0u;
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int64_t a = a0 + 256 * c, at = a + 8 * lane;
-            if (at >= d) break;
-            float v[8];
-            if (METHOD == PA_MXFP4) {
-                values_of(v, code[c], e8m0_value(byte[c]));
-            } else {
-                values_of(v, code[c], e4m3_value(byte[c]));
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int64_t a = a0 + 256 * c;
+            if (a >= d) break;  // uniform
+            const float scale = METHOD == PA_MXFP4 ? e8m0_value(byte[c]) : e4m3_value(byte[c]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], s);
-            }
-            if (vec) {
-                *reinterpret_cast<float4 *>(to + a) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4 *>(to + a + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (at + j < d) to[a + j] = v[j];
+            for (int k = 0; k < 2; ++k) {
+                const int src = 16 * k + lane / 2;
+                const uint32_t mine = __shfl_sync(0xffffffffu, code[c], src) >> (16 * (lane & 1));
+                const float by = __shfl_sync(0xffffffffu, scale, src);
+                float4 v = values_of(mine, by);
+                if (METHOD == PA_NVFP4) {
+                    v.x = __fmul_rn(v.x, s); v.y = __fmul_rn(v.y, s);
+                    v.z = __fmul_rn(v.z, s); v.w = __fmul_rn(v.w, s);
+                }
+                const int64_t at = a + 128 * k + 4 * lane;
+                float *p = to + a + 128 * k;
+                if (vec && at < d) {
+                    *reinterpret_cast<float4 *>(p) = v;
+                } else {
+                    if (at < d) p[0] = v.x;
+                    if (at + 1 < d) p[1] = v.y;
+                    if (at + 2 < d) p[2] = v.z;
+                    if (at + 3 < d) p[3] = v.w;
+                }
             }
         }
     }
 }
+
+// chunks of 256 values a row has, at most 4
+int chunks_of(int64_t d) { return static_cast<int>(d > 768 ? 4 : (d + 255) / 256); }
 
 template <typename T>
 int quantize_launch(uint8_t *codes, uint8_t *scales, float *row_scale, const void *x, int64_t rows,
                     int64_t d, int64_t ldx, int method, cudaStream_t s) {
     const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
     const bool vec = aligned16(x) && ldx * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 32 * kWarps, 0, s>>>(codes, scales, row_scale, static_cast<const T *>(x),
+                                            rows, d, ldx, vec);
+    };
+    const int chunks = chunks_of(d);
     if (method == PA_MXFP4)
-        quantize_kernel<T, PA_MXFP4><<<grid, 32 * kWarps, 0, s>>>(
-            codes, scales, row_scale, static_cast<const T *>(x), rows, d, ldx, vec);
+        chunks == 1   ? go(quantize_kernel<T, PA_MXFP4, 1>)
+        : chunks == 2 ? go(quantize_kernel<T, PA_MXFP4, 2>)
+        : chunks == 3 ? go(quantize_kernel<T, PA_MXFP4, 3>)
+                      : go(quantize_kernel<T, PA_MXFP4, 4>);
     else
-        quantize_kernel<T, PA_NVFP4><<<grid, 32 * kWarps, 0, s>>>(
-            codes, scales, row_scale, static_cast<const T *>(x), rows, d, ldx, vec);
+        chunks == 1   ? go(quantize_kernel<T, PA_NVFP4, 1>)
+        : chunks == 2 ? go(quantize_kernel<T, PA_NVFP4, 2>)
+        : chunks == 3 ? go(quantize_kernel<T, PA_NVFP4, 3>)
+                      : go(quantize_kernel<T, PA_NVFP4, 4>);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
@@ -269,13 +320,21 @@ extern "C" int pa_dequantize_fp4(float *out, const uint8_t *codes, const uint8_t
     PA_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
     const unsigned grid = static_cast<unsigned>((rows + fp4::kWarps - 1) / fp4::kWarps);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool vec = aligned16(out) && d % 8 == 0;
+    const bool vec = aligned16(out) && d % 4 == 0;
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 32 * fp4::kWarps, 0, s>>>(out, codes, scales, row_scale, rows, d, vec);
+    };
+    const int chunks = fp4::chunks_of(d);
     if (method == PA_MXFP4)
-        fp4::dequantize_kernel<PA_MXFP4><<<grid, 32 * fp4::kWarps, 0, s>>>(out, codes, scales,
-                                                                           row_scale, rows, d, vec);
+        chunks == 1   ? go(fp4::dequantize_kernel<PA_MXFP4, 1>)
+        : chunks == 2 ? go(fp4::dequantize_kernel<PA_MXFP4, 2>)
+        : chunks == 3 ? go(fp4::dequantize_kernel<PA_MXFP4, 3>)
+                      : go(fp4::dequantize_kernel<PA_MXFP4, 4>);
     else
-        fp4::dequantize_kernel<PA_NVFP4><<<grid, 32 * fp4::kWarps, 0, s>>>(out, codes, scales,
-                                                                           row_scale, rows, d, vec);
+        chunks == 1   ? go(fp4::dequantize_kernel<PA_NVFP4, 1>)
+        : chunks == 2 ? go(fp4::dequantize_kernel<PA_NVFP4, 2>)
+        : chunks == 3 ? go(fp4::dequantize_kernel<PA_NVFP4, 3>)
+                      : go(fp4::dequantize_kernel<PA_NVFP4, 4>);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;

@@ -11,6 +11,7 @@
 // l + 96 per lane (512 values of mxfp4, 256 of nvfp4), which is a 4 x 4 transpose in its
 // registers, stores four 16-byte rows without bank conflicts, and tcgen05.cp spreads them.
 // nvfp4's row scales, powers of two, multiply the finished sum.
+#include "epilogue.cuh"
 #include "fp4.cuh"
 #include "grouped.cuh"
 #include "segments.cuh"
@@ -22,6 +23,7 @@ namespace fp4 {
 
 using grouped::from_f32;
 using grouped::Segments;
+using grouped::Walk;
 
 namespace mma {
 constexpr int BM = 128, BK = 256;        // values; 128 bytes of codes
@@ -29,14 +31,20 @@ constexpr int A_BYTES = BM * BK / 2;
 constexpr int SCALE_SLOTS = 4;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_blocks(int bn) { return bn > 128 ? 2 : 1; }
-__host__ __device__ constexpr int threads(int bn) { return 32 * (7 + b_blocks(bn)); }
+// Loader warps of a block of 128 rows of scales: each has two pieces of 16 bytes a row on their
+// way, about 1 us from DRAM, while a tile of short rows needs a piece every 0.6 us.
+__host__ __device__ constexpr int loaders(int bn) { return bn > 128 ? 3 : 4; }
+__host__ __device__ constexpr int threads(int bn) {
+    return 32 * (6 + (1 + b_blocks(bn)) * loaders(bn));
+}
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK / 2; }
 __host__ __device__ constexpr int scale_bytes(int bn) { return (1 + b_blocks(bn)) * 2048; }
 __host__ __device__ constexpr int stages(int bn) {
-    return bn >= 192 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 7 : bn >= 32 ? 9 : 10;
+    return bn >= 192 ? 4 : bn >= 128 ? 5 : bn >= 64 ? 7 : bn >= 32 ? 9 : 10;
 }
 __host__ __device__ constexpr int smem_bytes(int bn) {
-    return stages(bn) * stage_bytes(bn) + SCALE_SLOTS * scale_bytes(bn) + 1024;
+    return stages(bn) * stage_bytes(bn) + SCALE_SLOTS * scale_bytes(bn) +
+           epilogue::bytes(bn) + 1024;
 }
 }  // namespace mma
 
@@ -49,6 +57,7 @@ struct Args {
     int rows, n_groups, values;          // values of a row, padded to 32
     int q_pitch, t_pitch;                // bytes of scales from row to row
     int out_dtype;
+    bool vec;                            // 16-bit result rows are whole pieces of 16 bytes
     int *status;
 };
 
@@ -93,12 +102,13 @@ __device__ __forceinline__ uint4 scales_take(const Piece &p, const uint8_t *row,
 template <int METHOD, int BN>
 __global__ void __launch_bounds__(mma::threads(BN), 1)
 project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_q,
-               const __grid_constant__ Args args) {
+               const __grid_constant__ CUtensorMap map_tail, const __grid_constant__ Args args) {
     using namespace mma;
     constexpr int THREADS = threads(BN), STAGES = stages(BN), STAGE_BYTES = stage_bytes(BN);
     constexpr int NB = b_blocks(BN), SLOT_BYTES = scale_bytes(BN);
     constexpr int GROUP = METHOD == PA_MXFP4 ? 2 : 1;   // stages that 16 scale bytes last
     constexpr int SCALE_COLS = 16 * (1 + NB);
+    constexpr int BOX = BN < 64 ? BN : 64, BOX_BYTES = BOX * BK / 2;  // of the queries' codes
     constexpr int ACC_COLS = 2 * BN;
     constexpr uint32_t COLS = ACC_COLS + 2 * SCALE_COLS <= 128 ? 128
                               : ACC_COLS + 2 * SCALE_COLS <= 256 ? 256 : 512;
@@ -109,6 +119,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_s;
     __shared__ Segments segs;
+    __shared__ float t_scale_s[2][BM], q_scale_s[2][BN];  // nvfp4's row scales of two tiles
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
     const uint32_t scale_ring = ring + STAGES * STAGE_BYTES;
@@ -140,16 +151,15 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     const uint32_t tmem = tmem_slot;
 
     const int m_tiles = static_cast<int>((args.d_out + BM - 1) / BM);
-    const int64_t n_tiles = static_cast<int64_t>(segs.tiles[args.n_groups + 2]) * m_tiles;
+    Walk walk(blockIdx.x, gridDim.x, segs.tiles[args.n_groups + 2], m_tiles);
     const int n_stages = (args.values + BK - 1) / BK;
     struct Tile { int g, m0, c0, c_end; };
-    auto tile_at = [&](int64_t t) {
+    auto tile_at = [&]() {
         Tile r;
-        const int row = static_cast<int>(t / m_tiles);
-        r.m0 = static_cast<int>(t - static_cast<int64_t>(row) * m_tiles) * BM;
-        const int seg = grouped::segs_find(segs, args.n_groups, row);
+        r.m0 = walk.col * BM;
+        const int seg = walk.segment(segs);
         r.g = seg >= 1 && seg <= args.n_groups ? seg - 1 : -1;  // -1: rows of no group, zeros
-        r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
+        r.c0 = segs.edge[seg] + (walk.row - segs.tiles[seg]) * BN;
         r.c_end = segs.edge[seg + 1];
         return r;
     };
@@ -158,9 +168,10 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // ---- codes ----
         if (lane == 0) {
             uint32_t it = 0;
-            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
-                const Tile tile = tile_at(t);
+            for (; walk.live() && !abort_s; walk.next()) {
+                const Tile tile = tile_at();
                 if (tile.g < 0) continue;
+                const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
                 for (int k = 0; k < n_stages; ++k, ++it) {
                     const int s = it % STAGES;
                     if (it >= STAGES &&
@@ -171,9 +182,15 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     }
                     const uint32_t a = ring + s * STAGE_BYTES;
                     const uint32_t bar = tc05::smem_u32(&full_bar[s]);
-                    tc05::mbar_expect_tx(bar, STAGE_BYTES);
+                    tc05::mbar_expect_tx(bar, A_BYTES + boxes * BOX_BYTES);
                     tc05::tma_load_3d(a, &map_t, k * (BK / 2), tile.m0, tile.g, bar);
-                    tc05::tma_load_2d(a + A_BYTES, &map_q, k * (BK / 2), tile.c0, bar);
+                    if (boxes * BOX == BN) {
+                        tc05::tma_load_2d(a + A_BYTES, &map_q, k * (BK / 2), tile.c0, bar);
+                    } else {
+                        for (int j = 0; j < boxes; ++j)
+                            tc05::tma_load_2d(a + A_BYTES + j * BOX_BYTES, &map_tail, k * (BK / 2),
+                                              tile.c0 + BOX * j, bar);
+                    }
                 }
             }
             if (abort_s) {  // no copy is left in flight behind the CTA
@@ -186,8 +203,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // ---- products ----
         if (lane == 0) {
             uint32_t it = 0, sg = 0, acc_it = 0;
-            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
-                const Tile tile = tile_at(t);
+            // of the first stage and slot; a descriptor counts 16 bytes, so others are sums
+            const uint64_t desc_a = tc05::smem_desc_sw128(ring);
+            const uint64_t desc_s = tc05::smem_desc_rows16(scale_ring);
+            for (; walk.live() && !abort_s; walk.next()) {
+                const Tile tile = tile_at();
                 if (tile.g < 0) continue;
                 const int acc = acc_it & 1;
                 if (acc_it >= 2 && !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[acc]),
@@ -197,6 +217,9 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 }
                 tc05::fence_after_sync();
                 const uint32_t d = tmem + acc * BN;
+                const int cols = min(BN, tile.c_end - tile.c0);
+                const uint32_t idesc0 =
+                    tc05::idesc_mxf4(METHOD == PA_MXFP4, (cols + 15) / 16 * 16);
                 uint32_t sa = 0, sb = 0;
                 for (int k = 0; k < n_stages; ++k, ++it) {
                     const int s = it % STAGES, slot = sg % SCALE_SLOTS;
@@ -214,31 +237,29 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                         tc05::fence_after_sync();
                         sa = tmem + ACC_COLS + (sg & 1) * SCALE_COLS;
                         sb = sa + 16;
-                        const uint32_t from = scale_ring + slot * SLOT_BYTES;
+                        const uint64_t from = desc_s + slot * (SLOT_BYTES / 16);
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            tc05::tmem_cp_scales(sa + 4 * w,
-                                                 tc05::smem_desc_rows16(from + 512 * w));
+                            tc05::tmem_cp_scales(sa + 4 * w, from + 32 * w);
 #pragma unroll
                             for (int j = 0; j < NB; ++j)
-                                tc05::tmem_cp_scales(
+                                if (j == 0 || cols > 128) tc05::tmem_cp_scales(
                                     sb + 4 * (NB * w + j),
-                                    tc05::smem_desc_rows16(from + 2048 * (1 + j) + 512 * w));
+                                    from + 128 * (1 + j) + 32 * w);
                         }
                     }
                     tc05::fence_after_sync();
-                    const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                    const uint64_t a = desc_a + s * (STAGE_BYTES / 16), b = a + A_BYTES / 16;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (k * BK + 64 * j < args.values) {
                             // 64 values: two bytes of a scale word (mxfp4) or all four (nvfp4)
                             const int word = METHOD == PA_MXFP4 ? 2 * (k % GROUP) + j / 2 : j;
-                            const uint32_t idesc = tc05::idesc_mxf4(
-                                METHOD == PA_MXFP4, BN, METHOD == PA_MXFP4 ? 2 * (j & 1) : 0);
+                            const uint32_t idesc =
+                                idesc0 | tc05::idesc_scale_id(METHOD == PA_MXFP4 ? 2 * (j & 1) : 0);
                             tc05::mma_fp4<METHOD == PA_MXFP4>(
-                                d, tc05::smem_desc_sw128(a + 32 * j),
-                                tc05::smem_desc_sw128(b + 32 * j), idesc, sa + 4 * word,
-                                sb + 4 * NB * word, k > 0 || j > 0);
+                                d, a + 2 * j, b + 2 * j, idesc, sa + 4 * word, sb + 4 * NB * word,
+                                k > 0 || j > 0);
                         }
                     }
                     tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
@@ -256,22 +277,22 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             }
         }
     } else if (warp < 4 || warp >= 8) {
-        // ---- scales: warp 2 the table's 128 rows, warps 3 and 8 the queries' ----
-        const int block = warp == 2 ? 0 : warp == 3 ? 1 : 2;
+        // ---- scales: block 0 the table's 128 rows, 1 and 2 the queries' ----
+        const int li = warp < 4 ? warp - 2 : warp - 6;
+        const int block = li % (1 + NB);
         const int pitch = block == 0 ? args.t_pitch : args.q_pitch;
         const int n_pieces = (n_stages + GROUP - 1) / GROUP;
-        int64_t t = blockIdx.x;
-        int piece = 0;
+        const int piece0 = li / (1 + NB);  // this warp has every loaders(BN)-th piece
+        int piece = piece0;
         Tile tile = {};
         const uint8_t *row[4];
         bool live[4];
         auto rows_of_tile = [&]() {  // skips tiles without a group; false at the end
-            while (t < n_tiles) {
-                tile = tile_at(t);
+            for (; walk.live(); walk.next()) {
+                tile = tile_at();
                 if (tile.g >= 0) break;
-                t += gridDim.x;
             }
-            if (t >= n_tiles) return false;
+            if (!walk.live()) return false;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const int r = 32 * b + lane;
@@ -287,25 +308,32 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             }
             return true;
         };
-        bool more = rows_of_tile();
+        // the piece of the current tile, or that far into the tiles behind it
+        auto settle = [&]() {
+            while (piece >= n_pieces) {
+                piece -= n_pieces;
+                walk.next();
+                if (!rows_of_tile()) return false;
+            }
+            return true;
+        };
+        bool more = rows_of_tile() && settle();
         Piece next[4];
+        int at = 16 * piece;
         if (more) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], 0, pitch, live[b]);
+            for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
         }
-        for (uint32_t sg = 0; more && !abort_s; ++sg) {
+        for (uint32_t sg = piece0; more && !abort_s; sg += loaders(BN)) {
             uint4 v[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) v[b] = scales_take(next[b], row[b], 16 * piece, pitch);
-            if (++piece == n_pieces) {
-                piece = 0;
-                t += gridDim.x;
-                more = rows_of_tile();
-            }
+            for (int b = 0; b < 4; ++b) v[b] = scales_take(next[b], row[b], at, pitch);
+            piece += loaders(BN);
+            more = settle();
+            at = 16 * piece;
             if (more) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    next[b] = scales_fetch(row[b], 16 * piece, pitch, live[b]);
+                for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
             }
             const int slot = sg % SCALE_SLOTS;
             if (sg >= SCALE_SLOTS &&
@@ -330,61 +358,82 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         }
     } else {
         // ---- results: warp w has lanes 32 (w - 4) .. of the accumulator ----
-        const int w = warp - 4;
-        uint32_t acc_it = 0;
-        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
-            const Tile tile = tile_at(t);
+        const int w = warp - 4, own = 32 * w + lane;
+        const uint32_t buf = scale_ring + SCALE_SLOTS * SLOT_BYTES;
+        constexpr int CHUNK = epilogue::cols(BN);
+        uint32_t acc_it = 0, n_tile = 0, chunk = 0;
+        for (; walk.live(); walk.next(), ++n_tile) {
+            const Tile tile = tile_at();
             const bool some = tile.g >= 0;
-            const int acc = acc_it & 1;
-            const int m = tile.m0 + 32 * w + lane;
-            const bool mine = m < args.d_out;
-            float t_scale = 1.0f;
-            if (METHOD == PA_NVFP4 && some && mine)
-                t_scale = __ldg(args.t_row_scale + tile.g * args.d_out + m);
-            if (some) {
-                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT)) {
-                    abort_s = 1;
-                    break;
-                }
-                tc05::fence_after_sync();
+            const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
+            const float *ts = t_scale_s[n_tile & 1], *qs = q_scale_s[n_tile & 1];
+            if (METHOD == PA_NVFP4 && some) {
+                t_scale_s[n_tile & 1][own] =
+                    tile.m0 + own < args.d_out
+                        ? __ldg(args.t_row_scale + tile.g * args.d_out + tile.m0 + own) : 0.0f;
+                for (int c = own; c < BN; c += 128)
+                    q_scale_s[n_tile & 1][c] = c < live ? __ldg(args.q_row_scale + tile.c0 + c) : 0.0f;
             }
-            const int live = min(BN, tile.c_end - tile.c0);
-            const int64_t at = tile.c0 * args.d_out + m;
-            constexpr int STEP = BN < 32 ? BN : 32;
+            bool ok = !abort_s;
+            if (some && ok)
+                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
+                                             WAIT_LIMIT);
+            if (!epilogue::all_agree(ok)) {
+                abort_s = 1;
+                break;
+            }
+            tc05::fence_after_sync();
+            const int m_left = static_cast<int>(min(args.d_out - tile.m0, static_cast<int64_t>(BM)));
+            const int64_t first = tile.c0 * args.d_out + tile.m0;
+            const uint32_t from = tmem + acc * BN;
+            auto scale = [&](float v, int m, int c) {
+                return METHOD == PA_NVFP4 && some ? v * (ts[m] * qs[c]) : v;
+            };
+            if (args.out_dtype == PA_F32) {
+                // 32 lanes store 128 bytes of a row as they are
+                float *dst = static_cast<float *>(args.out) + first + own;
+                const float mine = METHOD == PA_NVFP4 && some ? ts[own] : 1.0f;
 #pragma unroll 1
-            for (int c0 = 0; c0 < live; c0 += STEP) {
-                uint32_t r[STEP];
-                float q_scale = 1.0f;
-                if (METHOD == PA_NVFP4 && some && lane < STEP && c0 + lane < live)
-                    q_scale = __ldg(args.q_row_scale + tile.c0 + c0 + lane);
-                if (some) {
-                    const uint32_t col = tmem + ((32u * w) << 16) + acc * BN + c0;
-                    if constexpr (STEP == 32) tc05::tmem_ld_32x32(col, r);
-                    else tc05::tmem_ld_32x16(col, r);
-                    tc05::tmem_ld_wait();
-                } else {
+                for (int c0 = 0; c0 < live; c0 += CHUNK) {
+                    uint32_t r[CHUNK];
+                    if (some) {
+                        const uint32_t col = from + ((32u * w) << 16) + c0;
+                        if constexpr (CHUNK == 32) tc05::tmem_ld_32x32(col, r);
+                        else tc05::tmem_ld_32x16(col, r);
+                        tc05::tmem_ld_wait();
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < STEP; ++j) r[j] = 0;
-                }
-                if (METHOD == PA_NVFP4) {
+                        for (int j = 0; j < CHUNK; ++j) r[j] = 0;
+                    }
+                    if (METHOD == PA_NVFP4 && some) {
 #pragma unroll
-                    for (int j = 0; j < STEP; ++j)
-                        r[j] = __float_as_uint(__uint_as_float(r[j]) *
-                                               (t_scale * __shfl_sync(0xffffffffu, q_scale, j)));
+                        for (int j = 0; j < CHUNK; ++j)
+                            r[j] = __float_as_uint(__uint_as_float(r[j]) * (mine * qs[c0 + j]));
+                    }
+                    if (own < m_left) {
+                        if (c0 + CHUNK <= live) {
+#pragma unroll
+                            for (int j = 0; j < CHUNK; ++j, dst += args.d_out)
+                                *dst = __uint_as_float(r[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < CHUNK; ++j, dst += args.d_out)
+                                if (c0 + j < live) *dst = __uint_as_float(r[j]);
+                        }
+                    }
                 }
+            } else {
                 auto store = [&](auto *out) {
                     using O = typename std::remove_pointer<decltype(out)>::type;
-                    O *dst = out + at + c0 * args.d_out;
-#pragma unroll
-                    for (int j = 0; j < STEP; ++j)
-                        if (c0 + j < live) dst[j * args.d_out] = from_f32<O>(__uint_as_float(r[j]));
+#pragma unroll 1
+                    for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
+                        epilogue::store_chunk<O, CHUNK>(
+                            out + first + c0 * args.d_out, args.d_out, from + c0, some, live - c0,
+                            m_left, args.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
+                            [&](float v, int m, int c) { return scale(v, m, c0 + c); });
                 };
-                if (mine) {
-                    if (args.out_dtype == PA_F32) store(static_cast<float *>(args.out));
-                    else if (args.out_dtype == PA_BF16) store(static_cast<__nv_bfloat16 *>(args.out));
-                    else store(static_cast<__half *>(args.out));
-                }
+                if (args.out_dtype == PA_BF16) store(static_cast<__nv_bfloat16 *>(args.out));
+                else store(static_cast<__half *>(args.out));
             }
             if (some) {
                 tc05::fence_before_sync();
@@ -430,10 +479,13 @@ static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t
     if (rc != PA_OK) return rc;
     rc = map_codes(&map_q, q_codes, args.values, args.rows, 0, BN);
     if (rc != PA_OK) return rc;
+    CUtensorMap tail = map_q;
+    if (BN > 64 && (rc = map_codes(&tail, q_codes, args.values, args.rows, 0, 64)) != PA_OK)
+        return rc;
     const int64_t most = (static_cast<int64_t>(args.rows) / BN + args.n_groups + 2) *
                          ((args.d_out + mma::BM - 1) / mma::BM);
     const unsigned grid = static_cast<unsigned>(most < sms ? most : sms);
-    project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q,
+    project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q, tail,
                                                                                    args);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
@@ -478,7 +530,8 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     const int values = static_cast<int>(fp4::padded(d));
     const int pitch = values / fp4::block_of(method);
     const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,
-                         static_cast<int>(rows), n_groups, values, pitch, pitch, out_dtype, status};
+                         static_cast<int>(rows), n_groups, values, pitch, pitch, out_dtype,
+                         aligned16(out) && d_out % 8 == 0, status};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return method == PA_MXFP4
                ? fp4::project_method<PA_MXFP4>(args, query_codes, codes, s)

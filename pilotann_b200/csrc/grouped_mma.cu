@@ -8,7 +8,8 @@
 //   matrices  m = k of dw,  c = n of dw,           t = i:  A = x, B = dy (m and c contiguous)
 // The rows of a group are on the narrow side of the tile (16 to 256 columns), so that groups
 // of a few rows do not multiply 128; columns behind the group's last row are not stored, so a tile
-// may hang over into the next group: those columns are computed and dropped.  In `matrices` t runs over rows: the tail of
+// may hang over into the next group: those columns are dropped.  The last tile of a group loads
+// and multiplies whole 64s and 16s of columns only.  In `matrices` t runs over rows: the tail of
 // the last slice belongs to the next group and is cleared in shared memory, in both operands,
 // so that a NaN there stays there.
 //
@@ -59,10 +60,12 @@ struct Tile {
 template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(mma::THREADS, 1)
 mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
-           const __grid_constant__ CUtensorMap map_b, const int64_t *__restrict__ offsets, Shape sh,
+           const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_tail,
+           const int64_t *__restrict__ offsets, Shape sh,
            int *__restrict__ status) {
     using namespace mma;
     constexpr int STAGES = stages(BN), B_BYTES = b_bytes(BN), STAGE_BYTES = A_BYTES + B_BYTES;
+    constexpr int BOX = BN < 64 ? BN : 64, BOX_BYTES = BOX * BK * 2;  // of B
     constexpr bool A_MN = MODE != FORWARD, B_MN = MODE == MATRICES;
     constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // TMEM columns: a power of two
     extern __shared__ uint8_t dyn_smem[];
@@ -98,25 +101,23 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 
     const int m_tiles = (sh.m_size + BM - 1) / BM;
     const int c_tiles = (sh.c_size + BN - 1) / BN;
-    const int64_t n_tiles = MODE == MATRICES
-                                ? static_cast<int64_t>(sh.n_groups) * c_tiles * m_tiles
-                                : static_cast<int64_t>(segs.tiles[sh.n_groups + 2]) * m_tiles;
-    auto tile_at = [&](int64_t t) {
+    const int row_tiles = MODE == MATRICES ? sh.n_groups * c_tiles : segs.tiles[sh.n_groups + 2];
+    Walk walk(blockIdx.x, gridDim.x, row_tiles, m_tiles);
+    auto tile_at = [&]() {
         Tile r;
-        const int row = static_cast<int>(t / m_tiles);
-        r.m0 = static_cast<int>(t - static_cast<int64_t>(row) * m_tiles) * BM;
+        r.m0 = walk.col * BM;
         if (MODE == MATRICES) {
-            r.g = row / c_tiles;
-            r.c0 = (row - r.g * c_tiles) * BN;
+            r.g = walk.row / c_tiles;
+            r.c0 = (walk.row - r.g * c_tiles) * BN;
             r.c_end = sh.c_size;
             r.t0 = segs.edge[r.g + 1];
-            r.t_end = max(r.t0, segs.edge[r.g + 2]);
+            r.t_end = segs.edge[r.g + 2];
             r.out_row = static_cast<int64_t>(r.g) * sh.c_size + r.c0;
         } else {
-            const int lo = segs_find(segs, sh.n_groups, row);
-            r.g = lo >= 1 && lo <= sh.n_groups ? lo - 1 : -1;
-            r.c0 = segs.edge[lo] + (row - segs.tiles[lo]) * BN;
-            r.c_end = segs.edge[lo + 1];
+            const int seg = walk.segment(segs);
+            r.g = seg >= 1 && seg <= sh.n_groups ? seg - 1 : -1;
+            r.c0 = segs.edge[seg] + (walk.row - segs.tiles[seg]) * BN;
+            r.c_end = segs.edge[seg + 1];
             r.t0 = 0;
             r.t_end = r.g >= 0 ? sh.t_size : 0;
             r.out_row = r.c0;
@@ -127,8 +128,9 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
-            for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
-                const Tile tile = tile_at(t);
+            for (; walk.live() && !abort_s; walk.next()) {
+                const Tile tile = tile_at();
+                const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
                 for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                     const int s = it % STAGES;
                     if (it >= STAGES &&
@@ -139,20 +141,23 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     }
                     const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
                     const uint32_t bar = tc05::smem_u32(&full_bar[s]);
-                    tc05::mbar_expect_tx(bar, STAGE_BYTES);
+                    tc05::mbar_expect_tx(bar, A_BYTES + boxes * BOX_BYTES);
                     if (MODE == FORWARD) {
                         tc05::tma_load_3d(a, &map_a, t0, tile.m0, tile.g, bar);
-                        tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
                     } else if (MODE == ROWS) {
                         tc05::tma_load_3d(a, &map_a, tile.m0, t0, tile.g, bar);
                         tc05::tma_load_3d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, tile.g, bar);
-                        tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
                     } else {
                         tc05::tma_load_2d(a, &map_a, tile.m0, t0, bar);
                         tc05::tma_load_2d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, bar);
-#pragma unroll
-                        for (int j = 0; j < BN / 64; ++j)
-                            tc05::tma_load_2d(b + j * 8192, &map_b, tile.c0 + 64 * j, t0, bar);
+                    }
+                    if (MODE != MATRICES && boxes * BOX == BN) {
+                        tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
+                    } else {
+                        for (int j = 0; j < boxes; ++j)
+                            tc05::tma_load_2d(b + j * BOX_BYTES, &map_tail,
+                                              MODE == MATRICES ? tile.c0 + BOX * j : t0,
+                                              MODE == MATRICES ? t0 : tile.c0 + BOX * j, bar);
                     }
                 }
             }
@@ -163,11 +168,14 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc =
-            tc05::idesc_f16(sizeof(T) == 2 && is_bf16<T>(), A_MN, B_MN, BM, BN);
         uint32_t it = 0, acc_it = 0;
-        for (int64_t t = blockIdx.x; t < n_tiles && !abort_s; t += gridDim.x) {
-            const Tile tile = tile_at(t);
+        // of the first stage; a descriptor counts 16 bytes, so others are sums
+        const uint64_t desc_a = A_MN ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
+                                     : tc05::smem_desc_sw128(ring);
+        const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, 8192)
+                                     : tc05::smem_desc_sw128(ring + A_BYTES);
+        for (; walk.live() && !abort_s; walk.next()) {
+            const Tile tile = tile_at();
             if (tile.t0 >= tile.t_end) continue;
             const int slot = acc_it & 1;
             if (acc_it >= 2 &&
@@ -178,6 +186,9 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
             tc05::fence_after_sync();
             const uint32_t d = tmem + slot * BN;
+            const int cols = min(BN, tile.c_end - tile.c0);
+            const uint32_t idesc =
+                tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, (cols + 15) / 16 * 16);
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
                 if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
@@ -185,12 +196,12 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     abort_s = 1;
                     break;
                 }
-                const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                const uint32_t a = ring + s * STAGE_BYTES, off = s * (STAGE_BYTES / 16);
                 const int live = MODE == MATRICES ? min(BK, tile.t_end - t0) : BK;
                 if (MODE == MATRICES && live % 16 != 0) {
                     // rows of the next group up to the end of the last k step: 128 bytes each
                     const int dead = 16 - live % 16;
-                    for (int i = lane; i < dead * 8 * (2 + BN / 64); i += 32) {
+                    for (int i = lane; i < dead * 8 * (2 + (cols + 63) / 64); i += 32) {
                         const int chunk = i / (dead * 8), rest = i - chunk * dead * 8;
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
                                          a + chunk * 8192 + live * 128 + rest * 16),
@@ -205,12 +216,9 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k) {
                         if (16 * k < live) {
-                            const uint64_t da =
-                                A_MN ? tc05::smem_desc_mn_sw128(a + k * 2048, A_BYTES / 2)
-                                     : tc05::smem_desc_sw128(a + k * 32);
-                            const uint64_t db = B_MN ? tc05::smem_desc_mn_sw128(b + k * 2048, 8192)
-                                                     : tc05::smem_desc_sw128(b + k * 32);
-                            tc05::mma_f16(d, da, db, idesc, t0 > tile.t0 || k > 0);
+                            tc05::mma_f16(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
+                                          desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16), idesc,
+                                          t0 > tile.t0 || k > 0);
                         }
                     }
                     tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
@@ -229,8 +237,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         const uint32_t buf = ring + STAGES * STAGE_BYTES;
         constexpr int CHUNK = epilogue::cols(BN);
         uint32_t acc_it = 0, chunk = 0;
-        for (int64_t t = blockIdx.x; t < n_tiles; t += gridDim.x) {
-            const Tile tile = tile_at(t);
+        for (; walk.live(); walk.next()) {
+            const Tile tile = tile_at();
             const bool some = tile.t0 < tile.t_end;
             const int slot = acc_it & 1;
             bool ok = !abort_s;
@@ -267,7 +275,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 
 // ---- host -------------------------------------------------------------------------
 template <typename T, int MODE, int BN>
-int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
+int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &tail, const int64_t *offsets,
            const Shape &sh, int64_t most_tiles, cudaStream_t s) {
     static bool configured[64] = {};
     int dev = 0, sms = 0;
@@ -282,7 +290,7 @@ int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *of
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
     const unsigned grid = static_cast<unsigned>(most_tiles < sms ? most_tiles : sms);
-    mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, offsets, sh,
+    mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, tail, offsets, sh,
                                                                             status);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
@@ -316,17 +324,19 @@ template <typename T, int MODE, int BN>
 static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
                        int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw,
                        int64_t ldo, cudaStream_t s) {
-    CUtensorMap a, b;
+    CUtensorMap a, b, tail;
     const bool fwd = MODE == mma::FORWARD;
     int rc = map_matrices<T>(&a, w, fwd ? d_sum : d_out, fwd ? d_out : d_sum, n_groups,
                              ldw, fwd ? 128 : 64);
     if (rc != PA_OK) return rc;
     rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN);
     if (rc != PA_OK) return rc;
+    tail = b;
+    if (BN > 64 && (rc = map_rows<T>(&tail, in, d_sum, rows, ldi, 64)) != PA_OK) return rc;
     const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum, ldo,
                    aligned16(out) && ldo % 8 == 0 && d_out % 8 == 0};
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
-    return launch<T, MODE, BN>(out, a, b, offsets, sh, most, s);
+    return launch<T, MODE, BN>(out, a, b, tail, offsets, sh, most, s);
 }
 
 template <typename T, int MODE>
@@ -371,7 +381,7 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0, d, aligned16(dw) && d % 8 == 0};
     const int64_t most =
         static_cast<int64_t>(n_groups) * ((d + 127) / 128) * ((d_out + BN - 1) / BN);
-    return launch<T, mma::MATRICES, BN>(dw, a, b, offsets, sh, most, s);
+    return launch<T, mma::MATRICES, BN>(dw, a, b, b, offsets, sh, most, s);
 }
 
 template <typename T>

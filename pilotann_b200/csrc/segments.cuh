@@ -67,15 +67,27 @@ __device__ __forceinline__ void segs_make(Segments &s, const int64_t *offsets, i
     if (threadIdx.x == 0) s.tiles[segs] = carry;
 }
 
-// the segment that has row tile `tile`
-__device__ __forceinline__ int segs_find(const Segments &s, int n_groups, int tile) {
-    int lo = 0, hi = n_groups + 2;  // tiles[lo] <= tile < tiles[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s.tiles[mid] <= tile) lo = mid; else hi = mid;
+// The tiles of one CTA: every `step`-th of rows x n_col tiles, columns innermost, without a division
+// a tile; the segment of the row is looked for from the last one on.  (Results fit the memory, so
+// tile numbers fit 32 bits.)
+struct Walk {
+    int row, col, seg;
+    int step_row, step_col, n_col, n_row;
+
+    __device__ __forceinline__ Walk(int first, int step, int n_row_, int n_col_)
+        : row(first / n_col_), col(first % n_col_), seg(0), step_row(step / n_col_),
+          step_col(step % n_col_), n_col(n_col_), n_row(n_row_) {}
+    __device__ __forceinline__ bool live() const { return row < n_row; }
+    __device__ __forceinline__ void next() {
+        row += step_row;
+        col += step_col;
+        if (col >= n_col) { col -= n_col; ++row; }
     }
-    return lo;
-}
+    __device__ __forceinline__ int segment(const Segments &s) {
+        while (s.tiles[seg + 1] <= row) ++seg;
+        return seg;
+    }
+};
 
 }  // namespace grouped
 }  // namespace pa

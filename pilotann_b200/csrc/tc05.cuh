@@ -133,12 +133,13 @@ __device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t addr) {
     d |= static_cast<uint64_t>(1) << 46;
     return d;
 }
-// kind::mxf4 and kind::mxf4nvf4, both operands E2M1 and K-major, tile 128 x N, K = 64; `id`: which
-// byte of a 4-byte scale word the step starts at (same for A and B)
-__host__ __device__ constexpr uint32_t idesc_mxf4(bool e8m0, int N, uint32_t id) {
-    return (id << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
-           ((e8m0 ? 1u : 0u) << 23) | (1u << 27) | (id << 29);
+// kind::mxf4 and kind::mxf4nvf4, both operands E2M1 and K-major, tile 128 x N, K = 64
+__host__ __device__ constexpr uint32_t idesc_mxf4(bool e8m0, int N) {
+    return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+           ((e8m0 ? 1u : 0u) << 23) | (1u << 27);
 }
+// which byte of a 4-byte scale word the step starts at (same for A and B)
+__host__ __device__ constexpr uint32_t idesc_scale_id(uint32_t id) { return (id << 4) | (id << 29); }
 // kind::f16, fp32 accumulate; bf16 or fp16 operands, MN-major where said
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn, int M, int N) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
