@@ -22,8 +22,10 @@ namespace pa {
 namespace fp4 {
 
 using grouped::from_f32;
+using grouped::kNoTile;
 using grouped::Segments;
-using grouped::Walk;
+using grouped::Tile;
+using grouped::TileRing;
 
 namespace mma {
 constexpr int BM = 128, BK = 256;        // values; 128 bytes of codes
@@ -31,11 +33,11 @@ constexpr int A_BYTES = BM * BK / 2;
 constexpr int SCALE_SLOTS = 4;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_blocks(int bn) { return bn > 128 ? 2 : 1; }
-// Loader warps of a block of 128 rows of scales: each has two pieces of 16 bytes a row on their
-// way, about 1 us from DRAM, while a tile of short rows needs a piece every 0.6 us.
+// Loader warps of a block of 128 rows of scales: each has a piece of 16 bytes a row on its way,
+// about 1 us from DRAM, while a tile of short rows needs a piece every 0.6 us.
 __host__ __device__ constexpr int loaders(int bn) { return bn > 128 ? 3 : 4; }
 __host__ __device__ constexpr int threads(int bn) {
-    return 32 * (6 + (1 + b_blocks(bn)) * loaders(bn));
+    return 32 * (7 + (1 + b_blocks(bn)) * loaders(bn));
 }
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK / 2; }
 __host__ __device__ constexpr int scale_bytes(int bn) { return (1 + b_blocks(bn)) * 2048; }
@@ -119,6 +121,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_s;
     __shared__ Segments segs;
+    __shared__ TileRing tiles;
     __shared__ float t_scale_s[2][BM], q_scale_s[2][BN];  // nvfp4's row scales of two tiles
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
@@ -138,6 +141,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 4);
         }
         tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
+        grouped::ring_init(tiles, 6 + (1 + NB) * loaders(BN));
         abort_s = 0;
         tc05::fence_barrier_init();
         tc05::tma_prefetch_desc(&map_t);
@@ -151,16 +155,19 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     const uint32_t tmem = tmem_slot;
 
     const int m_tiles = static_cast<int>((args.d_out + BM - 1) / BM);
-    Walk walk(blockIdx.x, gridDim.x, segs.tiles[args.n_groups + 2], m_tiles);
     const int n_stages = (args.values + BK - 1) / BK;
-    struct Tile { int g, m0, c0, c_end; };
-    auto tile_at = [&]() {
+    const int row_tiles = segs.tiles[args.n_groups + 2];
+    auto make = [&](int index) {
         Tile r;
-        r.m0 = walk.col * BM;
-        const int seg = walk.segment(segs);
-        r.g = seg >= 1 && seg <= args.n_groups ? seg - 1 : -1;  // -1: rows of no group, zeros
-        r.c0 = segs.edge[seg] + (walk.row - segs.tiles[seg]) * BN;
+        const int row = index / m_tiles;
+        r.g = kNoTile;
+        if (row >= row_tiles) return r;
+        r.m0 = (index - row * m_tiles) * BM;
+        const int seg = grouped::segs_find(segs, args.n_groups, row);
+        r.g = seg >= 1 && seg <= args.n_groups ? seg - 1 : -1;
+        r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
         r.c_end = segs.edge[seg + 1];
+        r.t0 = r.t_end = 0;
         return r;
     };
 
@@ -168,8 +175,8 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // ---- codes ----
         if (lane == 0) {
             uint32_t it = 0;
-            for (; walk.live() && !abort_s; walk.next()) {
-                const Tile tile = tile_at();
+            Tile tile;
+            for (uint32_t n = 0; grouped::ring_take<false>(tiles, abort_s, n, tile); ++n) {
                 if (tile.g < 0) continue;
                 const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
                 for (int k = 0; k < n_stages; ++k, ++it) {
@@ -206,8 +213,8 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             // of the first stage and slot; a descriptor counts 16 bytes, so others are sums
             const uint64_t desc_a = tc05::smem_desc_sw128(ring);
             const uint64_t desc_s = tc05::smem_desc_rows16(scale_ring);
-            for (; walk.live() && !abort_s; walk.next()) {
-                const Tile tile = tile_at();
+            Tile tile;
+            for (uint32_t n = 0; grouped::ring_take<false>(tiles, abort_s, n, tile); ++n) {
                 if (tile.g < 0) continue;
                 const int acc = acc_it & 1;
                 if (acc_it >= 2 && !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[acc]),
@@ -276,6 +283,9 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
             }
         }
+    } else if (warp == THREADS / 32 - 1) {
+        if (lane == 0)
+            grouped::ring_serve(tiles, abort_s, grouped::ring_depth(n_stages, STAGES), make);
     } else if (warp < 4 || warp >= 8) {
         // ---- scales: block 0 the table's 128 rows, 1 and 2 the queries' ----
         const int li = warp < 4 ? warp - 2 : warp - 6;
@@ -287,12 +297,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         Tile tile = {};
         const uint8_t *row[4];
         bool live[4];
+        uint32_t n = 0;
         auto rows_of_tile = [&]() {  // skips tiles without a group; false at the end
-            for (; walk.live(); walk.next()) {
-                tile = tile_at();
-                if (tile.g >= 0) break;
-            }
-            if (!walk.live()) return false;
+            do {
+                if (!grouped::ring_take<true>(tiles, abort_s, n++, tile)) return false;
+            } while (tile.g < 0);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const int r = 32 * b + lane;
@@ -312,7 +321,6 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         auto settle = [&]() {
             while (piece >= n_pieces) {
                 piece -= n_pieces;
-                walk.next();
                 if (!rows_of_tile()) return false;
             }
             return true;
@@ -324,21 +332,15 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
 #pragma unroll
             for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
         }
-        for (uint32_t sg = piece0; more && !abort_s; sg += loaders(BN)) {
+        for (uint32_t sg = piece0; more; sg += loaders(BN)) {
             uint4 v[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) v[b] = scales_take(next[b], row[b], at, pitch);
-            piece += loaders(BN);
-            more = settle();
-            at = 16 * piece;
-            if (more) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
-            }
             const int slot = sg % SCALE_SLOTS;
             if (sg >= SCALE_SLOTS &&
-                !tc05::mbar_wait_bounded(tc05::smem_u32(&sc_empty[slot]),
-                                         (sg / SCALE_SLOTS - 1) & 1, WAIT_LIMIT)) {
+                !__all_sync(0xffffffffu,
+                            tc05::mbar_wait_bounded(tc05::smem_u32(&sc_empty[slot]),
+                                                    (sg / SCALE_SLOTS - 1) & 1, WAIT_LIMIT))) {
                 abort_s = 1;
                 break;
             }
@@ -355,6 +357,14 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             tc05::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&sc_full[slot]));
+            // only now: the tile of the next piece may have to wait for this one's product
+            piece += loaders(BN);
+            more = settle();
+            at = 16 * piece;
+            if (more) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
+            }
         }
     } else {
         // ---- results: warp w has lanes 32 (w - 4) .. of the accumulator ----
@@ -362,9 +372,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         const uint32_t buf = scale_ring + SCALE_SLOTS * SLOT_BYTES;
         constexpr int CHUNK = epilogue::cols(BN);
         uint32_t acc_it = 0, n_tile = 0, chunk = 0;
-        for (; walk.live(); walk.next(), ++n_tile) {
-            const Tile tile = tile_at();
-            const bool some = tile.g >= 0;
+        for (;; ++n_tile) {
+            // the four warps must agree on what they do: they meet at barriers below
+            Tile tile;
+            bool ok = grouped::ring_take<true>(tiles, abort_s, n_tile, tile);
+            const bool some = ok && tile.g >= 0;
             const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
             const float *ts = t_scale_s[n_tile & 1], *qs = q_scale_s[n_tile & 1];
             if (METHOD == PA_NVFP4 && some) {
@@ -374,14 +386,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 for (int c = own; c < BN; c += 128)
                     q_scale_s[n_tile & 1][c] = c < live ? __ldg(args.q_row_scale + tile.c0 + c) : 0.0f;
             }
-            bool ok = !abort_s;
-            if (some && ok)
+            if (some)
                 ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT);
-            if (!epilogue::all_agree(ok)) {
-                abort_s = 1;
-                break;
-            }
+                                             WAIT_LIMIT) || (abort_s = 1, false);
+            __syncwarp();
+            if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
             const int m_left = static_cast<int>(min(args.d_out - tile.m0, static_cast<int64_t>(BM)));
             const int64_t first = tile.c0 * args.d_out + tile.m0;
@@ -465,9 +474,8 @@ template <int METHOD, int BN>
 static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t_codes,
                       cudaStream_t s) {
     static bool configured[64] = {};
-    int dev = 0, sms = 0;
+    int dev = 0;
     PA_CUDA_TRY(cudaGetDevice(&dev));
-    PA_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     if (dev < 64 && !configured[dev]) {
         PA_CUDA_TRY(cudaFuncSetAttribute(project_kernel<METHOD, BN>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -484,7 +492,8 @@ static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t
         return rc;
     const int64_t most = (static_cast<int64_t>(args.rows) / BN + args.n_groups + 2) *
                          ((args.d_out + mma::BM - 1) / mma::BM);
-    const unsigned grid = static_cast<unsigned>(most < sms ? most : sms);
+    PA_REQUIRE(most <= 0x7fffffff, "too many rows for one call");
+    const unsigned grid = static_cast<unsigned>(most);
     project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q, tail,
                                                                                    args);
     count_launch();

@@ -13,9 +13,9 @@
 // the last slice belongs to the next group and is cleared in shared memory, in both operands,
 // so that a NaN there stays there.
 //
-// Persistent CTAs; warp 0 keeps bulk-tensor copies ahead, warp 1 issues the MMAs, warps 4-7 store
-// the tile before while the next is multiplied (two accumulators in TMEM).  Every wait is
-// bounded.
+// Persistent CTAs; warp 2 takes tiles (segments.cuh), warp 0 keeps bulk-tensor copies ahead, warp 1
+// issues the MMAs, warps 4-7 store the tile before while the next is multiplied (two accumulators in
+// TMEM).  Every wait is bounded.
 #include "epilogue.cuh"
 #include "grouped.cuh"
 #include "segments.cuh"
@@ -49,13 +49,11 @@ struct Shape {
     bool vec;         // result rows start on 16 bytes and are whole pieces of 16
 };
 
-struct Tile {
-    int g;            // group, or -1: rows of no group, zeros
-    int m0;           // first of 128 along the contiguous axis
-    int c0, c_end;    // rows of the result: c0 .. min(c0 + BN, c_end)
-    int t0, t_end;    // summed axis
-    int64_t out_row;  // row of the result that column 0 is
-};
+// all lanes of the warp: the same answer for each of them
+__device__ __forceinline__ bool warp_wait(const uint64_t *bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, tc05::mbar_wait_bounded(tc05::smem_u32(bar), parity,
+                                                           mma::WAIT_LIMIT));
+}
 
 template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(mma::THREADS, 1)
@@ -74,6 +72,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_s;
     __shared__ Segments segs;
+    __shared__ TileRing tiles;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
 
@@ -87,6 +86,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 4);
         }
         tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
+        ring_init(tiles, 6);
         abort_s = 0;
         tc05::fence_barrier_init();
         tc05::tma_prefetch_desc(&map_a);
@@ -102,25 +102,25 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     const int m_tiles = (sh.m_size + BM - 1) / BM;
     const int c_tiles = (sh.c_size + BN - 1) / BN;
     const int row_tiles = MODE == MATRICES ? sh.n_groups * c_tiles : segs.tiles[sh.n_groups + 2];
-    Walk walk(blockIdx.x, gridDim.x, row_tiles, m_tiles);
-    auto tile_at = [&]() {
+    auto make = [&](int index) {
         Tile r;
-        r.m0 = walk.col * BM;
+        const int row = index / m_tiles;
+        r.g = kNoTile;
+        if (row >= row_tiles) return r;
+        r.m0 = (index - row * m_tiles) * BM;
         if (MODE == MATRICES) {
-            r.g = walk.row / c_tiles;
-            r.c0 = (walk.row - r.g * c_tiles) * BN;
+            r.g = row / c_tiles;
+            r.c0 = (row - r.g * c_tiles) * BN;
             r.c_end = sh.c_size;
             r.t0 = segs.edge[r.g + 1];
             r.t_end = segs.edge[r.g + 2];
-            r.out_row = static_cast<int64_t>(r.g) * sh.c_size + r.c0;
         } else {
-            const int seg = walk.segment(segs);
+            const int seg = segs_find(segs, sh.n_groups, row);
             r.g = seg >= 1 && seg <= sh.n_groups ? seg - 1 : -1;
-            r.c0 = segs.edge[seg] + (walk.row - segs.tiles[seg]) * BN;
+            r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
             r.c_end = segs.edge[seg + 1];
             r.t0 = 0;
             r.t_end = r.g >= 0 ? sh.t_size : 0;
-            r.out_row = r.c0;
         }
         return r;
     };
@@ -128,8 +128,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
-            for (; walk.live() && !abort_s; walk.next()) {
-                const Tile tile = tile_at();
+            Tile tile;
+            for (uint32_t n = 0; ring_take<false>(tiles, abort_s, n, tile); ++n) {
                 const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
                 for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                     const int s = it % STAGES;
@@ -174,13 +174,11 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                                      : tc05::smem_desc_sw128(ring);
         const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, 8192)
                                      : tc05::smem_desc_sw128(ring + A_BYTES);
-        for (; walk.live() && !abort_s; walk.next()) {
-            const Tile tile = tile_at();
+        Tile tile;
+        for (uint32_t n = 0; ring_take<true>(tiles, abort_s, n, tile); ++n) {
             if (tile.t0 >= tile.t_end) continue;
             const int slot = acc_it & 1;
-            if (acc_it >= 2 &&
-                !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[slot]), (acc_it / 2 - 1) & 1,
-                                         WAIT_LIMIT)) {
+            if (acc_it >= 2 && !warp_wait(&acc_empty[slot], (acc_it / 2 - 1) & 1)) {
                 abort_s = 1;
                 break;
             }
@@ -191,8 +189,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, (cols + 15) / 16 * 16);
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
-                if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
-                                             WAIT_LIMIT)) {
+                if (!warp_wait(&full_bar[s], (it / STAGES) & 1)) {
                     abort_s = 1;
                     break;
                 }
@@ -228,30 +225,37 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
             ++acc_it;
         }
+        __syncwarp();
         if (abort_s && lane == 0) {  // nor does a product read on
             tc05::mma_commit(tc05::smem_u32(&quit_bar));
             tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
+        }
+    } else if (warp == 2) {
+        if (lane == 0) {
+            const int sum = MODE == MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
+            ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), make);
         }
     } else if (warp >= 4) {
         const int w = warp - 4;
         const uint32_t buf = ring + STAGES * STAGE_BYTES;
         constexpr int CHUNK = epilogue::cols(BN);
         uint32_t acc_it = 0, chunk = 0;
-        for (; walk.live(); walk.next()) {
-            const Tile tile = tile_at();
-            const bool some = tile.t0 < tile.t_end;
+        for (uint32_t n = 0;; ++n) {
+            // the four warps must agree on what they do: they meet at barriers below
+            Tile tile;
+            bool ok = ring_take<true>(tiles, abort_s, n, tile);
+            const bool some = ok && tile.t0 < tile.t_end;
             const int slot = acc_it & 1;
-            bool ok = !abort_s;
-            if (some && ok)
+            if (some)
                 ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT);
-            if (!epilogue::all_agree(ok)) {
-                abort_s = 1;
-                break;
-            }
+                                             WAIT_LIMIT) || (abort_s = 1, false);
+            __syncwarp();
+            if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
             const int live = min(BN, tile.c_end - tile.c0);
-            T *dst = out + tile.out_row * sh.ldo + tile.m0;
+            const int64_t first =
+                (MODE == MATRICES ? static_cast<int64_t>(tile.g) * sh.c_size : 0) + tile.c0;
+            T *dst = out + first * sh.ldo + tile.m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
                 epilogue::store_chunk<T, CHUNK>(
@@ -278,9 +282,8 @@ template <typename T, int MODE, int BN>
 int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &tail, const int64_t *offsets,
            const Shape &sh, int64_t most_tiles, cudaStream_t s) {
     static bool configured[64] = {};
-    int dev = 0, sms = 0;
+    int dev = 0;
     PA_CUDA_TRY(cudaGetDevice(&dev));
-    PA_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     if (dev < 64 && !configured[dev]) {
         PA_CUDA_TRY(cudaFuncSetAttribute(mma_kernel<T, MODE, BN>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -289,7 +292,8 @@ int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap
     }
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
-    const unsigned grid = static_cast<unsigned>(most_tiles < sms ? most_tiles : sms);
+    PA_REQUIRE(most_tiles <= 0x7fffffff, "too many rows for one call");
+    const unsigned grid = static_cast<unsigned>(most_tiles);
     mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, tail, offsets, sh,
                                                                             status);
     count_launch();

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "grouped.cuh"
+#include "tc05.cuh"
 
 namespace pa {
 namespace grouped {
@@ -67,27 +68,125 @@ __device__ __forceinline__ void segs_make(Segments &s, const int64_t *offsets, i
     if (threadIdx.x == 0) s.tiles[segs] = carry;
 }
 
-// The tiles of one CTA: every `step`-th of rows x n_col tiles, columns innermost, without a division
-// a tile; the segment of the row is looked for from the last one on.  (Results fit the memory, so
-// tile numbers fit 32 bits.)
-struct Walk {
-    int row, col, seg;
-    int step_row, step_col, n_col, n_row;
-
-    __device__ __forceinline__ Walk(int first, int step, int n_row_, int n_col_)
-        : row(first / n_col_), col(first % n_col_), seg(0), step_row(step / n_col_),
-          step_col(step % n_col_), n_col(n_col_), n_row(n_row_) {}
-    __device__ __forceinline__ bool live() const { return row < n_row; }
-    __device__ __forceinline__ void next() {
-        row += step_row;
-        col += step_col;
-        if (col >= n_col) { col -= n_col; ++row; }
-    }
-    __device__ __forceinline__ int segment(const Segments &s) {
-        while (s.tiles[seg + 1] <= row) ++seg;
-        return seg;
-    }
+// ---- tiles handed out while the kernel runs ----------------------------------------
+// The grid has a CTA per tile that the offsets could make; one CTA fits an SM.  A CTA works on its own
+// tile and then takes over the tile of a CTA that has not started (cluster launch control), until
+// there is none: SMs finish 15 to 25 % apart where tiles differ or the memory serves some SMs
+// sooner, and a fixed share of the tiles each waited for the slowest.  One warp asks, works the tile
+// out and leaves it in a ring for the warps that load, multiply and store.  It asks as late as the loads
+// allow: a tile taken early is one that an idle SM cannot have.
+struct Tile {
+    int g;            // group; -1: rows of no group, zeros; kNoTile: there are no more
+    int m0;           // first of 128 along the contiguous axis of the result
+    int c0, c_end;    // its rows: c0 .. min(c0 + BN, c_end)
+    int t0, t_end;    // summed axis
 };
+constexpr int kNoTile = -2;
+constexpr uint32_t kTileWait = 1u << 22;
+
+struct TileRing {
+    __align__(16) uint4 answer;
+    __align__(16) int4 a[4];
+    int2 b[4];
+    __align__(8) uint64_t full[4], empty[4], answered;
+};
+
+// Tiles known ahead of the slowest reader, for tiles of `slices` slices and a ring of `stages`: the
+// loads run `stages` slices ahead, and an answer takes about 1 us.
+__device__ __forceinline__ int ring_depth(int slices, int stages) {
+    return min(4, 1 + 3 * stages / max(1, slices));
+}
+
+// one thread, before the barrier behind which the ring is used; readers: arrivals a tile gets
+__device__ __forceinline__ void ring_init(TileRing &r, int readers) {
+    for (int i = 0; i < 4; ++i) {
+        tc05::mbar_init(tc05::smem_u32(&r.full[i]), 1);
+        tc05::mbar_init(tc05::smem_u32(&r.empty[i]), readers);
+    }
+    tc05::mbar_init(tc05::smem_u32(&r.answered), 1);
+}
+
+// One thread hands out tiles: make(index) is the tile, or has g == kNoTile for an index that the
+// offsets do not reach.
+template <typename Make>
+__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, Make make) {
+    const uint32_t answer = tc05::smem_u32(&r.answer), bar = tc05::smem_u32(&r.answered);
+    int index = blockIdx.x;
+    uint32_t n = 0;
+    for (uint32_t asked = 0;; ++asked) {
+        const Tile tile = make(index);
+        if (tile.g != kNoTile) {
+            r.a[n & 3] = make_int4(tile.g, tile.m0, tile.c0, tile.c_end);
+            r.b[n & 3] = make_int2(tile.t0, tile.t_end);
+            tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));
+            ++n;
+            // room for the next one: tile n - depth has been taken by all
+            const uint32_t old = n - depth;
+            if (n >= static_cast<uint32_t>(depth) &&
+                !tc05::mbar_wait_bounded(tc05::smem_u32(&r.empty[old & 3]), (old / 4) & 1, kTileWait))
+                abort_s = 1;
+        }
+        if (abort_s) break;
+        tc05::mbar_expect_tx(bar, 16);
+        asm volatile(
+            "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+            "[%0], [%1];" ::"r"(answer), "r"(bar)
+            : "memory");
+        if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) {
+            abort_s = 1;
+            break;
+        }
+        uint32_t more, next;
+        asm volatile(
+            "{\n"
+            ".reg .b128 h;\n"
+            ".reg .pred p;\n"
+            "ld.shared.b128 h, [%2];\n"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "mov.u32 %1, 0;\n"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n"
+            "}\n"
+            : "=r"(more), "=r"(next)
+            : "r"(answer)
+            : "memory");
+        tc05::fence_proxy_async_smem();  // the answer has been read before the next one is written
+        if (!more) break;
+        index = static_cast<int>(next);
+    }
+    r.a[n & 3] = make_int4(kNoTile, 0, 0, 0);
+    tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));
+}
+
+// A reader's side: the n-th tile of this CTA.  A thread for itself, or (WARP) a whole warp.
+// false: no more, or gave up.
+template <bool WARP>
+__device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, uint32_t n, Tile &tile) {
+    const int slot = n & 3;
+    bool ok = tc05::mbar_wait_bounded(tc05::smem_u32(&r.full[slot]), (n / 4) & 1, kTileWait) &&
+              !abort_s;
+    if (WARP) ok = __all_sync(0xffffffffu, ok);  // lanes that gave up must not leave others behind
+    if (!ok) {
+        abort_s = 1;
+        return false;
+    }
+    const int4 a = r.a[slot];
+    const int2 b = r.b[slot];
+    if (WARP) __syncwarp();
+    if (!WARP || (threadIdx.x & 31) == 0) tc05::mbar_arrive(tc05::smem_u32(&r.empty[slot]));
+    tile = Tile{a.x, a.y, a.z, a.w, b.x, b.y};
+    return a.x != kNoTile;
+}
+
+// the segment that has row tile `tile`
+__device__ __forceinline__ int segs_find(const Segments &s, int n_groups, int tile) {
+    int lo = 0, hi = n_groups + 2;  // tiles[lo] <= tile < tiles[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s.tiles[mid] <= tile) lo = mid; else hi = mid;
+    }
+    return lo;
+}
 
 }  // namespace grouped
 }  // namespace pa
