@@ -7,10 +7,12 @@
 //
 // Codes come by bulk-tensor copies, 256 values (128 bytes) of every row a stage.  Scales are
 // row-major bytes in memory, while the instruction wants, for 128 rows and four bytes each,
-// word (r % 32, r / 32) in TMEM: a loader warp takes 16 bytes of rows l, l + 32, l + 64,
-// l + 96 per lane (512 values of mxfp4, 256 of nvfp4), which is a 4 x 4 transpose in its
-// registers, stores four 16-byte rows without bank conflicts, and tcgen05.cp spreads them.
-// nvfp4's row scales, powers of two, multiply the finished sum.
+// word (r % 32, r / 32) in TMEM, in each quarter of the lanes: a loader warp takes 16 bytes of rows
+// l, l + 32, l + 64, l + 96 per lane (512 values of mxfp4, 256 of nvfp4), which is a 4 x 4 transpose
+// in its registers, and stores four 16-byte rows without bank conflicts; four writer warps, one a
+// quarter, take them to TMEM.  (tcgen05.cp from the issuing thread does the same, but each one, four
+// columns, kept the thread and the products behind it for 160 cycles: 12 of them on 8 products, which
+// take 96 each.  16384 x 4096 against 8192 rows took 458 us that way.)  nvfp4's row scales, powers of two, multiply the finished sum.
 #include "epilogue.cuh"
 #include "fp4.cuh"
 #include "grouped.cuh"
@@ -35,10 +37,12 @@ constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_blocks(int bn) { return bn > 128 ? 2 : 1; }
 // Loader warps of a block of 128 rows of scales: each has a piece of 16 bytes a row on its way,
 // about 1 us from DRAM, while a tile of short rows needs a piece every 0.6 us.
-__host__ __device__ constexpr int loaders(int bn) { return bn > 128 ? 3 : 4; }
+__host__ __device__ constexpr int loaders(int bn) { return bn > 128 ? 2 : 3; }
+// warps 0 codes, 1 products, 2 tiles, 4-7 results, 8-11 scales to TMEM, 12 on loaders of scales
 __host__ __device__ constexpr int threads(int bn) {
-    return 32 * (7 + (1 + b_blocks(bn)) * loaders(bn));
+    return 32 * (12 + (1 + b_blocks(bn)) * loaders(bn));
 }
+__host__ __device__ constexpr int scale_buffers(int bn) { return bn > 128 ? 2 : 4; }  // in TMEM
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK / 2; }
 __host__ __device__ constexpr int scale_bytes(int bn) { return (1 + b_blocks(bn)) * 2048; }
 __host__ __device__ constexpr int stages(int bn) {
@@ -58,6 +62,7 @@ struct Args {
     int64_t d_out;
     int rows, n_groups, values;          // values of a row, padded to 32
     int q_pitch, t_pitch;                // bytes of scales from row to row
+    int unit;                            // tiles a CTA takes at a time
     int out_dtype;
     bool vec;                            // 16-bit result rows are whole pieces of 16 bytes
     int *status;
@@ -112,12 +117,12 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     constexpr int SCALE_COLS = 16 * (1 + NB);
     constexpr int BOX = BN < 64 ? BN : 64, BOX_BYTES = BOX * BK / 2;  // of the queries' codes
     constexpr int ACC_COLS = 2 * BN;
-    constexpr uint32_t COLS = ACC_COLS + 2 * SCALE_COLS <= 128 ? 128
-                              : ACC_COLS + 2 * SCALE_COLS <= 256 ? 256 : 512;
-    static_assert(ACC_COLS + 2 * SCALE_COLS <= 512, "TMEM has 512 columns");
+    constexpr int BUFS = scale_buffers(BN), ALL_COLS = ACC_COLS + BUFS * SCALE_COLS;
+    constexpr uint32_t COLS = ALL_COLS <= 256 ? 256 : 512;
+    static_assert(ALL_COLS <= 512, "TMEM has 512 columns");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], sc_full[SCALE_SLOTS],
-        sc_empty[SCALE_SLOTS], acc_full[2], acc_empty[2], quit_bar;
+        sc_empty[SCALE_SLOTS], tm_full[BUFS], tm_empty[BUFS], acc_full[2], acc_empty[2], quit_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_s;
     __shared__ Segments segs;
@@ -134,14 +139,18 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         }
         for (int s = 0; s < SCALE_SLOTS; ++s) {
             tc05::mbar_init(tc05::smem_u32(&sc_full[s]), 1 + NB);
-            tc05::mbar_init(tc05::smem_u32(&sc_empty[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&sc_empty[s]), 4);
+        }
+        for (int s = 0; s < BUFS; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&tm_full[s]), 4);
+            tc05::mbar_init(tc05::smem_u32(&tm_empty[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
             tc05::mbar_init(tc05::smem_u32(&acc_full[s]), 1);
             tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 4);
         }
         tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
-        grouped::ring_init(tiles, 6 + (1 + NB) * loaders(BN));
+        grouped::ring_init(tiles, 10 + (1 + NB) * loaders(BN));
         abort_s = 0;
         tc05::fence_barrier_init();
         tc05::tma_prefetch_desc(&map_t);
@@ -210,9 +219,8 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // ---- products ----
         if (lane == 0) {
             uint32_t it = 0, sg = 0, acc_it = 0;
-            // of the first stage and slot; a descriptor counts 16 bytes, so others are sums
+            // of the first stage; a descriptor counts 16 bytes, so others are sums
             const uint64_t desc_a = tc05::smem_desc_sw128(ring);
-            const uint64_t desc_s = tc05::smem_desc_rows16(scale_ring);
             Tile tile;
             for (uint32_t n = 0; grouped::ring_take<false>(tiles, abort_s, n, tile); ++n) {
                 if (tile.g < 0) continue;
@@ -229,31 +237,20 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     tc05::idesc_mxf4(METHOD == PA_MXFP4, (cols + 15) / 16 * 16);
                 uint32_t sa = 0, sb = 0;
                 for (int k = 0; k < n_stages; ++k, ++it) {
-                    const int s = it % STAGES, slot = sg % SCALE_SLOTS;
+                    const int s = it % STAGES, buf = sg % BUFS;
                     if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
                                                  WAIT_LIMIT)) {
                         abort_s = 1;
                         break;
                     }
                     if (k % GROUP == 0) {
-                        if (!tc05::mbar_wait_bounded(tc05::smem_u32(&sc_full[slot]),
-                                                     (sg / SCALE_SLOTS) & 1, WAIT_LIMIT)) {
+                        if (!tc05::mbar_wait_bounded(tc05::smem_u32(&tm_full[buf]), (sg / BUFS) & 1,
+                                                     WAIT_LIMIT)) {
                             abort_s = 1;
                             break;
                         }
-                        tc05::fence_after_sync();
-                        sa = tmem + ACC_COLS + (sg & 1) * SCALE_COLS;
+                        sa = tmem + ACC_COLS + buf * SCALE_COLS;
                         sb = sa + 16;
-                        const uint64_t from = desc_s + slot * (SLOT_BYTES / 16);
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            tc05::tmem_cp_scales(sa + 4 * w, from + 32 * w);
-#pragma unroll
-                            for (int j = 0; j < NB; ++j)
-                                if (j == 0 || cols > 128) tc05::tmem_cp_scales(
-                                    sb + 4 * (NB * w + j),
-                                    from + 128 * (1 + j) + 32 * w);
-                        }
                     }
                     tc05::fence_after_sync();
                     const uint64_t a = desc_a + s * (STAGE_BYTES / 16), b = a + A_BYTES / 16;
@@ -271,7 +268,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     }
                     tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
                     if (k % GROUP == GROUP - 1 || k + 1 == n_stages) {
-                        tc05::mma_commit(tc05::smem_u32(&sc_empty[slot]));
+                        tc05::mma_commit(tc05::smem_u32(&tm_empty[buf]));
                         ++sg;
                     }
                 }
@@ -283,12 +280,71 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
             }
         }
-    } else if (warp == THREADS / 32 - 1) {
+    } else if (warp == 2) {
         if (lane == 0)
-            grouped::ring_serve(tiles, abort_s, grouped::ring_depth(n_stages, STAGES), make);
-    } else if (warp < 4 || warp >= 8) {
+            grouped::ring_serve(tiles, abort_s, grouped::ring_depth(n_stages, STAGES), args.unit,
+                                make);
+    } else if (warp >= 8 && warp < 12) {
+        // ---- scales to TMEM: lanes 32 (w % 4) on, for all the products of this CTA ----
+        const uint32_t quarter = (32u * (warp & 3)) << 16;
+        const int n_pieces = (n_stages + GROUP - 1) / GROUP;
+        Tile tile;
+        uint32_t sg = 0;
+        bool ok = true;
+        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            if (tile.g < 0) continue;
+            for (int piece = 0; piece < n_pieces; ++piece, ++sg) {
+                const int slot = sg % SCALE_SLOTS, buf = sg % BUFS;
+                ok = __all_sync(0xffffffffu,
+                                tc05::mbar_wait_bounded(tc05::smem_u32(&sc_full[slot]),
+                                                        (sg / SCALE_SLOTS) & 1, WAIT_LIMIT));
+                if (!ok) break;
+                uint32_t r[1 + NB][16];
+                const uint32_t from = scale_ring + slot * SLOT_BYTES + 16 * lane;
+#pragma unroll
+                for (int j = 0; j <= NB; ++j)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(r[j][4 * w]), "=r"(r[j][4 * w + 1]),
+                                       "=r"(r[j][4 * w + 2]), "=r"(r[j][4 * w + 3])
+                                     : "r"(from + 2048 * j + 512 * w)
+                                     : "memory");
+                if (sg >= BUFS)
+                    ok = __all_sync(0xffffffffu,
+                                    tc05::mbar_wait_bounded(tc05::smem_u32(&tm_empty[buf]),
+                                                            (sg / BUFS - 1) & 1, WAIT_LIMIT));
+                if (!ok) break;
+                tc05::fence_after_sync();
+                const uint32_t to = tmem + ACC_COLS + buf * SCALE_COLS + quarter;
+                tc05::tmem_st_32x16(to, r[0]);
+                if constexpr (NB == 1) {
+                    tc05::tmem_st_32x16(to + 16, r[1]);
+                } else {  // word w of both blocks side by side
+                    uint32_t q[2][16];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            q[w / 2][8 * (w % 2) + i] = r[1][4 * w + i];
+                            q[w / 2][8 * (w % 2) + 4 + i] = r[NB][4 * w + i];
+                        }
+                    tc05::tmem_st_32x16(to + 16, q[0]);
+                    tc05::tmem_st_32x16(to + 32, q[1]);
+                }
+                tc05::tmem_st_wait();
+                tc05::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    tc05::mbar_arrive(tc05::smem_u32(&sc_empty[slot]));
+                    tc05::mbar_arrive(tc05::smem_u32(&tm_full[buf]));
+                }
+            }
+        }
+        if (!ok) abort_s = 1;
+    } else if (warp >= 12) {
         // ---- scales: block 0 the table's 128 rows, 1 and 2 the queries' ----
-        const int li = warp < 4 ? warp - 2 : warp - 6;
+        const int li = warp - 12;
         const int block = li % (1 + NB);
         const int pitch = block == 0 ? args.t_pitch : args.q_pitch;
         const int n_pieces = (n_stages + GROUP - 1) / GROUP;
@@ -354,7 +410,6 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512 * i),
                              "r"(w[i][0]), "r"(w[i][1]), "r"(w[i][2]), "r"(w[i][3])
                              : "memory");
-            tc05::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&sc_full[slot]));
             // only now: the tile of the next piece may have to wait for this one's product
@@ -366,7 +421,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                 for (int b = 0; b < 4; ++b) next[b] = scales_fetch(row[b], at, pitch, live[b]);
             }
         }
-    } else {
+    } else if (warp >= 4) {
         // ---- results: warp w has lanes 32 (w - 4) .. of the accumulator ----
         const int w = warp - 4, own = 32 * w + lane;
         const uint32_t buf = scale_ring + SCALE_SLOTS * SLOT_BYTES;
@@ -471,7 +526,7 @@ static int map_codes(CUtensorMap *map, const uint8_t *codes, int values, int64_t
 }
 
 template <int METHOD, int BN>
-static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t_codes,
+static int project_bn(Args args, const uint8_t *q_codes, const uint8_t *t_codes,
                       cudaStream_t s) {
     static bool configured[64] = {};
     int dev = 0;
@@ -493,7 +548,8 @@ static int project_bn(const Args &args, const uint8_t *q_codes, const uint8_t *t
     const int64_t most = (static_cast<int64_t>(args.rows) / BN + args.n_groups + 2) *
                          ((args.d_out + mma::BM - 1) / mma::BM);
     PA_REQUIRE(most <= 0x7fffffff, "too many rows for one call");
-    const unsigned grid = static_cast<unsigned>(most);
+    args.unit = grouped::tiles_per_unit(most, (args.values + mma::BK - 1) / mma::BK);
+    const unsigned grid = static_cast<unsigned>((most + args.unit - 1) / args.unit);
     project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q, tail,
                                                                                    args);
     count_launch();
@@ -539,7 +595,7 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     const int values = static_cast<int>(fp4::padded(d));
     const int pitch = values / fp4::block_of(method);
     const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,
-                         static_cast<int>(rows), n_groups, values, pitch, pitch, out_dtype,
+                         static_cast<int>(rows), n_groups, values, pitch, pitch, 1, out_dtype,
                          aligned16(out) && d_out % 8 == 0, status};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return method == PA_MXFP4

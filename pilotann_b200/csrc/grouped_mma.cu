@@ -45,6 +45,7 @@ struct Shape {
     int m_size;       // of D: contiguous axis
     int c_size;       // MATRICES: rows of one matrix
     int t_size;       // FORWARD, ROWS: summed axis
+    int unit;         // tiles a CTA takes at a time
     int64_t ldo;
     bool vec;         // result rows start on 16 bytes and are whole pieces of 16
 };
@@ -233,7 +234,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     } else if (warp == 2) {
         if (lane == 0) {
             const int sum = MODE == MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
-            ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), make);
+            ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), sh.unit,
+                       make);
         }
     } else if (warp >= 4) {
         const int w = warp - 4;
@@ -293,7 +295,7 @@ int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
     PA_REQUIRE(most_tiles <= 0x7fffffff, "too many rows for one call");
-    const unsigned grid = static_cast<unsigned>(most_tiles);
+    const unsigned grid = static_cast<unsigned>((most_tiles + sh.unit - 1) / sh.unit);
     mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, tail, offsets, sh,
                                                                             status);
     count_launch();
@@ -337,9 +339,10 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
     if (rc != PA_OK) return rc;
     tail = b;
     if (BN > 64 && (rc = map_rows<T>(&tail, in, d_sum, rows, ldi, 64)) != PA_OK) return rc;
-    const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum, ldo,
-                   aligned16(out) && ldo % 8 == 0 && d_out % 8 == 0};
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
+    const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum,
+                   tiles_per_unit(most, (d_sum + mma::BK - 1) / mma::BK), ldo,
+                   aligned16(out) && ldo % 8 == 0 && d_out % 8 == 0};
     return launch<T, MODE, BN>(out, a, b, tail, offsets, sh, most, s);
 }
 
@@ -382,9 +385,12 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     if (rc != PA_OK) return rc;
     rc = map_rows<T>(&b, dy, d_out, rows, ldy, 64);
     if (rc != PA_OK) return rc;
-    const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0, d, aligned16(dw) && d % 8 == 0};
     const int64_t most =
         static_cast<int64_t>(n_groups) * ((d + 127) / 128) * ((d_out + BN - 1) / BN);
+    const int64_t each = (rows + n_groups - 1) / n_groups;
+    const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0,
+                   tiles_per_unit(most, static_cast<int>((each + mma::BK - 1) / mma::BK)), d,
+                   aligned16(dw) && d % 8 == 0};
     return launch<T, mma::MATRICES, BN>(dw, a, b, b, offsets, sh, most, s);
 }
 

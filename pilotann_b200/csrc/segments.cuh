@@ -106,16 +106,26 @@ __device__ __forceinline__ void ring_init(TileRing &r, int readers) {
     tc05::mbar_init(tc05::smem_u32(&r.answered), 1);
 }
 
+// Tiles that a CTA takes at a time: enough for 16 slices (an answer takes as long as a few), as
+// long as every SM asks eight times.
+inline int tiles_per_unit(int64_t tiles, int slices) {
+    int unit = 1;
+    while (unit < 8 && unit * slices < 16 && tiles / (2 * unit) >= 8 * 148) unit *= 2;
+    return unit;
+}
+
 // One thread hands out tiles: make(index) is the tile, or has g == kNoTile for an index that the
 // offsets do not reach.
 template <typename Make>
-__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, Make make) {
+__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
+                                           Make make) {
     const uint32_t answer = tc05::smem_u32(&r.answer), bar = tc05::smem_u32(&r.answered);
     int index = blockIdx.x;
     uint32_t n = 0;
     for (uint32_t asked = 0;; ++asked) {
-        const Tile tile = make(index);
-        if (tile.g != kNoTile) {
+        for (int u = 0; u < unit && !abort_s; ++u) {
+            const Tile tile = make(index * unit + u);
+            if (tile.g == kNoTile) break;
             r.a[n & 3] = make_int4(tile.g, tile.m0, tile.c0, tile.c_end);
             r.b[n & 3] = make_int2(tile.t0, tile.t_end);
             tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));

@@ -124,15 +124,6 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t c
     d |= static_cast<uint64_t>(2) << 61;
     return d;
 }
-// 32 rows of 16 bytes, no swizzle: 8-row groups 128 bytes apart (for tcgen05.cp of block scales)
-__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>(1) << 16;
-    d |= static_cast<uint64_t>(128 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    return d;
-}
 // kind::mxf4 and kind::mxf4nvf4, both operands E2M1 and K-major, tile 128 x N, K = 64
 __host__ __device__ constexpr uint32_t idesc_mxf4(bool e8m0, int N) {
     return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
@@ -202,11 +193,6 @@ __device__ __forceinline__ void mma_fp4(uint32_t tmem_d, uint64_t desc_a, uint64
             "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
             : "memory");
 }
-// 32 rows x 16 bytes of shared memory to four TMEM columns, the same for each warp's 32 lanes
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-                 : "memory");
-}
 // The mbarrier gets one arrival when all MMAs issued so far by this thread finish.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -262,6 +248,19 @@ __device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t (&r)[
 }
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// 32 lanes x 16 columns from registers
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 }  // namespace tc05
