@@ -216,47 +216,42 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             }
         }
     } else if (warp == 1) {
-        // ---- products ----
-        if (lane == 0) {
-            uint32_t it = 0, sg = 0, acc_it = 0;
-            // of the first stage; a descriptor counts 16 bytes, so others are sums
-            const uint64_t desc_a = tc05::smem_desc_sw128(ring);
-            Tile tile;
-            for (uint32_t n = 0; grouped::ring_take<false>(tiles, abort_s, n, tile); ++n) {
-                if (tile.g < 0) continue;
-                const int acc = acc_it & 1;
-                if (acc_it >= 2 && !tc05::mbar_wait_bounded(tc05::smem_u32(&acc_empty[acc]),
-                                                            (acc_it / 2 - 1) & 1, WAIT_LIMIT)) {
-                    abort_s = 1;
-                    break;
+        // ---- products: the warp runs together, one lane issues ----
+        const bool leader = tc05::elect_one();
+        uint32_t it = 0, sg = 0, acc_it = 0;
+        bool ok = true;
+        // of the first stage; a descriptor counts 16 bytes, so others are sums
+        const uint64_t desc_a = tc05::smem_desc_sw128(ring);
+        Tile tile;
+        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            if (tile.g < 0) continue;
+            const int acc = acc_it & 1;
+            if (acc_it >= 2)
+                ok = tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[acc]), (acc_it / 2 - 1) & 1,
+                                          WAIT_LIMIT);
+            const uint32_t d = tmem + acc * BN;
+            const int cols = min(BN, tile.c_end - tile.c0);
+            const uint32_t idesc0 = tc05::idesc_mxf4(METHOD == PA_MXFP4, (cols + 15) / 16 * 16);
+            uint32_t sa = 0, sb = 0;
+            for (int k = 0; ok && k < n_stages; ++k, ++it) {
+                const int s = it % STAGES, buf = sg % BUFS;
+                if (k % GROUP == 0) {
+                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&tm_full[buf]), (sg / BUFS) & 1,
+                                              WAIT_LIMIT);
+                    sa = tmem + ACC_COLS + buf * SCALE_COLS;
+                    sb = sa + 16;
                 }
+                ok = ok && tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
+                                                WAIT_LIMIT);
+                if (!ok) break;
                 tc05::fence_after_sync();
-                const uint32_t d = tmem + acc * BN;
-                const int cols = min(BN, tile.c_end - tile.c0);
-                const uint32_t idesc0 =
-                    tc05::idesc_mxf4(METHOD == PA_MXFP4, (cols + 15) / 16 * 16);
-                uint32_t sa = 0, sb = 0;
-                for (int k = 0; k < n_stages; ++k, ++it) {
-                    const int s = it % STAGES, buf = sg % BUFS;
-                    if (!tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
-                                                 WAIT_LIMIT)) {
-                        abort_s = 1;
-                        break;
-                    }
-                    if (k % GROUP == 0) {
-                        if (!tc05::mbar_wait_bounded(tc05::smem_u32(&tm_full[buf]), (sg / BUFS) & 1,
-                                                     WAIT_LIMIT)) {
-                            abort_s = 1;
-                            break;
-                        }
-                        sa = tmem + ACC_COLS + buf * SCALE_COLS;
-                        sb = sa + 16;
-                    }
-                    tc05::fence_after_sync();
-                    const uint64_t a = desc_a + s * (STAGE_BYTES / 16), b = a + A_BYTES / 16;
+                const uint64_t a = desc_a + s * (STAGE_BYTES / 16), b = a + A_BYTES / 16;
+                const int steps = min(4, (args.values - k * BK + 63) / 64);
+                const bool last = k + 1 == n_stages;
+                if (leader) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (k * BK + 64 * j < args.values) {
+                        if (j < steps) {
                             // 64 values: two bytes of a scale word (mxfp4) or all four (nvfp4)
                             const int word = METHOD == PA_MXFP4 ? 2 * (k % GROUP) + j / 2 : j;
                             const uint32_t idesc =
@@ -267,18 +262,19 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                         }
                     }
                     tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
-                    if (k % GROUP == GROUP - 1 || k + 1 == n_stages) {
+                    if (k % GROUP == GROUP - 1 || last)
                         tc05::mma_commit(tc05::smem_u32(&tm_empty[buf]));
-                        ++sg;
-                    }
+                    if (last) tc05::mma_commit(tc05::smem_u32(&acc_full[acc]));
                 }
-                if (!abort_s) tc05::mma_commit(tc05::smem_u32(&acc_full[acc]));
-                ++acc_it;
+                __syncwarp();
+                if (k % GROUP == GROUP - 1 || last) ++sg;
             }
-            if (abort_s) {  // nor does a product read on
-                tc05::mma_commit(tc05::smem_u32(&quit_bar));
-                tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
-            }
+            ++acc_it;
+        }
+        if (!ok) abort_s = 1;
+        if (abort_s && leader) {  // nor does a product read on
+            tc05::mma_commit(tc05::smem_u32(&quit_bar));
+            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
         }
     } else if (warp == 2) {
         if (lane == 0)

@@ -50,12 +50,6 @@ struct Shape {
     bool vec;         // result rows start on 16 bytes and are whole pieces of 16
 };
 
-// all lanes of the warp: the same answer for each of them
-__device__ __forceinline__ bool warp_wait(const uint64_t *bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, tc05::mbar_wait_bounded(tc05::smem_u32(bar), parity,
-                                                           mma::WAIT_LIMIT));
-}
-
 template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(mma::THREADS, 1)
 mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
@@ -169,6 +163,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
     } else if (warp == 1) {
+        const bool leader = tc05::elect_one();
         uint32_t it = 0, acc_it = 0;
         // of the first stage; a descriptor counts 16 bytes, so others are sums
         const uint64_t desc_a = A_MN ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
@@ -179,7 +174,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         for (uint32_t n = 0; ring_take<true>(tiles, abort_s, n, tile); ++n) {
             if (tile.t0 >= tile.t_end) continue;
             const int slot = acc_it & 1;
-            if (acc_it >= 2 && !warp_wait(&acc_empty[slot], (acc_it / 2 - 1) & 1)) {
+            if (acc_it >= 2 && !tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[slot]), (acc_it / 2 - 1) & 1,
+                                                     WAIT_LIMIT)) {
                 abort_s = 1;
                 break;
             }
@@ -190,7 +186,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, (cols + 15) / 16 * 16);
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
-                if (!warp_wait(&full_bar[s], (it / STAGES) & 1)) {
+                if (!tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1, WAIT_LIMIT)) {
                     abort_s = 1;
                     break;
                 }
@@ -210,7 +206,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 }
                 __syncwarp();
                 tc05::fence_after_sync();
-                if (lane == 0) {
+                if (leader) {
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k) {
                         if (16 * k < live) {
@@ -227,7 +223,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             ++acc_it;
         }
         __syncwarp();
-        if (abort_s && lane == 0) {  // nor does a product read on
+        if (abort_s && leader) {  // nor does a product read on
             tc05::mma_commit(tc05::smem_u32(&quit_bar));
             tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
         }

@@ -185,7 +185,15 @@ __device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, ui
     if (WARP) __syncwarp();
     if (!WARP || (threadIdx.x & 31) == 0) tc05::mbar_arrive(tc05::smem_u32(&r.empty[slot]));
     tile = Tile{a.x, a.y, a.z, a.w, b.x, b.y};
-    return a.x != kNoTile;
+    if (WARP) {  // one value for the warp
+        tile.g = __shfl_sync(0xffffffffu, tile.g, 0);
+        tile.m0 = __shfl_sync(0xffffffffu, tile.m0, 0);
+        tile.c0 = __shfl_sync(0xffffffffu, tile.c0, 0);
+        tile.c_end = __shfl_sync(0xffffffffu, tile.c_end, 0);
+        tile.t0 = __shfl_sync(0xffffffffu, tile.t0, 0);
+        tile.t_end = __shfl_sync(0xffffffffu, tile.t_end, 0);
+    }
+    return tile.g != kNoTile;
 }
 
 // the segment that has row tile `tile`
