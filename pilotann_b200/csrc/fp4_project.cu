@@ -182,22 +182,22 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
 
     if (warp == 0) {
         // ---- codes ----
-        if (lane == 0) {
-            uint32_t it = 0;
-            Tile tile;
-            for (uint32_t n = 0; grouped::ring_take<false>(tiles, abort_s, n, tile); ++n) {
-                if (tile.g < 0) continue;
-                const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
-                for (int k = 0; k < n_stages; ++k, ++it) {
-                    const int s = it % STAGES;
-                    if (it >= STAGES &&
-                        !tc05::mbar_wait_bounded(tc05::smem_u32(&empty_bar[s]),
-                                                 (it / STAGES - 1) & 1, WAIT_LIMIT)) {
-                        abort_s = 1;
-                        break;
-                    }
-                    const uint32_t a = ring + s * STAGE_BYTES;
-                    const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+        const bool leader = tc05::elect_one();
+        uint32_t it = 0;
+        bool ok = true;
+        Tile tile;
+        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            if (tile.g < 0) continue;
+            const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
+            for (int k = 0; k < n_stages; ++k, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES)
+                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
+                                              WAIT_LIMIT);
+                if (!ok) break;
+                const uint32_t a = ring + s * STAGE_BYTES;
+                const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+                if (leader) {
                     tc05::mbar_expect_tx(bar, A_BYTES + boxes * BOX_BYTES);
                     tc05::tma_load_3d(a, &map_t, k * (BK / 2), tile.m0, tile.g, bar);
                     if (boxes * BOX == BN) {
@@ -208,12 +208,14 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                                               tile.c0 + BOX * j, bar);
                     }
                 }
+                __syncwarp();
             }
-            if (abort_s) {  // no copy is left in flight behind the CTA
-                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                    tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]),
-                                            (i / STAGES) & 1, WAIT_LIMIT);
-            }
+        }
+        if (!ok) abort_s = 1;
+        if (abort_s) {  // no copy is left in flight behind the CTA
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
+                                        WAIT_LIMIT);
         }
     } else if (warp == 1) {
         // ---- products: the warp runs together, one lane issues ----

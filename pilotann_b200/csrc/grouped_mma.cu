@@ -121,21 +121,21 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     };
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            Tile tile;
-            for (uint32_t n = 0; ring_take<false>(tiles, abort_s, n, tile); ++n) {
-                const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
-                for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
-                    const int s = it % STAGES;
-                    if (it >= STAGES &&
-                        !tc05::mbar_wait_bounded(tc05::smem_u32(&empty_bar[s]),
-                                                 (it / STAGES - 1) & 1, WAIT_LIMIT)) {
-                        abort_s = 1;
-                        break;
-                    }
-                    const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
-                    const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+        const bool leader = tc05::elect_one();
+        uint32_t it = 0;
+        bool ok = true;
+        Tile tile;
+        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
+            for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES)
+                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
+                                              WAIT_LIMIT);
+                if (!ok) break;
+                const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+                if (leader) {
                     tc05::mbar_expect_tx(bar, A_BYTES + boxes * BOX_BYTES);
                     if (MODE == FORWARD) {
                         tc05::tma_load_3d(a, &map_a, t0, tile.m0, tile.g, bar);
@@ -155,12 +155,14 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                                               MODE == MATRICES ? t0 : tile.c0 + BOX * j, bar);
                     }
                 }
+                __syncwarp();
             }
-            if (abort_s) {  // no copy is left in flight behind the CTA
-                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                    tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]),
-                                            (i / STAGES) & 1, WAIT_LIMIT);
-            }
+        }
+        if (!ok) abort_s = 1;
+        if (abort_s) {  // no copy is left in flight behind the CTA
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
+                                        WAIT_LIMIT);
         }
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
