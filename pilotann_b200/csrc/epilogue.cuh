@@ -45,13 +45,16 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return r;
 }
 
-// One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (nullptr-like: `some` false = zeros), the
+// One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (`some` false: zeros instead), the
 // first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).  `m_left`: lanes that exist.
-// scale(lane of the tile, column of the chunk) multiplies before rounding.  All 128 threads.
-template <typename T, int COLS, typename Scale>
+// If SCALED, element (m, c) is multiplied by m_scale[i] c_scale[j] before it is rounded: i counts
+// the four lanes 32 w + 8 i + lane / 4 of this thread, j its columns 8 (j / 2) + 2 (lane % 4) + j % 2.
+// All 128 threads.
+template <typename T, int COLS, bool SCALED>
 __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, bool some, int live,
                                             int m_left, bool vec, uint32_t buf, int w, int lane,
-                                            Scale scale) {
+                                            const float (&m_scale)[4],
+                                            const float (&c_scale)[COLS / 4]) {
     uint32_t p[2][COLS / 8][2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -69,9 +72,12 @@ __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, b
         for (int i = 0; i < COLS / 8; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int m = 32 * w + 16 * half + 8 * h + lane / 4, c = 8 * i + 2 * (lane % 4);
-                p[half][i][h] = pack2<T>(scale(__uint_as_float(r[4 * i + 2 * h]), m, c),
-                                         scale(__uint_as_float(r[4 * i + 2 * h + 1]), m, c + 1));
+                float lo = __uint_as_float(r[4 * i + 2 * h]), hi = __uint_as_float(r[4 * i + 2 * h + 1]);
+                if (SCALED) {
+                    lo *= m_scale[2 * half + h] * c_scale[2 * i];
+                    hi *= m_scale[2 * half + h] * c_scale[2 * i + 1];
+                }
+                p[half][i][h] = pack2<T>(lo, hi);
             }
     }
     // lane l names row l % 8 of matrix l / 8: column block l / 16, rows 8 (l / 8 % 2) on

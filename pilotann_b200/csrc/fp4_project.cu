@@ -448,9 +448,6 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             const int m_left = static_cast<int>(min(args.d_out - tile.m0, static_cast<int64_t>(BM)));
             const int64_t first = tile.c0 * args.d_out + tile.m0;
             const uint32_t from = tmem + acc * BN;
-            auto scale = [&](float v, int m, int c) {
-                return METHOD == PA_NVFP4 && some ? v * (ts[m] * qs[c]) : v;
-            };
             if (args.out_dtype == PA_F32) {
                 // 32 lanes store 128 bytes of a row as they are
                 float *dst = static_cast<float *>(args.out) + first + own;
@@ -485,14 +482,24 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     }
                 }
             } else {
+                constexpr bool SCALED = METHOD == PA_NVFP4;  // zeros by zeros where there is no group
+                float m_scale[4] = {}, c_scale[CHUNK / 4] = {};
+                if (SCALED && some)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m_scale[i] = ts[32 * w + 8 * i + lane / 4];
                 auto store = [&](auto *out) {
                     using O = typename std::remove_pointer<decltype(out)>::type;
 #pragma unroll 1
-                    for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
-                        epilogue::store_chunk<O, CHUNK>(
+                    for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk) {
+                        if (SCALED && some)
+#pragma unroll
+                            for (int j = 0; j < CHUNK / 4; ++j)
+                                c_scale[j] = qs[c0 + 8 * (j / 2) + 2 * (lane % 4) + j % 2];
+                        epilogue::store_chunk<O, CHUNK, SCALED>(
                             out + first + c0 * args.d_out, args.d_out, from + c0, some, live - c0,
                             m_left, args.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
-                            [&](float v, int m, int c) { return scale(v, m, c0 + c); });
+                            m_scale, c_scale);
+                    }
                 };
                 if (args.out_dtype == PA_BF16) store(static_cast<__nv_bfloat16 *>(args.out));
                 else store(static_cast<__half *>(args.out));

@@ -6,10 +6,10 @@
 // consecutive rows and a counter per group in shared memory, so that the place of a row is
 // (rows of earlier groups) + (earlier blocks) + (earlier warps) + (earlier rows of the warp):
 // no counter is ever shared between rows whose order matters, and the result does not depend
-// on timing.  One block: one launch.  More: a histogram per block, one CTA that turns the
-// histograms into places, and the pass that writes.  Bound by launch latency up to some ten
-// thousand rows; above that by the three passes over the ids (8 bytes a row each, from L2
-// after the first).
+// on timing.  Up to kSingleRows rows: one launch of one CTA, bound by its latency (1024 ids, 64
+// groups: 4 us on the GPU, less than the call).  More: a histogram per block; the places of the
+// blocks within each group, 32 groups a CTA; the pass that writes, which also sums up the groups.
+// The passes read 8 bytes a row twice, the second time from L2, and write 8.
 #include "pa_common.cuh"
 
 namespace pa {
@@ -17,8 +17,9 @@ namespace pa {
 namespace group {
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kBlockRows = 8192;
-constexpr int kScanThreads = 1024;
+constexpr int kSingleRows = 8192;
+constexpr int kBlockRows = 4096;
+constexpr int kScanBlocks = 256;  // blocks of rows per step of the scan: 32 warps, 8 blocks each
 }  // namespace group
 
 __device__ __forceinline__ int group_of(int64_t id, int n_groups) {
@@ -63,49 +64,59 @@ __device__ __forceinline__ int64_t cta_exclusive(int64_t v, int64_t *warp_sum_s,
     return before + x - v;
 }
 
-// histograms of the blocks -> places of the blocks within their group; offsets
-__global__ void __launch_bounds__(group::kScanThreads)
-group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ block_counts, int n_blocks,
+// Histograms of the blocks -> places of the blocks within their group; sums of the groups.  A lane
+// has a group, a warp eight consecutive blocks, so that loads and stores are whole lines.
+__global__ void __launch_bounds__(1024)
+group_scan_kernel(int32_t *__restrict__ totals, int32_t *__restrict__ block_counts, int n_blocks,
                   int n_groups) {
-    __shared__ int64_t warp_sum_s[32];
-    const int bins = n_groups + 1;
-    int64_t base = 0;
-    for (int g0 = 0; g0 < bins; g0 += group::kScanThreads) {
-        const int g = g0 + threadIdx.x;
+    __shared__ int32_t part_s[32][33];
+    const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int g = blockIdx.x * 32 + lane;
+    int32_t carry = 0;
+    for (int b0 = 0; b0 < n_blocks; b0 += group::kScanBlocks) {
+        int32_t *p = block_counts + static_cast<int64_t>(b0 + 8 * w) * bins + g;
+        int32_t c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            c[j] = g < bins && b0 + 8 * w + j < n_blocks ? p[static_cast<int64_t>(j) * bins] : 0;
         int32_t sum = 0;
-        if (g < bins) {
-            int32_t *p = block_counts + g;
-            for (int b = 0; b < n_blocks; b += 8) {  // eight loads in flight
-                int32_t c[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    c[j] = b + j < n_blocks ? p[static_cast<int64_t>(b + j) * bins] : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (b + j < n_blocks) p[static_cast<int64_t>(b + j) * bins] = sum;
-                    sum += c[j];
-                }
-            }
+        for (int j = 0; j < 8; ++j) {
+            const int32_t v = c[j];
+            c[j] = sum;
+            sum += v;
         }
-        int64_t total;
-        const int64_t place = cta_exclusive(sum, warp_sum_s, &total) + base;
-        if (g < bins) offsets[g] = place;  // offsets[n_groups]: where the ungrouped rows start
-        base += total;
+        part_s[w][lane] = sum;
+        __syncthreads();
+        int32_t before = carry, all = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int32_t v = part_s[i][lane];
+            if (i < w) before += v;
+            all += v;
+        }
+        carry += all;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (g < bins && b0 + 8 * w + j < n_blocks)
+                p[static_cast<int64_t>(j) * bins] = before + c[j];
+        __syncthreads();
     }
+    if (w == 0 && g < bins) totals[g] = carry;
 }
 
 // block_counts == nullptr: this CTA has all rows and makes the offsets itself
 __global__ void __launch_bounds__(group::kThreads)
 group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
-                     const int32_t *__restrict__ block_counts, const int64_t *__restrict__ ids,
-                     int64_t rows, int n_groups) {
+                     const int32_t *__restrict__ block_counts, const int32_t *__restrict__ totals,
+                     const int64_t *__restrict__ ids, int64_t rows, int n_groups, int block_rows) {
     extern __shared__ int32_t count_s[];  // [kWarps][n_groups + 1]
     __shared__ int64_t warp_sum_s[32];
     const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (int i = threadIdx.x; i < group::kWarps * bins; i += group::kThreads) count_s[i] = 0;
     __syncthreads();
-    const int64_t r0 = blockIdx.x * static_cast<int64_t>(group::kBlockRows);
-    const int n = static_cast<int>(min(static_cast<int64_t>(group::kBlockRows), rows - r0));
+    const int64_t r0 = blockIdx.x * static_cast<int64_t>(block_rows);
+    const int n = static_cast<int>(min(static_cast<int64_t>(block_rows), rows - r0));
     // each warp a run of whole groups of 32 rows
     const int run = 32 * ((n + 32 * group::kWarps - 1) / (32 * group::kWarps));
     const int lo = min(n, w * run), hi = min(n, lo + run);
@@ -120,16 +131,13 @@ group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
         int32_t sum = 0;
         if (g < bins)
             for (int i = 0; i < group::kWarps; ++i) sum += count_s[i * bins + g];
-        int64_t place;
-        if (block_counts == nullptr) {
-            int64_t total;
-            place = cta_exclusive(sum, warp_sum_s, &total) + base;
-            base += total;
-            if (g < bins) offsets[g] = place;
-        } else {
-            place = g < bins ? offsets[g] + block_counts[blockIdx.x * static_cast<int64_t>(bins) + g]
-                             : 0;
-        }
+        if (block_counts != nullptr) sum = g < bins ? totals[g] : 0;
+        int64_t total;
+        int64_t place = cta_exclusive(sum, warp_sum_s, &total) + base;
+        base += total;
+        if (blockIdx.x == 0 && g < bins) offsets[g] = place;  // [n_groups]: the ungrouped rows
+        if (block_counts != nullptr && g < bins)
+            place += block_counts[blockIdx.x * static_cast<int64_t>(bins) + g];
         if (g < bins) {
             int32_t at = static_cast<int32_t>(place);
             for (int i = 0; i < group::kWarps; ++i) {
@@ -159,9 +167,9 @@ group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
 }  // namespace pa
 
 extern "C" int64_t pa_group_rows_workspace_bytes(int64_t rows, int n_groups) {
-    if (rows <= pa::group::kBlockRows || n_groups < 1) return 0;
+    if (rows <= pa::group::kSingleRows || n_groups < 1) return 0;
     const int64_t blocks = (rows + pa::group::kBlockRows - 1) / pa::group::kBlockRows;
-    return blocks * (n_groups + 1) * static_cast<int64_t>(sizeof(int32_t));
+    return (blocks + 1) * (n_groups + 1) * static_cast<int64_t>(sizeof(int32_t));
 }
 
 extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *router, int64_t rows,
@@ -171,24 +179,28 @@ extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *ro
     PA_REQUIRE(n_groups >= 1 && n_groups <= PA_MAX_GROUPS, "n_groups must be in [1, %d]",
                PA_MAX_GROUPS);
     PA_REQUIRE(offsets && (rows == 0 || (order && router)), "null pointer");
+    const bool single = rows <= group::kSingleRows;
+    PA_REQUIRE(single || workspace, "workspace missing (pa_group_rows_workspace_bytes)");
     const int bins = n_groups + 1;
-    const int blocks = static_cast<int>((rows + group::kBlockRows - 1) / group::kBlockRows);
-    PA_REQUIRE(blocks <= 1 || workspace, "workspace missing (pa_group_rows_workspace_bytes)");
+    const int blocks =
+        single ? 1 : static_cast<int>((rows + group::kBlockRows - 1) / group::kBlockRows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const size_t scatter_smem = static_cast<size_t>(group::kWarps) * bins * sizeof(int32_t);
     if (scatter_smem > 48 * 1024)
         PA_CUDA_TRY(cudaFuncSetAttribute(group_scatter_kernel,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(scatter_smem)));
-    int32_t *counts = blocks > 1 ? static_cast<int32_t *>(workspace) : nullptr;
-    if (blocks > 1) {
+    int32_t *counts = single ? nullptr : static_cast<int32_t *>(workspace);
+    int32_t *totals = single ? nullptr : counts + static_cast<int64_t>(blocks) * bins;
+    if (!single) {
         group_count_kernel<<<blocks, group::kThreads, bins * sizeof(int32_t), s>>>(counts, router,
                                                                                    rows, n_groups);
-        group_scan_kernel<<<1, group::kScanThreads, 0, s>>>(offsets, counts, blocks, n_groups);
+        group_scan_kernel<<<(bins + 31) / 32, 1024, 0, s>>>(totals, counts, blocks, n_groups);
         count_launch(2);
     }
-    group_scatter_kernel<<<blocks > 1 ? blocks : 1, group::kThreads, scatter_smem, s>>>(
-        order, offsets, counts, router, rows, n_groups);
+    group_scatter_kernel<<<blocks, group::kThreads, scatter_smem, s>>>(
+        order, offsets, counts, totals, router, rows, n_groups,
+        single ? group::kSingleRows : group::kBlockRows);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;

@@ -12,111 +12,298 @@ namespace pa {
 
 namespace grouped {
 
-constexpr int kT = 64;   // output tile, both ways
-constexpr int kK = 16;   // slice of the summed axis
+// ---- fp32 values: fma on the CUDA cores ---------------------------------------------
+// Tiles of TR rows x TC columns by 256 threads, each TR / 16 x TC / 16 outputs:
+//   C[r, c] = sum_t P(r, t) Q(c, t), P(r, t) = p[r * pr + t * pt], Q likewise,
+// where the axis that is contiguous in memory is t (T_FAST) or r, c.  Slices of 16 t go through
+// registers into two buffers in shared memory, the next one on its way while one is multiplied.
+// A sum is kept in two levels, 256 terms at a time, so that its error grows with the square root of
+// 256 terms rather than of all (65536 rows in one sum: 5e-6 of the result in one level, below 1e-6 in
+// two).  128 x 128 tiles are bound by the fma units, smaller ones by latency and by the loads
+// from shared memory.
+constexpr int kK = 16;
+constexpr int kTerms = 256;
 
-// 64 x 64 outputs, 256 threads with 4 x 4 each, fp32 fma along the summed axis.
-//   C[r, c] = sum_t P(r, t) Q(c, t), P(r, t) = p[r * pr + t * pt], Q likewise
-template <typename T, bool P_T_FAST, bool Q_T_FAST>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], const T *p, int64_t pr, int64_t pt,
-                                             int n_r, const T *q, int64_t qc, int64_t qt, int n_c,
-                                             int64_t n_t, float (*p_s)[kT + 4],
-                                             float (*q_s)[kT + 4]) {
+template <int T, bool T_FAST> struct Slice {
+    static constexpr int kEach = T * kK / 256;  // values a thread loads
+    float v[kEach];
+
+    // 16-byte loads where there are four values a thread and rows start on 16 bytes (`vec`)
+    __device__ __forceinline__ void load(const float *p, int64_t pr, int64_t pt, int n_r, int64_t t0,
+                                         int64_t n_t, bool vec) {
+        const int tid = threadIdx.x;
+        if (kEach >= 4 && vec) {
+#pragma unroll
+            for (int i = 0; i < kEach / 4; ++i) {
+                const int j = tid + 256 * i;
+                const int r = T_FAST ? j / 4 : 4 * (j % (T / 4)), t = T_FAST ? 4 * (j % 4) : j / (T / 4);
+                float4 x = make_float4(0, 0, 0, 0);
+                const float *q = p + (T_FAST ? r * pr + t0 + t : r + (t0 + t) * pt);
+                const int64_t left = T_FAST ? (r < n_r ? n_t - t0 - t : 0) : (t0 + t < n_t ? n_r - r : 0);
+                if (left >= 4) {
+                    x = __ldg(reinterpret_cast<const float4 *>(q));
+                } else {
+                    if (left > 0) x.x = __ldg(q);
+                    if (left > 1) x.y = __ldg(q + 1);
+                    if (left > 2) x.z = __ldg(q + 2);
+                }
+                v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int j = tid + 256 * i;
+                const int r = T_FAST ? j / kK : j % T, t = T_FAST ? j % kK : j / T;
+                v[i] = r < n_r && t0 + t < n_t ? __ldg(p + r * pr + (t0 + t) * pt) : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float (*to)[T + 4], bool vec) const {
+        const int tid = threadIdx.x;
+        if (kEach >= 4 && vec) {
+#pragma unroll
+            for (int i = 0; i < kEach / 4; ++i) {
+                const int j = tid + 256 * i;
+                if (T_FAST) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) to[4 * (j % 4) + k][j / 4] = v[4 * i + k];
+                } else {
+                    *reinterpret_cast<float4 *>(&to[j / (T / 4)][4 * (j % (T / 4))]) =
+                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int j = tid + 256 * i;
+                to[T_FAST ? j % kK : j / T][T_FAST ? j / kK : j % T] = v[i];
+            }
+        }
+    }
+};
+
+// outputs of a thread along an axis of T: four neighbours per 64, or T / 16 neighbours
+template <int T> __device__ __forceinline__ int place(int thread, int i) {
+    return T >= 64 ? 64 * (i / 4) + 4 * thread + i % 4 : (T / 16) * thread + i;
+}
+template <int T>
+__device__ __forceinline__ void fetch(float (&v)[T / 16], const float *row, int thread) {
+    if (T >= 64) {
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(row + 64 * i + 4 * thread);
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < T / 16; ++i) v[i] = row[place<T>(thread, i)];
+    }
+}
+
+template <int TR, int TC> struct Buffers {
+    __align__(16) float p[2][kK][TR + 4];
+    __align__(16) float q[2][kK][TC + 4];
+};
+
+template <int TR, int TC, bool P_T_FAST, bool Q_T_FAST>
+__device__ __forceinline__ void tile_product(float (&acc)[TR / 16][TC / 16], Buffers<TR, TC> &s,
+                                             const float *p, int64_t pr, int64_t pt, int n_r,
+                                             bool p_vec, const float *q, int64_t qc, int64_t qt,
+                                             int n_c, bool q_vec, int64_t n_t) {
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int64_t t0 = 0; t0 < n_t; t0 += kK) {
-#pragma unroll
-        for (int i = threadIdx.x; i < kT * kK; i += 256) {
-            const int r = P_T_FAST ? i / kK : i % kT, t = P_T_FAST ? i % kK : i / kT;
-            p_s[t][r] = r < n_r && t0 + t < n_t ? to_f32(p[r * pr + (t0 + t) * pt]) : 0.0f;
+    Slice<TR, P_T_FAST> ps;
+    Slice<TC, Q_T_FAST> qs;
+    float part[TR / 16][TC / 16] = {};
+    ps.load(p, pr, pt, n_r, 0, n_t, p_vec);
+    qs.load(q, qc, qt, n_c, 0, n_t, q_vec);
+    int b = 0;
+    for (int64_t t0 = 0; t0 < n_t; t0 += kK, b ^= 1) {
+        ps.store(s.p[b], p_vec);
+        qs.store(s.q[b], q_vec);
+        __syncthreads();  // (the other buffer was read before the barrier of the slice before)
+        if (t0 + kK < n_t) {
+            ps.load(p, pr, pt, n_r, t0 + kK, n_t, p_vec);
+            qs.load(q, qc, qt, n_c, t0 + kK, n_t, q_vec);
         }
-#pragma unroll
-        for (int i = threadIdx.x; i < kT * kK; i += 256) {
-            const int c = Q_T_FAST ? i / kK : i % kT, t = Q_T_FAST ? i % kK : i / kT;
-            q_s[t][c] = c < n_c && t0 + t < n_t ? to_f32(q[c * qc + (t0 + t) * qt]) : 0.0f;
-        }
-        __syncthreads();
 #pragma unroll
         for (int t = 0; t < kK; ++t) {
-            const float4 a = *reinterpret_cast<const float4 *>(&p_s[t][4 * ty]);
-            const float4 b = *reinterpret_cast<const float4 *>(&q_s[t][4 * tx]);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+            float av[TR / 16], bv[TC / 16];
+            fetch<TR>(av, s.p[b][t], ty);
+            fetch<TC>(bv, s.q[b][t], tx);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < TR / 16; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(av[i], bv[j], acc[i][j]);
+                for (int j = 0; j < TC / 16; ++j) part[i][j] = __fmaf_rn(av[i], bv[j], part[i][j]);
         }
-        __syncthreads();
+        if ((t0 + kK) % kTerms == 0 || t0 + kK >= n_t) {
+#pragma unroll
+            for (int i = 0; i < TR / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < TC / 16; ++j) {
+                    acc[i][j] += part[i][j];
+                    part[i][j] = 0.0f;
+                }
+        }
     }
+}
+
+template <int TR, int TC>
+__device__ __forceinline__ void tile_store(const float (&acc)[TR / 16][TC / 16], float *out,
+                                           int64_t ldo, int n_r, int n_c, bool vec) {
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+    for (int i = 0; i < TR / 16; ++i) {
+        const int r = place<TR>(ty, i);
+        if (r >= n_r) continue;
+#pragma unroll
+        for (int j = 0; j < TC / 16; j += 4) {
+            const int c = place<TC>(tx, j);
+            float *to = out + r * ldo + c;
+            if (vec && c + 4 <= n_c) {
+                *reinterpret_cast<float4 *>(to) =
+                    make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c + k < n_c) to[k] = acc[i][j + k];
+            }
+        }
+    }
+}
+
+// The rows of slot `slot` of T rows: segment i owns the slots from floor(edge_i / T) + i on, which are
+// enough for its tiles wherever it starts.  False: a slot without rows.  All threads of the CTA.
+struct SlotRows { int seg; int64_t r0; int n_r; };
+__device__ __forceinline__ bool slot_rows(SlotRows &s, const int64_t *offsets, int64_t rows,
+                                          int n_groups, int64_t slot, int T) {
+    int below = 0;  // segments that start at or before this slot
+    for (int i0 = 0; i0 < n_groups + 2; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x;
+        below += __syncthreads_count(i < n_groups + 2 &&
+                                     edge(offsets, n_groups, rows, i) / T + i <= slot);
+    }
+    s.seg = below - 1;
+    const int64_t lo = edge(offsets, n_groups, rows, s.seg),
+                  hi = edge(offsets, n_groups, rows, s.seg + 1);
+    s.r0 = lo + (slot - (lo / T + s.seg)) * T;
+    s.n_r = static_cast<int>(min(static_cast<int64_t>(T), hi - s.r0));
+    return s.r0 >= lo && s.n_r > 0;
 }
 
 // Rows side: forward (W_T_FAST: w's last axis is summed) and the gradient of the rows.
-// blockIdx.x = a slot of 64 rows.  Segment i owns the slots from floor(edge_i / 64) + i on, which
-// are enough for its tiles of 64 rows wherever it starts; a slot without rows returns.
-template <typename T, bool W_T_FAST>
+template <int TR, int TC, bool W_T_FAST>
 __global__ void __launch_bounds__(256)
-rows_kernel(T *__restrict__ out, const T *__restrict__ x, const T *__restrict__ w,
+rows_kernel(float *__restrict__ out, const float *__restrict__ x, const float *__restrict__ w,
             const int64_t *__restrict__ offsets, int64_t rows, int n_groups, int d_sum, int d_out,
-            int64_t ldx, int64_t ldo) {
-    __shared__ __align__(16) float p_s[kK][kT + 4], q_s[kK][kT + 4];
-    const int64_t slot = blockIdx.x;
-    int below = 0;  // segments that start at or before this slot
-    for (int i0 = 0; i0 < n_groups + 2; i0 += 256) {
-        const int i = i0 + threadIdx.x;
-        below += __syncthreads_count(i < n_groups + 2 &&
-                                     edge(offsets, n_groups, rows, i) / kT + i <= slot);
-    }
-    const int seg = below - 1;
-    const int64_t lo = edge(offsets, n_groups, rows, seg),
-                  hi = edge(offsets, n_groups, rows, seg + 1);
-    const int64_t r0 = lo + (slot - (lo / kT + seg)) * kT;
-    if (r0 < lo || r0 >= hi) return;
-    const int n_r = static_cast<int>(min(static_cast<int64_t>(kT), hi - r0));
-    const int c0 = blockIdx.y * kT, n_c = min(kT, d_out - c0);
-    float acc[4][4] = {};
-    if (seg >= 1 && seg <= n_groups) {
-        const T *wg = w + static_cast<int64_t>(seg - 1) * d_sum * d_out;
+            int64_t ldx, int64_t ldo, bool x_vec, bool w_vec, bool out_vec) {
+    __shared__ Buffers<TR, TC> s;
+    SlotRows slot;
+    if (!slot_rows(slot, offsets, rows, n_groups, blockIdx.x, TR)) return;
+    const int c0 = blockIdx.y * TC, n_c = min(TC, d_out - c0);
+    float acc[TR / 16][TC / 16] = {};
+    if (slot.seg >= 1 && slot.seg <= n_groups) {
+        const float *wg = w + static_cast<int64_t>(slot.seg - 1) * d_sum * d_out;
+        const float *xr = x + slot.r0 * ldx;
         if (W_T_FAST)
-            tile_product<T, true, true>(acc, x + r0 * ldx, ldx, 1, n_r,
-                                        wg + static_cast<int64_t>(c0) * d_sum, d_sum, 1, n_c, d_sum,
-                                        p_s, q_s);
+            tile_product<TR, TC, true, true>(acc, s, xr, ldx, 1, slot.n_r, x_vec,
+                                             wg + static_cast<int64_t>(c0) * d_sum, d_sum, 1, n_c,
+                                             w_vec, d_sum);
         else
-            tile_product<T, true, false>(acc, x + r0 * ldx, ldx, 1, n_r, wg + c0, 1, d_out, n_c,
-                                         d_sum, p_s, q_s);
+            tile_product<TR, TC, true, false>(acc, s, xr, ldx, 1, slot.n_r, x_vec, wg + c0, 1, d_out,
+                                              n_c, w_vec, d_sum);
     }
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = 4 * ty + i, c = 4 * tx + j;
-            if (r < n_r && c < n_c) out[(r0 + r) * ldo + c0 + c] = from_f32<T>(acc[i][j]);
-        }
+    tile_store<TR, TC>(acc, out + slot.r0 * ldo + c0, ldo, slot.n_r, n_c, out_vec);
 }
 
-// Gradient of the matrices: one 64 x 64 tile of one group per CTA, summed over its rows.
-template <typename T>
+// Gradient of the matrices: one tile of one group per CTA, summed over its rows.
+template <int T>
 __global__ void __launch_bounds__(256)
-matrices_kernel(T *__restrict__ dw, const T *__restrict__ dy, const T *__restrict__ x,
+matrices_kernel(float *__restrict__ dw, const float *__restrict__ dy, const float *__restrict__ x,
                 const int64_t *__restrict__ offsets, int64_t rows, int n_groups, int d, int d_out,
-                int64_t ldy, int64_t ldx) {
-    __shared__ __align__(16) float p_s[kK][kT + 4], q_s[kK][kT + 4];
+                int64_t ldy, int64_t ldx, bool y_vec, bool x_vec, bool out_vec) {
+    __shared__ Buffers<T, T> s;
     const int g = blockIdx.z;
-    const int n0 = blockIdx.y * kT, k0 = blockIdx.x * kT;
-    const int n_n = min(kT, d_out - n0), n_k = min(kT, d - k0);
+    const int n0 = blockIdx.y * T, k0 = blockIdx.x * T;
+    const int n_n = min(T, d_out - n0), n_k = min(T, d - k0);
     const int64_t lo = edge(offsets, n_groups, rows, g + 1),
                   hi = edge(offsets, n_groups, rows, g + 2);
-    float acc[4][4] = {};
-    tile_product<T, false, false>(acc, dy + lo * ldy + n0, 1, ldy, n_n, x + lo * ldx + k0, 1, ldx,
-                                  n_k, hi - lo, p_s, q_s);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    float acc[T / 16][T / 16] = {};
+    if (hi > lo)
+        tile_product<T, T, false, false>(acc, s, dy + lo * ldy + n0, 1, ldy, n_n, y_vec,
+                                         x + lo * ldx + k0, 1, ldx, n_k, x_vec, hi - lo);
+    tile_store<T, T>(acc, dw + (static_cast<int64_t>(g) * d_out + n0) * d + k0, d, n_n, n_k, out_vec);
+}
+
+// Forward of groups of a few rows, which read their matrix and do little with it: a warp has two rows
+// of w, its lanes run along them, four values (or one) each, and multiply them with up to eight
+// rows of x from shared memory; butterfly over the lanes.  Reads w at the memory's rate up to about
+// eight rows a group.
+constexpr int kFewRows = 8;
+constexpr int kFewWarps = 8;
+constexpr int kFewSlice = 1024;  // values of a row of x in shared memory
+
+template <bool VEC>
+__global__ void __launch_bounds__(32 * kFewWarps)
+rows_few_kernel(float *__restrict__ out, const float *__restrict__ x, const float *__restrict__ w,
+                const int64_t *__restrict__ offsets, int64_t rows, int n_groups, int d_sum,
+                int d_out, int64_t ldx, int64_t ldo) {
+    __shared__ __align__(16) float x_s[kFewRows][kFewSlice];
+    const int lane = threadIdx.x & 31;
+    SlotRows slot;
+    if (!slot_rows(slot, offsets, rows, n_groups, blockIdx.x, kFewRows)) return;
+    const int c0 = 2 * (blockIdx.y * kFewWarps + (threadIdx.x >> 5));
+    const bool some = slot.seg >= 1 && slot.seg <= n_groups;
+    const float *w0 = w + (static_cast<int64_t>(slot.seg - 1) * d_out + c0) * d_sum, *w1 = w0 + d_sum;
+    float acc[kFewRows][2] = {};
+    for (int t0 = 0; some && t0 < d_sum; t0 += kFewSlice) {
+        const int len = min(kFewSlice, d_sum - t0);
+        __syncthreads();
+        for (int r = 0; r < slot.n_r; ++r)
+            for (int t = threadIdx.x; t < len; t += 32 * kFewWarps)
+                x_s[r][t] = __ldg(x + (slot.r0 + r) * ldx + t0 + t);
+        __syncthreads();
+        constexpr int N = VEC ? 4 : 1;
+#pragma unroll 4
+        for (int t = N * lane; t < len; t += 32 * N) {
+            float a[N], b[N];
+            if constexpr (VEC) {
+                const float4 z = make_float4(0, 0, 0, 0);
+                const float4 u = c0 < d_out ? __ldg(reinterpret_cast<const float4 *>(w0 + t0 + t)) : z;
+                const float4 v = c0 + 1 < d_out ? __ldg(reinterpret_cast<const float4 *>(w1 + t0 + t)) : z;
+                a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
+                b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+            } else {
+                a[0] = c0 < d_out ? __ldg(w0 + t0 + t) : 0.0f;
+                b[0] = c0 + 1 < d_out ? __ldg(w1 + t0 + t) : 0.0f;
+            }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+            for (int r = 0; r < kFewRows; ++r)
+                if (r < slot.n_r) {  // uniform
+                    float xv[N];
+                    if constexpr (VEC) {
+                        const float4 u = *reinterpret_cast<const float4 *>(&x_s[r][t]);
+                        xv[0] = u.x; xv[1] = u.y; xv[2] = u.z; xv[3] = u.w;
+                    } else {
+                        xv[0] = x_s[r][t];
+                    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = 4 * ty + i, k = 4 * tx + j;
-            if (n < n_n && k < n_k)
-                dw[(static_cast<int64_t>(g) * d_out + n0 + n) * d + k0 + k] =
-                    from_f32<T>(acc[i][j]);
+                    for (int i = 0; i < N; ++i) {
+                        acc[r][0] = __fmaf_rn(xv[i], a[i], acc[r][0]);
+                        acc[r][1] = __fmaf_rn(xv[i], b[i], acc[r][1]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kFewRows; ++r)
+        if (r < slot.n_r) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float v = acc[r][c];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == c && c0 + c < d_out) out[(slot.r0 + r) * ldo + c0 + c] = v;
+            }
         }
 }
 
@@ -198,28 +385,69 @@ int matrices_make_ok(const void **w, int64_t *ld, int n_groups, int d, int d_out
     return rc;
 }
 
+bool vec4(const void *p, int64_t ld) { return aligned16(p) && ld % 4 == 0; }
+
+template <int TR, int TC>
+void rows_tiles(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
+                int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
+                cudaStream_t s) {
+    dim3 grid(static_cast<unsigned>(rows / TR + n_groups + 2),
+              static_cast<unsigned>((d_out + TC - 1) / TC));
+    const bool x_vec = vec4(x, ldx), w_vec = vec4(w, transposed ? d_out : d_sum),
+               out_vec = vec4(out, ldo);
+    if (transposed)
+        rows_kernel<TR, TC, false><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
+                                                        d_out, ldx, ldo, x_vec, w_vec, out_vec);
+    else
+        rows_kernel<TR, TC, true><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
+                                                       d_out, ldx, ldo, x_vec, w_vec, out_vec);
+}
+
 int rows_f32(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
              int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
              cudaStream_t s) {
-    dim3 grid(static_cast<unsigned>(rows / kT + n_groups + 2),
-              static_cast<unsigned>((d_out + kT - 1) / kT));
-    if (transposed)
-        rows_kernel<float, false><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
-                                                       d_out, ldx, ldo);
-    else
-        rows_kernel<float, true><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
-                                                      d_out, ldx, ldo);
+    const int64_t each = (rows + n_groups - 1) / n_groups;  // on average
+    if (!transposed && each <= kFewRows) {
+        dim3 grid(static_cast<unsigned>(rows / kFewRows + n_groups + 2),
+                  static_cast<unsigned>((d_out + 2 * kFewWarps - 1) / (2 * kFewWarps)));
+        if (vec4(w, d_sum))
+            rows_few_kernel<true><<<grid, 32 * kFewWarps, 0, s>>>(out, x, w, offsets, rows, n_groups,
+                                                                  d_sum, d_out, ldx, ldo);
+        else
+            rows_few_kernel<false><<<grid, 32 * kFewWarps, 0, s>>>(out, x, w, offsets, rows, n_groups,
+                                                                   d_sum, d_out, ldx, ldo);
+    } else if (each <= 16) {
+        rows_tiles<16, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
+    } else if (each <= 32) {
+        rows_tiles<32, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
+    } else if (each <= 192 || d_out <= 64 || (rows / 128) * ((d_out + 127) / 128) < 148) {
+        // 128 x 128 needs a tile for every SM and groups that fill it
+        rows_tiles<64, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
+    } else {
+        rows_tiles<128, 128>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed,
+                             s);
+    }
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
 }
 
+template <int T>
+void matrices_tiles(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
+                    int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
+    dim3 grid(static_cast<unsigned>((d + T - 1) / T), static_cast<unsigned>((d_out + T - 1) / T),
+              static_cast<unsigned>(n_groups));
+    matrices_kernel<T><<<grid, 256, 0, s>>>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx,
+                                            vec4(dy, ldy), vec4(x, ldx), vec4(dw, d));
+}
+
 int matrices_f32(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
                  int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
-    dim3 grid(static_cast<unsigned>((d + kT - 1) / kT), static_cast<unsigned>((d_out + kT - 1) / kT),
-              static_cast<unsigned>(n_groups));
-    matrices_kernel<float><<<grid, 256, 0, s>>>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy,
-                                                ldx);
+    const int64_t large = static_cast<int64_t>((d + 127) / 128) * ((d_out + 127) / 128) * n_groups;
+    if (d > 64 && d_out > 64 && large >= 148)
+        matrices_tiles<128>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
+    else
+        matrices_tiles<64>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;

@@ -258,10 +258,10 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             T *dst = out + first * sh.ldo + tile.m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
-                epilogue::store_chunk<T, CHUNK>(
+                epilogue::store_chunk<T, CHUNK, false>(
                     dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
                     sh.m_size - tile.m0, sh.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
-                    lane, [](float v, int, int) { return v; });
+                    lane, {}, {});
             if (some) {
                 tc05::fence_before_sync();
                 __syncwarp();

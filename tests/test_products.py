@@ -65,7 +65,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.pa_project_grouped_workspace_bytes(18, 16, 4, 2, 8, 8, 8, 1) == 4 * 8 * 2
     assert L.pa_project_grouped_workspace_bytes(16, 16, 4, 2, 9, 8, 9, 1) == (4 + 2 * 8) * 16 * 2
     assert L.pa_group_rows_workspace_bytes(8192, 64) == 0
-    assert L.pa_group_rows_workspace_bytes(8193, 64) == 2 * 65 * 4
+    assert L.pa_group_rows_workspace_bytes(8193, 64) >= 3 * 65 * 4
 
 
 def test_cpu_tensors_are_refused():
