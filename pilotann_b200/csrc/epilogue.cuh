@@ -45,6 +45,41 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return r;
 }
 
+// Bytes that result rows of `width` 16-bit values can be stored in: all rows start on as many, and are
+// whole pieces.
+inline int piece_of(const void *out, int64_t ld, int64_t width) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(2 * ld) |
+                           static_cast<uintptr_t>(2 * width);
+    return bits & 2 ? 2 : bits & 4 ? 4 : bits & 8 ? 8 : 16;
+}
+
+// rows of 256 bytes from shared memory, V a thread
+template <typename V, typename T>
+__device__ __forceinline__ void store_rows(T *dst, int64_t ld, uint32_t buf, int rows, int m_left,
+                                           int tid) {
+    constexpr int kEach = sizeof(V) / 2, kThreadsPerRow = 128 / kEach;
+    const int m = kEach * (tid % kThreadsPerRow);
+    if (m >= m_left) return;
+    if constexpr (kThreadsPerRow <= kThreads) {
+#pragma unroll 4
+        for (int c = tid / kThreadsPerRow; c < rows; c += kThreads / kThreadsPerRow) {
+            V v;
+            const uint32_t from = buf + c * kPitch + 2 * m;
+            if constexpr (sizeof(V) == 16)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+            else if constexpr (sizeof(V) == 8)
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                             : "=r"(v.x), "=r"(v.y) : "r"(from) : "memory");
+            else if constexpr (sizeof(V) == 4)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+            else
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+            *reinterpret_cast<V *>(dst + c * ld + m) = v;
+        }
+    }
+}
+
 // One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (`some` false: zeros instead), the
 // first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).  `m_left`: lanes that exist.
 // If SCALED, element (m, c) is multiplied by m_scale[i] c_scale[j] before it is rounded: i counts
@@ -52,7 +87,7 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
 // All 128 threads.
 template <typename T, int COLS, bool SCALED>
 __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, bool some, int live,
-                                            int m_left, bool vec, uint32_t buf, int w, int lane,
+                                            int m_left, int piece, uint32_t buf, int w, int lane,
                                             const float (&m_scale)[4],
                                             const float (&c_scale)[COLS / 4]) {
     uint32_t p[2][COLS / 8][2];
@@ -93,29 +128,11 @@ __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, b
                 "r"(p[half][i + 1][1])
                 : "memory");
     sync();
-    const int tid = 32 * w + lane;
-    if (vec) {
-        const int m = 8 * (tid % 16);
-#pragma unroll
-        for (int c = tid / 16; c < COLS; c += 8) {
-            uint4 v;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(buf + c * kPitch + 2 * m)
-                         : "memory");
-            if (c < live && m < m_left) *reinterpret_cast<uint4 *>(dst + c * ld + m) = v;
-        }
-    } else {
-        const int rows = live < COLS ? live : COLS;
-        for (int c = w; c < rows; c += 4)
-#pragma unroll
-            for (int m = lane; m < 128; m += 32) {
-                uint16_t v;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + c * kPitch + 2 * m)
-                             : "memory");
-                if (m < m_left) *reinterpret_cast<uint16_t *>(dst + c * ld + m) = v;
-            }
-    }
+    const int rows = live < COLS ? live : COLS;
+    if (piece == 16) store_rows<uint4>(dst, ld, buf, rows, m_left, 32 * w + lane);
+    else if (piece == 8) store_rows<uint2>(dst, ld, buf, rows, m_left, 32 * w + lane);
+    else if (piece == 4) store_rows<uint32_t>(dst, ld, buf, rows, m_left, 32 * w + lane);
+    else store_rows<uint16_t>(dst, ld, buf, rows, m_left, 32 * w + lane);
 }
 
 }  // namespace epilogue

@@ -64,7 +64,7 @@ struct Args {
     int q_pitch, t_pitch;                // bytes of scales from row to row
     int unit;                            // tiles a CTA takes at a time
     int out_dtype;
-    bool vec;                            // 16-bit result rows are whole pieces of 16 bytes
+    int piece;                           // bytes that 16-bit result rows are stored in
     int *status;
 };
 
@@ -497,7 +497,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                                 c_scale[j] = qs[c0 + 8 * (j / 2) + 2 * (lane % 4) + j % 2];
                         epilogue::store_chunk<O, CHUNK, SCALED>(
                             out + first + c0 * args.d_out, args.d_out, from + c0, some, live - c0,
-                            m_left, args.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
+                            m_left, args.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
                             m_scale, c_scale);
                     }
                 };
@@ -601,7 +601,7 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     const int pitch = values / fp4::block_of(method);
     const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,
                          static_cast<int>(rows), n_groups, values, pitch, pitch, 1, out_dtype,
-                         aligned16(out) && d_out % 8 == 0, status};
+                         epilogue::piece_of(out, d_out, d_out), status};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return method == PA_MXFP4
                ? fp4::project_method<PA_MXFP4>(args, query_codes, codes, s)

@@ -47,7 +47,7 @@ struct Shape {
     int t_size;       // FORWARD, ROWS: summed axis
     int unit;         // tiles a CTA takes at a time
     int64_t ldo;
-    bool vec;         // result rows start on 16 bytes and are whole pieces of 16
+    int piece;        // bytes that result rows are stored in
 };
 
 template <typename T, int MODE, int BN>
@@ -260,7 +260,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
                 epilogue::store_chunk<T, CHUNK, false>(
                     dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
-                    sh.m_size - tile.m0, sh.vec, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
+                    sh.m_size - tile.m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
                     lane, {}, {});
             if (some) {
                 tc05::fence_before_sync();
@@ -340,7 +340,7 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
     const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum,
                    tiles_per_unit(most, (d_sum + mma::BK - 1) / mma::BK), ldo,
-                   aligned16(out) && ldo % 8 == 0 && d_out % 8 == 0};
+                   epilogue::piece_of(out, ldo, d_out)};
     return launch<T, MODE, BN>(out, a, b, tail, offsets, sh, most, s);
 }
 
@@ -388,7 +388,7 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     const int64_t each = (rows + n_groups - 1) / n_groups;
     const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0,
                    tiles_per_unit(most, static_cast<int>((each + mma::BK - 1) / mma::BK)), d,
-                   aligned16(dw) && d % 8 == 0};
+                   epilogue::piece_of(dw, d, d)};
     return launch<T, mma::MATRICES, BN>(dw, a, b, b, offsets, sh, most, s);
 }
 
