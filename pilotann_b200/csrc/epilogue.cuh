@@ -90,31 +90,35 @@ __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, b
                                             int m_left, int piece, uint32_t buf, int w, int lane,
                                             const float (&m_scale)[4],
                                             const float (&c_scale)[COLS / 4]) {
-    uint32_t p[2][COLS / 8][2];
+    uint32_t r[2][COLS / 2], p[2][COLS / 8][2];
+    if (some) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint32_t r[COLS / 2];
-        if (some) {
+        for (int half = 0; half < 2; ++half) {
             const uint32_t at = tmem + ((32u * w + 16u * half) << 16);
-            if constexpr (COLS == 32) tc05::tmem_ld_16x256_x4(at, r);
-            else tc05::tmem_ld_16x256_x2(at, r);
-            tc05::tmem_ld_wait();
-        } else {
-#pragma unroll
-            for (int j = 0; j < COLS / 2; ++j) r[j] = 0;
+            if constexpr (COLS == 32) tc05::tmem_ld_16x256_x4(at, r[half]);
+            else tc05::tmem_ld_16x256_x2(at, r[half]);
         }
+        tc05::tmem_ld_wait();
+    } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) r[half][j] = 0;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int i = 0; i < COLS / 8; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float lo = __uint_as_float(r[4 * i + 2 * h]), hi = __uint_as_float(r[4 * i + 2 * h + 1]);
+                float lo = __uint_as_float(r[half][4 * i + 2 * h]),
+                      hi = __uint_as_float(r[half][4 * i + 2 * h + 1]);
                 if (SCALED) {
                     lo *= m_scale[2 * half + h] * c_scale[2 * i];
                     hi *= m_scale[2 * half + h] * c_scale[2 * i + 1];
                 }
                 p[half][i][h] = pack2<T>(lo, hi);
             }
-    }
     // lane l names row l % 8 of matrix l / 8: column block l / 16, rows 8 (l / 8 % 2) on
     const uint32_t row = buf + (8 * (lane / 16) + lane % 8) * kPitch + (32 * w + 8 * (lane / 8 % 2)) * 2;
 #pragma unroll

@@ -46,7 +46,7 @@ __host__ __device__ constexpr int scale_buffers(int bn) { return bn > 128 ? 2 : 
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK / 2; }
 __host__ __device__ constexpr int scale_bytes(int bn) { return (1 + b_blocks(bn)) * 2048; }
 __host__ __device__ constexpr int stages(int bn) {
-    return bn >= 192 ? 4 : bn >= 128 ? 5 : bn >= 64 ? 7 : bn >= 32 ? 9 : 10;
+    return bn >= 192 ? 4 : bn >= 128 ? 5 : bn >= 64 ? 7 : bn >= 32 ? 8 : 10;
 }
 __host__ __device__ constexpr int smem_bytes(int bn) {
     return stages(bn) * stage_bytes(bn) + SCALE_SLOTS * scale_bytes(bn) +
@@ -127,7 +127,10 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     __shared__ volatile int abort_s;
     __shared__ Segments segs;
     __shared__ TileRing tiles;
-    __shared__ float t_scale_s[2][BM], q_scale_s[2][BN];  // nvfp4's row scales of two tiles
+    // nvfp4's row scales, of a tile each: the writers are at most five tiles ahead of the results
+    constexpr int ROW_BUFS = METHOD == PA_NVFP4 ? 8 : 1;
+    __shared__ float t_scale_s[ROW_BUFS][BM], q_scale_s[ROW_BUFS][BN];
+    __shared__ __align__(8) uint64_t row_full[ROW_BUFS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
     const uint32_t scale_ring = ring + STAGES * STAGE_BYTES;
@@ -141,6 +144,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             tc05::mbar_init(tc05::smem_u32(&sc_full[s]), 1 + NB);
             tc05::mbar_init(tc05::smem_u32(&sc_empty[s]), 4);
         }
+        for (int s = 0; s < ROW_BUFS; ++s) tc05::mbar_init(tc05::smem_u32(&row_full[s]), 4);
         for (int s = 0; s < BUFS; ++s) {
             tc05::mbar_init(tc05::smem_u32(&tm_full[s]), 4);
             tc05::mbar_init(tc05::smem_u32(&tm_empty[s]), 1);
@@ -286,11 +290,21 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // ---- scales to TMEM: lanes 32 (w % 4) on, for all the products of this CTA ----
         const uint32_t quarter = (32u * (warp & 3)) << 16;
         const int n_pieces = (n_stages + GROUP - 1) / GROUP;
+        const int own = 32 * (warp & 3) + lane;
         Tile tile;
-        uint32_t sg = 0;
+        uint32_t sg = 0, n_some = 0;
         bool ok = true;
         for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0) continue;
+            float t_row = 0.0f, q_row[NB] = {};
+            if (METHOD == PA_NVFP4) {  // on their way while the first scales are written
+                if (tile.m0 + own < args.d_out)
+                    t_row = __ldg(args.t_row_scale + tile.g * args.d_out + tile.m0 + own);
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    if (128 * j + own < BN && tile.c0 + 128 * j + own < tile.c_end)
+                        q_row[j] = __ldg(args.q_row_scale + tile.c0 + 128 * j + own);
+            }
             for (int piece = 0; piece < n_pieces; ++piece, ++sg) {
                 const int slot = sg % SCALE_SLOTS, buf = sg % BUFS;
                 ok = __all_sync(0xffffffffu,
@@ -337,7 +351,17 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     tc05::mbar_arrive(tc05::smem_u32(&sc_empty[slot]));
                     tc05::mbar_arrive(tc05::smem_u32(&tm_full[buf]));
                 }
+                if (METHOD == PA_NVFP4 && piece == 0) {
+                    const int at = n_some % ROW_BUFS;
+                    t_scale_s[at][own] = t_row;
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        if (128 * j + own < BN) q_scale_s[at][128 * j + own] = q_row[j];
+                    __syncwarp();
+                    if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&row_full[at]));
+                }
             }
+            ++n_some;
         }
         if (!ok) abort_s = 1;
     } else if (warp >= 12) {
@@ -431,15 +455,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             bool ok = grouped::ring_take<true>(tiles, abort_s, n_tile, tile);
             const bool some = ok && tile.g >= 0;
             const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
-            const float *ts = t_scale_s[n_tile & 1], *qs = q_scale_s[n_tile & 1];
-            if (METHOD == PA_NVFP4 && some) {
-                t_scale_s[n_tile & 1][own] =
-                    tile.m0 + own < args.d_out
-                        ? __ldg(args.t_row_scale + tile.g * args.d_out + tile.m0 + own) : 0.0f;
-                for (int c = own; c < BN; c += 128)
-                    q_scale_s[n_tile & 1][c] = c < live ? __ldg(args.q_row_scale + tile.c0 + c) : 0.0f;
-            }
-            if (some)
+            const float *ts = t_scale_s[acc_it % ROW_BUFS], *qs = q_scale_s[acc_it % ROW_BUFS];
+            if (METHOD == PA_NVFP4 && some)
+                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&row_full[acc_it % ROW_BUFS]),
+                                             (acc_it / ROW_BUFS) & 1, WAIT_LIMIT) || (abort_s = 1, false);
+            if (some && ok)
                 ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
                                              WAIT_LIMIT) || (abort_s = 1, false);
             __syncwarp();

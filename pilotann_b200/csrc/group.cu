@@ -8,7 +8,7 @@
 // no counter is ever shared between rows whose order matters, and the result does not depend
 // on timing.  Up to kSingleRows rows: one launch of one CTA, bound by its latency (1024 ids, 64
 // groups: 4 us on the GPU, less than the call).  More: a histogram per block; the places of the
-// blocks within each group, 32 groups a CTA; the pass that writes, which also sums up the groups.
+// blocks within each group, 32 groups a CTA, and the groups' sums; the pass that writes.
 // The passes read 8 bytes a row twice, the second time from L2, and write 8.
 #include "pa_common.cuh"
 
@@ -17,8 +17,8 @@ namespace pa {
 namespace group {
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kSingleRows = 8192;
-constexpr int kBlockRows = 4096;
+constexpr int kBlockRows = 256 * kWarps;
+constexpr int kSingleRows = 2 * kBlockRows;  // by a CTA of twice the warps
 constexpr int kScanBlocks = 256;  // blocks of rows per step of the scan: 32 warps, 8 blocks each
 }  // namespace group
 
@@ -27,10 +27,11 @@ __device__ __forceinline__ int group_of(int64_t id, int n_groups) {
 }
 
 __global__ void __launch_bounds__(group::kThreads)
-group_count_kernel(int32_t *__restrict__ block_counts, const int64_t *__restrict__ ids,
-                   int64_t rows, int n_groups) {
+group_count_kernel(int32_t *__restrict__ block_counts, unsigned *__restrict__ done,
+                   const int64_t *__restrict__ ids, int64_t rows, int n_groups) {
     extern __shared__ int32_t count_s[];  // [n_groups + 1]
     const int bins = n_groups + 1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
     for (int g = threadIdx.x; g < bins; g += group::kThreads) count_s[g] = 0;
     __syncthreads();
     const int64_t r0 = blockIdx.x * static_cast<int64_t>(group::kBlockRows);
@@ -65,9 +66,10 @@ __device__ __forceinline__ int64_t cta_exclusive(int64_t v, int64_t *warp_sum_s,
 }
 
 // Histograms of the blocks -> places of the blocks within their group; sums of the groups.  A lane
-// has a group, a warp eight consecutive blocks, so that loads and stores are whole lines.
+// has a group, a warp eight consecutive blocks, so that loads and stores are whole lines.  The CTA that
+// is done last adds up the groups.
 __global__ void __launch_bounds__(1024)
-group_scan_kernel(int32_t *__restrict__ totals, int32_t *__restrict__ block_counts, int n_blocks,
+group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ totals, unsigned *done, int32_t *__restrict__ block_counts, int n_blocks,
                   int n_groups) {
     __shared__ int32_t part_s[32][33];
     const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -103,65 +105,104 @@ group_scan_kernel(int32_t *__restrict__ totals, int32_t *__restrict__ block_coun
         __syncthreads();
     }
     if (w == 0 && g < bins) totals[g] = carry;
+    __shared__ bool last_s;
+    __shared__ int64_t warp_sum_s[32];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last_s = atomicAdd(done, 1u) == gridDim.x - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last_s) return;
+    int64_t base = 0;
+    for (int g0 = 0; g0 < bins; g0 += 1024) {
+        const int i = g0 + threadIdx.x;
+        int64_t total;
+        const int64_t at = cta_exclusive(i < bins ? __ldcg(totals + i) : 0, warp_sum_s, &total) + base;
+        if (i < bins) offsets[i] = at;  // [n_groups]: where the ungrouped rows start
+        base += total;
+    }
 }
 
-// block_counts == nullptr: this CTA has all rows and makes the offsets itself
-__global__ void __launch_bounds__(group::kThreads)
+// A warp has 256 consecutive rows, eight a lane, kept in registers from the count to the end.
+// block_counts == nullptr: this CTA has all rows and makes the offsets itself.
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
 group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
-                     const int32_t *__restrict__ block_counts, const int32_t *__restrict__ totals,
-                     const int64_t *__restrict__ ids, int64_t rows, int n_groups, int block_rows) {
-    extern __shared__ int32_t count_s[];  // [kWarps][n_groups + 1]
+                     const int32_t *__restrict__ block_counts, const int64_t *__restrict__ ids,
+                     int64_t rows, int n_groups) {
+    extern __shared__ int32_t count_s[];  // [WARPS][n_groups + 1]
     __shared__ int64_t warp_sum_s[32];
+    constexpr int kThreads = 32 * WARPS, kEach = 8;
     const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < group::kWarps * bins; i += group::kThreads) count_s[i] = 0;
+    const int64_t lo = (blockIdx.x * static_cast<int64_t>(WARPS) + w) * (32 * kEach) + lane;
+    int g[kEach];  // -1: no row
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        g[j] = lo + 32 * j < rows ? group_of(__ldg(ids + lo + 32 * j), n_groups) : -1;
+    for (int i = threadIdx.x; i < WARPS * bins; i += kThreads) count_s[i] = 0;
     __syncthreads();
-    const int64_t r0 = blockIdx.x * static_cast<int64_t>(block_rows);
-    const int n = static_cast<int>(min(static_cast<int64_t>(block_rows), rows - r0));
-    // each warp a run of whole groups of 32 rows
-    const int run = 32 * ((n + 32 * group::kWarps - 1) / (32 * group::kWarps));
-    const int lo = min(n, w * run), hi = min(n, lo + run);
     int32_t *mine = count_s + w * bins;
-    for (int i = lo + lane; i < hi; i += 32)
-        atomicAdd(&mine[group_of(__ldg(ids + r0 + i), n_groups)], 1);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        if (g[j] >= 0) atomicAdd(&mine[g[j]], 1);
     __syncthreads();
     // places: rows of earlier groups and blocks, then of earlier warps (32 bits: rows < 2^31)
     int64_t base = 0;
-    for (int g0 = 0; g0 < bins; g0 += group::kThreads) {
-        const int g = g0 + threadIdx.x;
-        int32_t sum = 0;
-        if (g < bins)
-            for (int i = 0; i < group::kWarps; ++i) sum += count_s[i * bins + g];
-        if (block_counts != nullptr) sum = g < bins ? totals[g] : 0;
-        int64_t total;
-        int64_t place = cta_exclusive(sum, warp_sum_s, &total) + base;
-        base += total;
-        if (blockIdx.x == 0 && g < bins) offsets[g] = place;  // [n_groups]: the ungrouped rows
-        if (block_counts != nullptr && g < bins)
-            place += block_counts[blockIdx.x * static_cast<int64_t>(bins) + g];
-        if (g < bins) {
+    for (int g0 = 0; g0 < bins; g0 += kThreads) {
+        const int i = g0 + threadIdx.x;
+        int64_t place = 0;
+        if (block_counts != nullptr) {
+            if (i < bins)
+                place = __ldg(offsets + i) +
+                        __ldg(block_counts + blockIdx.x * static_cast<int64_t>(bins) + i);
+        } else {
+            int32_t sum = 0;
+            if (i < bins)
+                for (int k = 0; k < WARPS; ++k) sum += count_s[k * bins + i];
+            int64_t total;
+            place = cta_exclusive(sum, warp_sum_s, &total) + base;
+            base += total;
+            if (i < bins) offsets[i] = place;
+        }
+        if (i < bins) {
             int32_t at = static_cast<int32_t>(place);
-            for (int i = 0; i < group::kWarps; ++i) {
-                const int32_t c = count_s[i * bins + g];
-                count_s[i * bins + g] = at;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k) {
+                const int32_t c = count_s[k * bins + i];
+                count_s[k * bins + i] = at;
                 at += c;
             }
         }
     }
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const bool live = i < hi;
-        // lanes past the end share a key that no row has
-        const int g = live ? group_of(__ldg(ids + r0 + i), n_groups) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, g);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const unsigned peers = __match_any_sync(0xffffffffu, g[j]);
         const int rank = __popc(peers & ((1u << lane) - 1u));
         int32_t at = 0;
-        if (live) at = mine[g];
+        if (g[j] >= 0) at = mine[g[j]];
         __syncwarp();
-        if (live && rank == 0) mine[g] = at + __popc(peers);
+        if (g[j] >= 0 && rank == 0) mine[g[j]] = at + __popc(peers);
         __syncwarp();
-        if (live) order[at + rank] = r0 + i;
+        if (g[j] >= 0) order[at + rank] = lo + 32 * j;
     }
+}
+
+template <int WARPS>
+int scatter_launch(int64_t *order, int64_t *offsets, const int32_t *counts, const int64_t *ids,
+                   int64_t rows, int n_groups, int blocks, cudaStream_t s) {
+    const size_t smem = static_cast<size_t>(WARPS) * (n_groups + 1) * sizeof(int32_t);
+    if (smem > 48 * 1024)
+        PA_CUDA_TRY(cudaFuncSetAttribute(group_scatter_kernel<WARPS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(smem)));
+    group_scatter_kernel<WARPS><<<blocks, 32 * WARPS, smem, s>>>(order, offsets, counts, ids, rows,
+                                                                 n_groups);
+    count_launch();
+    PA_CUDA_TRY(cudaGetLastError());
+    return PA_OK;
 }
 
 }  // namespace pa
@@ -169,7 +210,7 @@ group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
 extern "C" int64_t pa_group_rows_workspace_bytes(int64_t rows, int n_groups) {
     if (rows <= pa::group::kSingleRows || n_groups < 1) return 0;
     const int64_t blocks = (rows + pa::group::kBlockRows - 1) / pa::group::kBlockRows;
-    return (blocks + 1) * (n_groups + 1) * static_cast<int64_t>(sizeof(int32_t));
+    return ((blocks + 1) * (n_groups + 1) + 1) * static_cast<int64_t>(sizeof(int32_t));
 }
 
 extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *router, int64_t rows,
@@ -181,27 +222,21 @@ extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *ro
     PA_REQUIRE(offsets && (rows == 0 || (order && router)), "null pointer");
     const bool single = rows <= group::kSingleRows;
     PA_REQUIRE(single || workspace, "workspace missing (pa_group_rows_workspace_bytes)");
-    const int bins = n_groups + 1;
-    const int blocks =
-        single ? 1 : static_cast<int>((rows + group::kBlockRows - 1) / group::kBlockRows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const size_t scatter_smem = static_cast<size_t>(group::kWarps) * bins * sizeof(int32_t);
-    if (scatter_smem > 48 * 1024)
-        PA_CUDA_TRY(cudaFuncSetAttribute(group_scatter_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(scatter_smem)));
-    int32_t *counts = single ? nullptr : static_cast<int32_t *>(workspace);
-    int32_t *totals = single ? nullptr : counts + static_cast<int64_t>(blocks) * bins;
-    if (!single) {
-        group_count_kernel<<<blocks, group::kThreads, bins * sizeof(int32_t), s>>>(counts, router,
-                                                                                   rows, n_groups);
-        group_scan_kernel<<<(bins + 31) / 32, 1024, 0, s>>>(totals, counts, blocks, n_groups);
-        count_launch(2);
-    }
-    group_scatter_kernel<<<blocks, group::kThreads, scatter_smem, s>>>(
-        order, offsets, counts, totals, router, rows, n_groups,
-        single ? group::kSingleRows : group::kBlockRows);
-    count_launch();
+    if (rows <= group::kBlockRows)
+        return scatter_launch<group::kWarps>(order, offsets, nullptr, router, rows, n_groups, 1, s);
+    if (single)
+        return scatter_launch<2 * group::kWarps>(order, offsets, nullptr, router, rows, n_groups, 1, s);
+    const int bins = n_groups + 1;
+    const int blocks = static_cast<int>((rows + group::kBlockRows - 1) / group::kBlockRows);
+    int32_t *counts = static_cast<int32_t *>(workspace);
+    int32_t *totals = counts + static_cast<int64_t>(blocks) * bins;
+    unsigned *done = reinterpret_cast<unsigned *>(totals + bins);
+    group_count_kernel<<<blocks, group::kThreads, bins * sizeof(int32_t), s>>>(counts, done, router,
+                                                                               rows, n_groups);
+    group_scan_kernel<<<(bins + 31) / 32, 1024, 0, s>>>(offsets, totals, done, counts, blocks,
+                                                        n_groups);
+    count_launch(2);
     PA_CUDA_TRY(cudaGetLastError());
-    return PA_OK;
+    return scatter_launch<group::kWarps>(order, offsets, counts, router, rows, n_groups, blocks, s);
 }
