@@ -15,6 +15,8 @@ MAX_GROUPS = 1024
 MAX_WIDTH = 65536
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOATS = tuple(_DTYPE)
+_INT64 = (torch.int64,)
 _METHOD = {"mxfp4": 0, "nvfp4": 1}
 _BLOCK = {"mxfp4": 32, "nvfp4": 16}
 
@@ -52,13 +54,17 @@ def _same_device(a: torch.Tensor, name: str, x: torch.Tensor) -> None:
         raise RuntimeError(f"{name} must be on {a.device}, got {x.device}")
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream     # a number, without a Stream object around it
+# The calls of a small batch are as long as their Python side: the raw handle instead of a Stream
+# object saves 2 us of 10, checks that stop at the first look at sound arguments 2 to 3.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_empty = torch.empty
 
 
 def _call(device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on the tensors' device and its current stream."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
@@ -74,15 +80,16 @@ def group_rows(router: torch.Tensor, n_groups: int):
     are the rows of group ``g``, ascending.  Rows whose id is not in ``[0, n_groups)`` come
     last, behind ``offsets[n_groups]``.  ``x[order]`` is what :func:`project_grouped` takes;
     ``y.new_empty(y.shape).index_copy_(0, order, y)`` brings its result back."""
-    _check("router", router, 1, (torch.int64,))
+    _check("router", router, 1, _INT64)
     _contiguous("router", router)
-    _require(1 <= n_groups <= MAX_GROUPS, f"1 <= n_groups <= {MAX_GROUPS}")
+    if not 1 <= n_groups <= MAX_GROUPS:
+        _require(False, f"1 <= n_groups <= {MAX_GROUPS}")
     rows, dev = router.size(0), router.device
-    order = torch.empty(rows, dtype=torch.int64, device=dev)
-    offsets = torch.empty(n_groups + 1, dtype=torch.int64, device=dev)
+    order = torch.empty_like(router)
+    offsets = _empty(n_groups + 1, dtype=torch.int64, device=dev)
     L = _C.lib()
     need = L.pa_group_rows_workspace_bytes(rows, n_groups)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = _empty(need, dtype=torch.uint8, device=dev) if need else None
     _call(dev, L.pa_group_rows, order.data_ptr(), offsets.data_ptr(), router.data_ptr(), rows,
           n_groups, 0 if ws is None else ws.data_ptr())
     return order, offsets
@@ -90,9 +97,21 @@ def group_rows(router: torch.Tensor, n_groups: int):
 
 # ---- a matrix per group --------------------------------------------------------------
 def _grouped_checks(query, VT, offsets) -> None:
-    _check("query", query, 2, tuple(_DTYPE))
+    try:
+        if (query.is_cuda and VT.is_cuda and offsets.is_cuda and query.dtype in _DTYPE
+                and VT.dtype is query.dtype and offsets.dtype is torch.int64
+                and query.device == VT.device == offsets.device
+                and VT.is_contiguous() and offsets.is_contiguous()):
+            n_groups, d_out, d = VT.shape
+            if (query.size(1) == d and query.dim() == 2 and offsets.shape == (n_groups + 1,)
+                    and 1 <= n_groups <= MAX_GROUPS and 1 <= d_out <= MAX_WIDTH
+                    and 1 <= d <= MAX_WIDTH):
+                return
+    except (AttributeError, IndexError, ValueError):
+        pass
+    _check("query", query, 2, _FLOATS)
     _check("VT", VT, 3, (query.dtype,))
-    _check("offsets", offsets, 1, (torch.int64,))
+    _check("offsets", offsets, 1, _INT64)
     _contiguous("VT", VT)
     _contiguous("offsets", offsets)
     _same_device(query, "VT", VT)
@@ -110,9 +129,10 @@ def _grouped_forward(query, VT, offsets):
     dev, dtype = query.device, _DTYPE[query.dtype]
     L = _C.lib()
     q, w, ld = query.data_ptr(), VT.data_ptr(), _row_stride("query", query)
-    need = L.pa_project_grouped_workspace_bytes(q, w, rows, n_groups, d, d_out, ld, dtype)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    out = torch.empty(rows, d_out, dtype=query.dtype, device=dev)
+    need = 0 if dtype == 0 or ((q | w) % 16 == 0 and (d | ld) % 8 == 0) else \
+        L.pa_project_grouped_workspace_bytes(q, w, rows, n_groups, d, d_out, ld, dtype)
+    ws = _empty(need, dtype=torch.uint8, device=dev) if need else None
+    out = _empty(rows, d_out, dtype=query.dtype, device=dev)
     _call(dev, L.pa_project_grouped, out.data_ptr(), q, w, offsets.data_ptr(), rows, n_groups, d,
           d_out, ld, d_out, dtype, 0 if ws is None else ws.data_ptr())
     return out
@@ -125,11 +145,12 @@ def _grouped_backward(grad, query, VT, offsets, want_query, want_VT):
     L = _C.lib()
     y, q, w = grad.data_ptr(), query.data_ptr(), VT.data_ptr()
     ldy, ldq = _row_stride("grad", grad), _row_stride("query", query)
-    need = L.pa_project_grouped_backward_workspace_bytes(y, q, w, rows, n_groups, d, d_out, ldy, ldq,
-                                                         dtype, want_query, want_VT)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    dq = torch.empty(rows, d, dtype=query.dtype, device=dev) if want_query else None
-    dw = torch.empty(n_groups, d_out, d, dtype=query.dtype, device=dev) if want_VT else None
+    need = 0 if dtype == 0 or ((y | q | w) % 16 == 0 and (d | ldy | ldq) % 8 == 0) else \
+        L.pa_project_grouped_backward_workspace_bytes(y, q, w, rows, n_groups, d, d_out, ldy, ldq,
+                                                      dtype, want_query, want_VT)
+    ws = _empty(need, dtype=torch.uint8, device=dev) if need else None
+    dq = _empty(rows, d, dtype=query.dtype, device=dev) if want_query else None
+    dw = torch.empty_like(VT) if want_VT else None
     _call(dev, L.pa_project_grouped_backward, 0 if dq is None else dq.data_ptr(),
           0 if dw is None else dw.data_ptr(), y, q, w, offsets.data_ptr(), rows, n_groups, d, d_out,
           ldy, ldq, d, dtype, 0 if ws is None else ws.data_ptr())
@@ -146,6 +167,9 @@ class _ProjectGrouped(torch.autograd.Function):
     def backward(ctx, grad):
         if torch.is_grad_enabled():       # create_graph: the gradients have none themselves
             raise RuntimeError("project_grouped can be differentiated only once")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("project_grouped is not differentiated in a stream capture: call "
+                               "project_grouped_backward")
         query, VT, offsets = ctx.saved_tensors
         if not grad.is_contiguous() and (grad.stride(1) != 1 or grad.stride(0) < grad.size(1)):
             grad = grad.contiguous()      # an expanded gradient, as of a sum
@@ -252,19 +276,25 @@ def quantize_fp4(x: torch.Tensor, method: str = "mxfp4") -> Fp4Table:
     if method not in _METHOD:
         raise RuntimeError(f"unknown 4-bit method {method!r}: mxfp4 or nvfp4")
     dim = x.dim() if isinstance(x, torch.Tensor) else 2
-    _require(dim in (2, 3), "x.dim() in (2, 3)")
-    _check("x", x, dim, tuple(_DTYPE))
-    d = x.size(-1)
-    _require(1 <= d <= MAX_WIDTH, f"1 <= d <= {MAX_WIDTH}")
-    if dim == 3:
+    if dim not in (2, 3):
+        _require(False, "x.dim() in (2, 3)")
+    _check("x", x, dim, _FLOATS)
+    d, dev = x.size(-1), x.device
+    if not 1 <= d <= MAX_WIDTH:
+        _require(False, f"1 <= d <= {MAX_WIDTH}")
+    width, blocks = (d + 31) // 32 * 16, (d + 31) // 32 * (32 // _BLOCK[method])
+    row_scale = None
+    if dim == 2:
+        rows, ld = x.size(0), _row_stride("x", x)
+        codes = _empty(rows, width, dtype=torch.uint8, device=dev)
+        scales = _empty(rows, blocks, dtype=torch.uint8, device=dev)
+    else:
         _contiguous("x", x)
-    ld = d if dim == 3 else _row_stride("x", x)
-    lead, dev = x.shape[:-1], x.device
-    rows = x.size(0) if dim == 2 else x.size(0) * x.size(1)
-    padded = -(-d // 32) * 32
-    codes = torch.empty(*lead, padded // 2, dtype=torch.uint8, device=dev)
-    scales = torch.empty(*lead, padded // _BLOCK[method], dtype=torch.uint8, device=dev)
-    row_scale = torch.empty(lead, dtype=torch.float32, device=dev) if method == "nvfp4" else None
+        rows, ld = x.size(0) * x.size(1), d
+        codes = _empty(x.size(0), x.size(1), width, dtype=torch.uint8, device=dev)
+        scales = _empty(x.size(0), x.size(1), blocks, dtype=torch.uint8, device=dev)
+    if method == "nvfp4":
+        row_scale = _empty(x.shape[:-1], dtype=torch.float32, device=dev)
     _call(dev, _C.lib().pa_quantize_fp4, codes.data_ptr(), scales.data_ptr(),
           0 if row_scale is None else row_scale.data_ptr(), x.data_ptr(), rows, d, ld,
           _DTYPE[x.dtype], _METHOD[method])
@@ -278,10 +308,17 @@ def dequantize_fp4(table: Fp4Table) -> torch.Tensor:
     """What the codes stand for, float32 of ``table.shape``."""
     if not isinstance(table, Fp4Table):
         raise RuntimeError("table must be an Fp4Table")
-    out = torch.empty(table.shape, dtype=torch.float32, device=table.device)
-    _call(table.device, _C.lib().pa_dequantize_fp4, out.data_ptr(), table.codes.data_ptr(),
-          table.scales.data_ptr(), 0 if table.row_scale is None else table.row_scale.data_ptr(),
-          table.codes.shape[:-1].numel(), table.d, _METHOD[table.method])
+    codes, row_scale, dev = table.codes, table.row_scale, table.codes.device
+    shape = codes.shape
+    if len(shape) == 2:
+        rows = shape[0]
+        out = _empty(rows, table.d, dtype=torch.float32, device=dev)
+    else:
+        rows = shape[0] * shape[1]
+        out = _empty(shape[0], shape[1], table.d, dtype=torch.float32, device=dev)
+    _call(dev, _C.lib().pa_dequantize_fp4, out.data_ptr(), codes.data_ptr(),
+          table.scales.data_ptr(), 0 if row_scale is None else row_scale.data_ptr(), rows,
+          table.d, _METHOD[table.method])
     return out
 
 
@@ -296,14 +333,14 @@ def project_fp4(query, table: Fp4Table, offsets: torch.Tensor | None = None,
         raise RuntimeError("table must be an Fp4Table")
     if dtype not in _DTYPE:
         raise RuntimeError(f"dtype must be one of {' or '.join(map(str, _DTYPE))}")
-    dev, d, method = table.device, table.d, table.method
-    codes = table.codes
+    codes, d, method = table.codes, table.d, table.method
+    dev = codes.device
     if offsets is None:
         _require(codes.dim() == 2, "table of [rows, d] without offsets")
         n_groups, d_out = 1, codes.size(0)
     else:
         _require(codes.dim() == 3, "table of [n_groups, d_out, d] with offsets")
-        _check("offsets", offsets, 1, (torch.int64,))
+        _check("offsets", offsets, 1, _INT64)
         _contiguous("offsets", offsets)
         _same_device(codes, "offsets", offsets)
         n_groups, d_out = codes.size(0), codes.size(1)
@@ -320,19 +357,20 @@ def project_fp4(query, table: Fp4Table, offsets: torch.Tensor | None = None,
         q = (query.codes.data_ptr(), query.scales.data_ptr(),
              0 if query.row_scale is None else query.row_scale.data_ptr())
     else:
-        _check("query", query, 2, tuple(_DTYPE))
-        _require(query.size(1) == d, "query.size(1) == table.d")
+        _check("query", query, 2, _FLOATS)
+        if query.size(1) != d:
+            _require(False, "query.size(1) == table.d")
         _same_device(codes, "query", query)
         rows = query.size(0)
         ld = _row_stride("query", query)
         # scratch: codes, row scales, block scales of the quantised queries
         width = padded // 2 + 4 + padded // _BLOCK[method]
-        ws = torch.empty(rows * width, dtype=torch.uint8, device=dev)
+        ws = _empty(rows * width, dtype=torch.uint8, device=dev)
         at = ws.data_ptr()
         q = (at, at + rows * (padded // 2 + 4), at + rows * (padded // 2))
         _call(dev, L.pa_quantize_fp4, q[0], q[1], q[2] if method == "nvfp4" else 0,
               query.data_ptr(), rows, d, ld, _DTYPE[query.dtype], _METHOD[method])
-    out = torch.empty(rows, d_out, dtype=dtype, device=dev)
+    out = _empty(rows, d_out, dtype=dtype, device=dev)
     _call(dev, L.pa_project_fp4, out.data_ptr(), *q, codes.data_ptr(), table.scales.data_ptr(),
           0 if table.row_scale is None else table.row_scale.data_ptr(),
           0 if offsets is None else offsets.data_ptr(), rows, n_groups, d, d_out, _DTYPE[dtype],
