@@ -6,169 +6,222 @@
 // Rows before offsets[0] and from offsets[n_groups] on belong to no group: y and dx are zero
 // there.  Offsets are clamped to [0, rows], so that none of them makes an access leave the
 // tensors, whatever they hold.
+#include <cooperative_groups.h>
+
 #include "grouped.cuh"
+#include "tc05.cuh"
 
 namespace pa {
 
 namespace grouped {
 
+namespace cg = cooperative_groups;
+
 // ---- fp32 values: fma on the CUDA cores ---------------------------------------------
 // Tiles of TR rows x TC columns by 256 threads, each TR / 16 x TC / 16 outputs:
 //   C[r, c] = sum_t P(r, t) Q(c, t), P(r, t) = p[r * pr + t * pt], Q likewise,
-// where the axis that is contiguous in memory is t (T_FAST) or r, c.  Slices of 16 t go through
-// registers into two buffers in shared memory, the next one on its way while one is multiplied.
+// where the axis that is contiguous in memory is t (T_FAST) or r, c.  Slices of 16 t are copied to
+// shared memory as they lie there, asynchronously and up to five slices ahead (a slice of a small
+// tile is multiplied in 150 cycles, its data is 800 away), and read 16 bytes a thread.
 // A sum is kept in two levels, 256 terms at a time, so that its error grows with the square root of
 // 256 terms rather than of all (65536 rows in one sum: 5e-6 of the result in one level, below 1e-6 in
-// two).  128 x 128 tiles are bound by the fma units, smaller ones by latency and by the loads
-// from shared memory.
+// two).  Where there are fewer tiles than the GPU can hold, a cluster of up to eight CTAs shares a tile
+// and its sum, and adds the parts in order through distributed shared memory.
+// 128 x 128 tiles are bound by the fma units, smaller ones by their loads.
 constexpr int kK = 16;
 constexpr int kTerms = 256;
+constexpr int kPitch = kK + 4;  // of a row of a T_FAST slice: 8 rows fall into different banks
 
-template <int T, bool T_FAST> struct Slice {
-    static constexpr int kEach = T * kK / 256;  // values a thread loads
-    float v[kEach];
-
-    // 16-byte loads where there are four values a thread and rows start on 16 bytes (`vec`)
-    __device__ __forceinline__ void load(const float *p, int64_t pr, int64_t pt, int n_r, int64_t t0,
-                                         int64_t n_t, bool vec) {
-        const int tid = threadIdx.x;
-        if (kEach >= 4 && vec) {
-#pragma unroll
-            for (int i = 0; i < kEach / 4; ++i) {
-                const int j = tid + 256 * i;
-                const int r = T_FAST ? j / 4 : 4 * (j % (T / 4)), t = T_FAST ? 4 * (j % 4) : j / (T / 4);
-                float4 x = make_float4(0, 0, 0, 0);
-                const float *q = p + (T_FAST ? r * pr + t0 + t : r + (t0 + t) * pt);
-                const int64_t left = T_FAST ? (r < n_r ? n_t - t0 - t : 0) : (t0 + t < n_t ? n_r - r : 0);
-                if (left >= 4) {
-                    x = __ldg(reinterpret_cast<const float4 *>(q));
-                } else {
-                    if (left > 0) x.x = __ldg(q);
-                    if (left > 1) x.y = __ldg(q + 1);
-                    if (left > 2) x.z = __ldg(q + 2);
-                }
-                v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int j = tid + 256 * i;
-                const int r = T_FAST ? j / kK : j % T, t = T_FAST ? j % kK : j / T;
-                v[i] = r < n_r && t0 + t < n_t ? __ldg(p + r * pr + (t0 + t) * pt) : 0.0f;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(float (*to)[T + 4], bool vec) const {
-        const int tid = threadIdx.x;
-        if (kEach >= 4 && vec) {
-#pragma unroll
-            for (int i = 0; i < kEach / 4; ++i) {
-                const int j = tid + 256 * i;
-                if (T_FAST) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) to[4 * (j % 4) + k][j / 4] = v[4 * i + k];
-                } else {
-                    *reinterpret_cast<float4 *>(&to[j / (T / 4)][4 * (j % (T / 4))]) =
-                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int j = tid + 256 * i;
-                to[T_FAST ? j % kK : j / T][T_FAST ? j / kK : j % T] = v[i];
-            }
-        }
-    }
-};
-
-// outputs of a thread along an axis of T: four neighbours per 64, or T / 16 neighbours
-template <int T> __device__ __forceinline__ int place(int thread, int i) {
-    return T >= 64 ? 64 * (i / 4) + 4 * thread + i % 4 : (T / 16) * thread + i;
+template <int T, bool T_FAST> __host__ __device__ constexpr int slice_floats() {
+    return T_FAST ? T * kPitch : kK * (T + 4);
 }
-template <int T>
-__device__ __forceinline__ void fetch(float (&v)[T / 16], const float *row, int thread) {
-    if (T >= 64) {
+template <int TR, int TC> __host__ __device__ constexpr int slices() {
+    return TR * TC >= 128 * 128 ? 3 : TR * TC >= 64 * 64 ? 5 : 6;
+}
+
+__device__ __forceinline__ void copy_async(float *to, const float *from, int floats) {  // of 4
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc05::smem_u32(to)),
+                 "l"(from), "r"(4 * floats)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_async1(float *to, const float *from, bool some) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc05::smem_u32(to)),
+                 "l"(from), "r"(some ? 4 : 0)
+                 : "memory");
+}
+
+// t0 .. t0 + 16 of the operand to `to`; zeros behind n_r, n_t.  vec: rows start on 16 bytes.
+template <int T, bool T_FAST>
+__device__ __forceinline__ void slice_load(float *to, const float *p, int64_t pr, int64_t pt, int n_r,
+                                           int64_t t0, int64_t n_t, bool vec) {
+    constexpr int kPieces = T * kK / 4;
+    if (vec) {
 #pragma unroll
-        for (int i = 0; i < T / 64; ++i) {
-            const float4 x = *reinterpret_cast<const float4 *>(row + 64 * i + 4 * thread);
-            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        for (int j = threadIdx.x; j < kPieces; j += 256) {
+            const int r = T_FAST ? j / 4 : 4 * (j % (T / 4)), t = T_FAST ? 4 * (j % 4) : j / (T / 4);
+            const int64_t left = T_FAST ? (r < n_r ? n_t - t0 - t : 0) : (t0 + t < n_t ? n_r - r : 0);
+            const int have = static_cast<int>(left < 0 ? 0 : left > 4 ? 4 : left);
+            const float *from = T_FAST ? p + r * pr + t0 + t : p + (t0 + t) * pt + r;
+            copy_async(to + (T_FAST ? r * kPitch + t : t * (T + 4) + r), have ? from : p, have);
+        }
+    } else {
+#pragma unroll 4
+        for (int j = threadIdx.x; j < 4 * kPieces; j += 256) {
+            const int r = T_FAST ? j / kK : j % T, t = T_FAST ? j % kK : j / T;
+            const bool some = r < n_r && t0 + t < n_t;
+            copy_async1(to + (T_FAST ? r * kPitch + t : t * (T + 4) + r),
+                        some ? p + r * pr + (t0 + t) * pt : p, some);
+        }
+    }
+}
+
+// the T / 16 rows of an operand that a thread has: every 16th of a T_FAST one, else four neighbours
+// per 64 (or T / 16 neighbours)
+template <int T, bool T_FAST> __device__ __forceinline__ int place(int thread, int i) {
+    return T_FAST ? thread + 16 * i
+           : T >= 64 ? 64 * (i / 4) + 4 * thread + i % 4 : (T / 16) * thread + i;
+}
+// v[k][i]: value t + k of row i of the thread
+template <int T, bool T_FAST>
+__device__ __forceinline__ void fetch4(float (&v)[4][T / 16], const float *s, int t, int thread) {
+    if (T_FAST) {
+#pragma unroll
+        for (int i = 0; i < T / 16; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(s + (thread + 16 * i) * kPitch + t);
+            v[0][i] = x.x; v[1][i] = x.y; v[2][i] = x.z; v[3][i] = x.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < T / 16; ++i) v[i] = row[place<T>(thread, i)];
-    }
-}
-
-template <int TR, int TC> struct Buffers {
-    __align__(16) float p[2][kK][TR + 4];
-    __align__(16) float q[2][kK][TC + 4];
-};
-
-template <int TR, int TC, bool P_T_FAST, bool Q_T_FAST>
-__device__ __forceinline__ void tile_product(float (&acc)[TR / 16][TC / 16], Buffers<TR, TC> &s,
-                                             const float *p, int64_t pr, int64_t pt, int n_r,
-                                             bool p_vec, const float *q, int64_t qc, int64_t qt,
-                                             int n_c, bool q_vec, int64_t n_t) {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    Slice<TR, P_T_FAST> ps;
-    Slice<TC, Q_T_FAST> qs;
-    float part[TR / 16][TC / 16] = {};
-    ps.load(p, pr, pt, n_r, 0, n_t, p_vec);
-    qs.load(q, qc, qt, n_c, 0, n_t, q_vec);
-    int b = 0;
-    for (int64_t t0 = 0; t0 < n_t; t0 += kK, b ^= 1) {
-        ps.store(s.p[b], p_vec);
-        qs.store(s.q[b], q_vec);
-        __syncthreads();  // (the other buffer was read before the barrier of the slice before)
-        if (t0 + kK < n_t) {
-            ps.load(p, pr, pt, n_r, t0 + kK, n_t, p_vec);
-            qs.load(q, qc, qt, n_c, t0 + kK, n_t, q_vec);
-        }
+        for (int k = 0; k < 4; ++k) {
+            const float *row = s + (t + k) * (T + 4);
+            if constexpr (T >= 64) {
 #pragma unroll
-        for (int t = 0; t < kK; ++t) {
-            float av[TR / 16], bv[TC / 16];
-            fetch<TR>(av, s.p[b][t], ty);
-            fetch<TC>(bv, s.q[b][t], tx);
-#pragma unroll
-            for (int i = 0; i < TR / 16; ++i)
-#pragma unroll
-                for (int j = 0; j < TC / 16; ++j) part[i][j] = __fmaf_rn(av[i], bv[j], part[i][j]);
-        }
-        if ((t0 + kK) % kTerms == 0 || t0 + kK >= n_t) {
-#pragma unroll
-            for (int i = 0; i < TR / 16; ++i)
-#pragma unroll
-                for (int j = 0; j < TC / 16; ++j) {
-                    acc[i][j] += part[i][j];
-                    part[i][j] = 0.0f;
+                for (int i = 0; i < T / 64; ++i) {
+                    const float4 x = *reinterpret_cast<const float4 *>(row + 64 * i + 4 * thread);
+                    v[k][4 * i] = x.x; v[k][4 * i + 1] = x.y;
+                    v[k][4 * i + 2] = x.z; v[k][4 * i + 3] = x.w;
                 }
-        }
-    }
-}
-
-template <int TR, int TC>
-__device__ __forceinline__ void tile_store(const float (&acc)[TR / 16][TC / 16], float *out,
-                                           int64_t ldo, int n_r, int n_c, bool vec) {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < TR / 16; ++i) {
-        const int r = place<TR>(ty, i);
-        if (r >= n_r) continue;
-#pragma unroll
-        for (int j = 0; j < TC / 16; j += 4) {
-            const int c = place<TC>(tx, j);
-            float *to = out + r * ldo + c;
-            if (vec && c + 4 <= n_c) {
-                *reinterpret_cast<float4 *>(to) =
-                    make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (c + k < n_c) to[k] = acc[i][j + k];
+                for (int i = 0; i < T / 16; ++i) v[k][i] = row[(T / 16) * thread + i];
             }
         }
     }
+}
+
+template <int TR, int TC, bool PF, bool QF> __host__ __device__ constexpr int tile_bytes() {
+    return 4 * slices<TR, TC>() * (slice_floats<TR, PF>() + slice_floats<TC, QF>());
+}
+
+struct Operand {
+    const float *p;
+    int64_t pr, pt;
+    int n;
+    bool vec;
+};
+
+template <int TR, int TC, bool PF, bool QF>
+__device__ __forceinline__ void tile_product(float (&acc)[TR / 16][TC / 16], float *smem,
+                                             const Operand &p, const Operand &q, int64_t n_t) {
+    constexpr int S = slices<TR, TC>(), P = slice_floats<TR, PF>(), ALL = P + slice_floats<TC, QF>();
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int n_slices = static_cast<int>((n_t + kK - 1) / kK);
+    auto load = [&](int i) {
+        if (i < n_slices) {
+            float *to = smem + (i % S) * ALL;
+            slice_load<TR, PF>(to, p.p, p.pr, p.pt, p.n, static_cast<int64_t>(i) * kK, n_t, p.vec);
+            slice_load<TC, QF>(to + P, q.p, q.pr, q.pt, q.n, static_cast<int64_t>(i) * kK, n_t, q.vec);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float part[TR / 16][TC / 16] = {};
+    for (int i = 0; i < S - 1; ++i) load(i);
+    for (int i = 0; i < n_slices; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncthreads();  // slice i is here for all, slice i - 1 has been read by all
+        load(i + S - 1);
+        const float *ps = smem + (i % S) * ALL, *qs = ps + P;
+#pragma unroll
+        for (int t = 0; t < kK; t += 4) {
+            float a[4][TR / 16], b[4][TC / 16];
+            fetch4<TR, PF>(a, ps, t, ty);
+            fetch4<TC, QF>(b, qs, t, tx);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int x = 0; x < TR / 16; ++x)
+#pragma unroll
+                    for (int y = 0; y < TC / 16; ++y)
+                        part[x][y] = __fmaf_rn(a[k][x], b[k][y], part[x][y]);
+        }
+        if ((i + 1) % (kTerms / kK) == 0 || i + 1 == n_slices) {
+#pragma unroll
+            for (int x = 0; x < TR / 16; ++x)
+#pragma unroll
+                for (int y = 0; y < TC / 16; ++y) {
+                    acc[x][y] += part[x][y];
+                    part[x][y] = 0.0f;
+                }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+}
+
+// The tile to memory.  In a cluster the CTAs have parts of the sum: each adds up, in the order of the
+// CTAs, its share of the tile.
+template <int TR, int TC, bool PF, bool QF>
+__device__ __forceinline__ void tile_store(const float (&acc)[TR / 16][TC / 16], float *smem, float *out,
+                                           int64_t ldo, int n_r, int n_c, bool vec) {
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = cluster.num_blocks();
+    if (parts == 1) {
+#pragma unroll
+        for (int i = 0; i < TR / 16; ++i) {
+            const int r = place<TR, PF>(ty, i);
+#pragma unroll
+            for (int j = 0; j < TC / 16; j += QF ? 1 : 4) {
+                const int c = place<TC, QF>(tx, j);
+                if constexpr (!QF) {
+                    if (r < n_r && c + 4 <= n_c && vec) {
+                        *reinterpret_cast<float4 *>(out + r * ldo + c) =
+                            make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (r < n_r && c + k < n_c) out[r * ldo + c + k] = acc[i][j + k];
+                    }
+                } else if (r < n_r && c < n_c) {
+                    out[r * ldo + c] = acc[i][j];
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < TR / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < TC / 16; ++j)
+            smem[place<TR, PF>(ty, i) * TC + place<TC, QF>(tx, j)] = acc[i][j];
+    cluster.sync();
+    const int share = TR * TC / parts, first = share * cluster.block_rank();
+    for (int e = first + threadIdx.x; e < first + share; e += 256) {
+        float v = 0.0f;
+        for (int k = 0; k < parts; ++k) v += cluster.map_shared_rank(smem, k)[e];
+        const int r = e / TC, c = e % TC;
+        if (r < n_r && c < n_c) out[r * ldo + c] = v;
+    }
+    cluster.sync();  // no CTA leaves while its part is read
+}
+
+// this CTA's share of a sum of n terms: whole slices
+__device__ __forceinline__ void share_of(int64_t &lo, int64_t &hi) {
+    const int parts = gridDim.z, k = blockIdx.z;  // a cluster spans z
+    const int64_t n = hi - lo, each = (n + static_cast<int64_t>(parts) * kK - 1) / (parts * kK) * kK;
+    const int64_t a = min(hi, lo + k * each);
+    hi = min(hi, a + each);
+    lo = a;
 }
 
 // The rows of slot `slot` of T rows: segment i owns the slots from floor(edge_i / T) + i on, which are
@@ -196,42 +249,45 @@ __global__ void __launch_bounds__(256)
 rows_kernel(float *__restrict__ out, const float *__restrict__ x, const float *__restrict__ w,
             const int64_t *__restrict__ offsets, int64_t rows, int n_groups, int d_sum, int d_out,
             int64_t ldx, int64_t ldo, bool x_vec, bool w_vec, bool out_vec) {
-    __shared__ Buffers<TR, TC> s;
+    extern __shared__ __align__(16) float smem[];
     SlotRows slot;
-    if (!slot_rows(slot, offsets, rows, n_groups, blockIdx.x, TR)) return;
+    if (!slot_rows(slot, offsets, rows, n_groups, blockIdx.x, TR)) return;  // the whole cluster
     const int c0 = blockIdx.y * TC, n_c = min(TC, d_out - c0);
     float acc[TR / 16][TC / 16] = {};
     if (slot.seg >= 1 && slot.seg <= n_groups) {
+        int64_t lo = 0, hi = d_sum;
+        share_of(lo, hi);
         const float *wg = w + static_cast<int64_t>(slot.seg - 1) * d_sum * d_out;
-        const float *xr = x + slot.r0 * ldx;
-        if (W_T_FAST)
-            tile_product<TR, TC, true, true>(acc, s, xr, ldx, 1, slot.n_r, x_vec,
-                                             wg + static_cast<int64_t>(c0) * d_sum, d_sum, 1, n_c,
-                                             w_vec, d_sum);
-        else
-            tile_product<TR, TC, true, false>(acc, s, xr, ldx, 1, slot.n_r, x_vec, wg + c0, 1, d_out,
-                                              n_c, w_vec, d_sum);
+        const Operand p{x + slot.r0 * ldx + lo, ldx, 1, slot.n_r, x_vec};
+        const Operand q = W_T_FAST
+                              ? Operand{wg + static_cast<int64_t>(c0) * d_sum + lo, d_sum, 1, n_c, w_vec}
+                              : Operand{wg + lo * d_out + c0, 1, d_out, n_c, w_vec};
+        tile_product<TR, TC, true, W_T_FAST>(acc, smem, p, q, hi - lo);
     }
-    tile_store<TR, TC>(acc, out + slot.r0 * ldo + c0, ldo, slot.n_r, n_c, out_vec);
+    tile_store<TR, TC, true, W_T_FAST>(acc, smem, out + slot.r0 * ldo + c0, ldo, slot.n_r, n_c,
+                                        out_vec);
 }
 
-// Gradient of the matrices: one tile of one group per CTA, summed over its rows.
+// Gradient of the matrices: one tile of one group, summed over its rows.  blockIdx.x = tile along d
+// and group.
 template <int T>
 __global__ void __launch_bounds__(256)
 matrices_kernel(float *__restrict__ dw, const float *__restrict__ dy, const float *__restrict__ x,
                 const int64_t *__restrict__ offsets, int64_t rows, int n_groups, int d, int d_out,
                 int64_t ldy, int64_t ldx, bool y_vec, bool x_vec, bool out_vec) {
-    __shared__ Buffers<T, T> s;
-    const int g = blockIdx.z;
-    const int n0 = blockIdx.y * T, k0 = blockIdx.x * T;
+    extern __shared__ __align__(16) float smem[];
+    const int d_tiles = (d + T - 1) / T, g = blockIdx.x / d_tiles;
+    const int n0 = blockIdx.y * T, k0 = (blockIdx.x - g * d_tiles) * T;
     const int n_n = min(T, d_out - n0), n_k = min(T, d - k0);
-    const int64_t lo = edge(offsets, n_groups, rows, g + 1),
-                  hi = edge(offsets, n_groups, rows, g + 2);
+    int64_t lo = edge(offsets, n_groups, rows, g + 1), hi = edge(offsets, n_groups, rows, g + 2);
     float acc[T / 16][T / 16] = {};
-    if (hi > lo)
-        tile_product<T, T, false, false>(acc, s, dy + lo * ldy + n0, 1, ldy, n_n, y_vec,
-                                         x + lo * ldx + k0, 1, ldx, n_k, x_vec, hi - lo);
-    tile_store<T, T>(acc, dw + (static_cast<int64_t>(g) * d_out + n0) * d + k0, d, n_n, n_k, out_vec);
+    if (hi > lo) {
+        share_of(lo, hi);
+        const Operand p{dy + lo * ldy + n0, 1, ldy, n_n, y_vec}, q{x + lo * ldx + k0, 1, ldx, n_k, x_vec};
+        tile_product<T, T, false, false>(acc, smem, p, q, hi - lo);
+    }
+    tile_store<T, T, false, false>(acc, smem, dw + (static_cast<int64_t>(g) * d_out + n0) * d + k0, d,
+                                   n_n, n_k, out_vec);
 }
 
 // Forward of groups of a few rows, which read their matrix and do little with it: a warp has two rows
@@ -387,20 +443,48 @@ int matrices_make_ok(const void **w, int64_t *ld, int n_groups, int d, int d_out
 
 bool vec4(const void *p, int64_t ld) { return aligned16(p) && ld % 4 == 0; }
 
+// CTAs that share a tile: until there are two for every SM, with 128 terms each at least
+int parts_of(int64_t tiles, int64_t terms) {
+    int parts = 1;
+    while (parts < 8 && tiles * parts < 2 * 148 && terms >= 2 * 128 * parts) parts *= 2;
+    return parts;
+}
+
+template <typename... P, typename... A>
+int launch_tiles(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t s, A... args) {
+    if (smem > 48 * 1024)
+        PA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(256);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = cluster.val.clusterDim.y = 1;
+    cluster.val.clusterDim.z = grid.z;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    PA_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
+    count_launch();
+    return PA_OK;
+}
+
 template <int TR, int TC>
-void rows_tiles(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
-                int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
-                cudaStream_t s) {
+int rows_tiles(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
+               int n_groups, int d_sum, int d_out, int64_t ldx, int64_t ldo, bool transposed,
+               cudaStream_t s) {
     dim3 grid(static_cast<unsigned>(rows / TR + n_groups + 2),
               static_cast<unsigned>((d_out + TC - 1) / TC));
-    const bool x_vec = vec4(x, ldx), w_vec = vec4(w, transposed ? d_out : d_sum),
-               out_vec = vec4(out, ldo);
+    // tiles that have rows: not more than the rows
+    const int64_t tiles = (rows / TR + (rows < n_groups ? rows : n_groups)) * grid.y;
+    grid.z = TR * TC > 64 * 64 ? 1 : parts_of(tiles, d_sum);
+    const bool x_vec = vec4(x, ldx), w_vec = vec4(w, transposed ? d_out : d_sum);
     if (transposed)
-        rows_kernel<TR, TC, false><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
-                                                        d_out, ldx, ldo, x_vec, w_vec, out_vec);
-    else
-        rows_kernel<TR, TC, true><<<grid, 256, 0, s>>>(out, x, w, offsets, rows, n_groups, d_sum,
-                                                       d_out, ldx, ldo, x_vec, w_vec, out_vec);
+        return launch_tiles(rows_kernel<TR, TC, false>, grid, tile_bytes<TR, TC, true, false>(), s, out,
+                            x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, x_vec, w_vec, vec4(out, ldo));
+    return launch_tiles(rows_kernel<TR, TC, true>, grid, tile_bytes<TR, TC, true, true>(), s, out, x, w,
+                        offsets, rows, n_groups, d_sum, d_out, ldx, ldo, x_vec, w_vec, vec4(out, ldo));
 }
 
 int rows_f32(float *out, const float *x, const float *w, const int64_t *offsets, int64_t rows,
@@ -416,41 +500,36 @@ int rows_f32(float *out, const float *x, const float *w, const int64_t *offsets,
         else
             rows_few_kernel<false><<<grid, 32 * kFewWarps, 0, s>>>(out, x, w, offsets, rows, n_groups,
                                                                    d_sum, d_out, ldx, ldo);
-    } else if (each <= 16) {
-        rows_tiles<16, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
-    } else if (each <= 32) {
-        rows_tiles<32, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
-    } else if (each <= 192 || d_out <= 64 || (rows / 128) * ((d_out + 127) / 128) < 148) {
-        // 128 x 128 needs a tile for every SM and groups that fill it
-        rows_tiles<64, 64>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s);
-    } else {
-        rows_tiles<128, 128>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed,
-                             s);
+        count_launch();
+        PA_CUDA_TRY(cudaGetLastError());
+        return PA_OK;
     }
-    count_launch();
-    PA_CUDA_TRY(cudaGetLastError());
-    return PA_OK;
+#define PA_GO(TR, TC) \
+    return rows_tiles<TR, TC>(out, x, w, offsets, rows, n_groups, d_sum, d_out, ldx, ldo, transposed, s)
+    if (each <= 16) PA_GO(16, 64);
+    if (each <= 32) PA_GO(32, 64);
+    // 128 x 128 needs a tile for every SM and groups that fill it
+    if (each <= 192 || d_out <= 64 || (rows / 128) * ((d_out + 127) / 128) < 148) PA_GO(64, 64);
+    PA_GO(128, 128);
+#undef PA_GO
 }
 
 template <int T>
-void matrices_tiles(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
-                    int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
-    dim3 grid(static_cast<unsigned>((d + T - 1) / T), static_cast<unsigned>((d_out + T - 1) / T),
-              static_cast<unsigned>(n_groups));
-    matrices_kernel<T><<<grid, 256, 0, s>>>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx,
-                                            vec4(dy, ldy), vec4(x, ldx), vec4(dw, d));
+int matrices_tiles(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
+                   int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
+    dim3 grid(static_cast<unsigned>((d + T - 1) / T) * n_groups,
+              static_cast<unsigned>((d_out + T - 1) / T));
+    grid.z = T > 64 ? 1 : parts_of(static_cast<int64_t>(grid.x) * grid.y, rows / n_groups);
+    return launch_tiles(matrices_kernel<T>, grid, tile_bytes<T, T, false, false>(), s, dw, dy, x,
+                        offsets, rows, n_groups, d, d_out, ldy, ldx, vec4(dy, ldy), vec4(x, ldx), vec4(dw, d));
 }
 
 int matrices_f32(float *dw, const float *dy, const float *x, const int64_t *offsets, int64_t rows,
                  int n_groups, int d, int d_out, int64_t ldy, int64_t ldx, cudaStream_t s) {
     const int64_t large = static_cast<int64_t>((d + 127) / 128) * ((d_out + 127) / 128) * n_groups;
     if (d > 64 && d_out > 64 && large >= 148)
-        matrices_tiles<128>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
-    else
-        matrices_tiles<64>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
-    count_launch();
-    PA_CUDA_TRY(cudaGetLastError());
-    return PA_OK;
+        return matrices_tiles<128>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
+    return matrices_tiles<64>(dw, dy, x, offsets, rows, n_groups, d, d_out, ldy, ldx, s);
 }
 
 int check(int64_t rows, int n_groups, int d, int d_out, int dtype) {
