@@ -40,16 +40,6 @@ __host__ __device__ constexpr int smem_bytes(int bn) {
 }
 }  // namespace mma
 
-struct Shape {
-    int rows, n_groups;
-    int m_size;       // of D: contiguous axis
-    int c_size;       // MATRICES: rows of one matrix
-    int t_size;       // FORWARD, ROWS: summed axis
-    int unit;         // tiles a CTA takes at a time
-    int64_t ldo;
-    int piece;        // bytes that result rows are stored in
-};
-
 template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(mma::THREADS, 1)
 mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
@@ -333,14 +323,16 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
     int rc = map_matrices<T>(&a, w, fwd ? d_sum : d_out, fwd ? d_out : d_sum, n_groups,
                              ldw, fwd ? 128 : 64);
     if (rc != PA_OK) return rc;
-    rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN);
+    rc = map_rows<T>(&tail, in, d_sum, rows, ldi, BN < 64 ? BN : 64);
     if (rc != PA_OK) return rc;
-    tail = b;
-    if (BN > 64 && (rc = map_rows<T>(&tail, in, d_sum, rows, ldi, 64)) != PA_OK) return rc;
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
     const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum,
                    tiles_per_unit(most, (d_sum + mma::BK - 1) / mma::BK), ldo,
                    epilogue::piece_of(out, ldo, d_out)};
+    if (BN == 256 && d_out > 128)  // pairs of CTAs have 256 neighbours of a result row
+        return pair_launch<T, MODE == mma::ROWS>(out, a, tail, offsets, sh, s);
+    b = tail;
+    if (BN > 64 && (rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN)) != PA_OK) return rc;
     return launch<T, MODE, BN>(out, a, b, tail, offsets, sh, most, s);
 }
 

@@ -1,0 +1,278 @@
+// Forward and gradient of the rows of grouped_mma.cu for large groups, by pairs of CTAs: a tile of 256 x
+// 256, 128 lanes of each CTA's TMEM.  Each CTA brings its 128 rows of A and half of B, and one MMA
+// (cta_group::2) reads both halves: 32 KB a slice and CTA instead of 48 for the same products.  What
+// bounds the single CTA is the traffic through shared memory (12 KB written and 12 KB read for
+// products that take 128 cycles, at 128 bytes a cycle), and, in a long step, the power it takes.
+//
+// CTA 0 issues the products and asks for tiles; it hands the answers to CTA 1.  Copies of both arrive
+// on CTA 0's barriers, commits on both CTAs'.  Otherwise as grouped_mma.cu.
+#include "epilogue.cuh"
+#include "grouped.cuh"
+#include "segments.cuh"
+#include "tc05.cuh"
+#include "tmap.cuh"
+
+namespace pa {
+namespace grouped {
+
+namespace pair {
+constexpr int BM = 256, BN = 256, BK = 64;
+constexpr int THREADS = 256, STAGES = 6;
+constexpr int A_BYTES = 128 * BK * 2, B_BYTES = 128 * BK * 2;  // of one CTA
+constexpr int BOX_BYTES = 64 * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SMEM = STAGES * STAGE_BYTES + epilogue::bytes(BN) + 1024;
+constexpr uint32_t COLS = 512;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+}  // namespace pair
+
+template <typename T, bool ROWS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
+pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
+            const __grid_constant__ CUtensorMap map_b, const int64_t *__restrict__ offsets, Shape sh,
+            int *__restrict__ status) {
+    using namespace pair;
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
+        ready_bar, told_bar, quit_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int told_s;  // CTA 1: the answer that CTA 0 got
+    __shared__ volatile int abort_s;
+    __shared__ Segments segs;
+    __shared__ TileRing tiles;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = tc05::cluster_rank();
+    const uint32_t ring = (tc05::smem_u32(dyn_smem) + 1023u) & ~1023u;
+
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&full_bar[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&empty_bar[s]), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&acc_full[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 8);
+        }
+        tc05::mbar_init(tc05::smem_u32(&ready_bar), 1);
+        tc05::mbar_init(tc05::smem_u32(&told_bar), 1);
+        tc05::mbar_init(tc05::smem_u32(&quit_bar), 1);
+        ring_init(tiles, 6);
+        abort_s = 0;
+        tc05::fence_barrier_init();
+        tc05::tma_prefetch_desc(&map_a);
+        tc05::tma_prefetch_desc(&map_b);
+    }
+    if (warp == 0) tc05::tmem_alloc_pair(tc05::smem_u32(&tmem_slot), COLS);
+    segs_make<THREADS>(segs, offsets, sh.n_groups, sh.rows, BN);
+    tc05::fence_before_sync();
+    __syncthreads();
+    tc05::cluster_sync();  // the other CTA's barriers are there
+    tc05::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+
+    const int m_tiles = (sh.m_size + BM - 1) / BM;
+    const int row_tiles = segs.tiles[sh.n_groups + 2];
+    auto make = [&](int index) {
+        Tile r;
+        const int row = index / m_tiles;
+        r.g = kNoTile;
+        if (row >= row_tiles) return r;
+        r.m0 = (index - row * m_tiles) * BM;
+        const int seg = segs_find(segs, sh.n_groups, row);
+        r.g = seg >= 1 && seg <= sh.n_groups ? seg - 1 : -1;
+        r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
+        r.c_end = segs.edge[seg + 1];
+        r.t0 = 0;
+        r.t_end = r.g >= 0 ? sh.t_size : 0;
+        return r;
+    };
+    // columns that are multiplied: half of them from each CTA
+    auto columns = [&](const Tile &tile) { return (min(BN, tile.c_end - tile.c0) + 31) / 32 * 32; };
+
+    if (warp == 0) {
+        const bool leader = tc05::elect_one();
+        uint32_t it = 0;
+        bool ok = true;
+        Tile tile;
+        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            const int half = columns(tile) / 2, boxes = (half + 63) / 64;
+            const int m = tile.m0 + 128 * static_cast<int>(rank);
+            const int c = tile.c0 + half * static_cast<int>(rank);
+            for (int t0 = 0; t0 < tile.t_end; t0 += BK, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES)
+                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
+                                              WAIT_LIMIT);
+                if (!ok) break;
+                const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
+                const uint32_t bar = tc05::map_rank(tc05::smem_u32(&full_bar[s]), 0);
+                if (leader) {
+                    if (rank == 0)
+                        tc05::mbar_expect_tx(tc05::smem_u32(&full_bar[s]),
+                                             2 * (A_BYTES + boxes * BOX_BYTES));
+                    if (ROWS) {
+                        tc05::tma_load_3d_pair(a, &map_a, m, t0, tile.g, bar);
+                        tc05::tma_load_3d_pair(a + A_BYTES / 2, &map_a, m + 64, t0, tile.g, bar);
+                    } else {
+                        tc05::tma_load_3d_pair(a, &map_a, t0, m, tile.g, bar);
+                    }
+                    for (int j = 0; j < boxes; ++j)
+                        tc05::tma_load_2d_pair(b + j * BOX_BYTES, &map_b, t0, c + 64 * j, bar);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) abort_s = 1;
+        if (abort_s && rank == 0) {  // no copy is left in flight behind the pair
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
+                                        WAIT_LIMIT);
+        }
+    } else if (warp == 1) {
+        const bool leader = tc05::elect_one();
+        uint32_t it = 0, acc_it = 0;
+        bool ok = true;
+        const uint64_t desc_a = ROWS ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
+                                     : tc05::smem_desc_sw128(ring);
+        const uint64_t desc_b = tc05::smem_desc_sw128(ring + A_BYTES);
+        Tile tile;
+        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+            if (rank != 0 || tile.g < 0) continue;  // CTA 0 issues for both
+            const int slot = acc_it & 1;
+            if (acc_it >= 2)
+                ok = __all_sync(0xffffffffu,
+                                tc05::mbar_wait_cluster(tc05::smem_u32(&acc_empty[slot]),
+                                                        (acc_it / 2 - 1) & 1, WAIT_LIMIT));
+            const uint32_t d = tmem + slot * BN;
+            const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), ROWS, false, BM, columns(tile));
+            for (int t0 = 0; ok && t0 < tile.t_end; t0 += BK, ++it) {
+                const int s = it % STAGES;
+                ok = __all_sync(0xffffffffu,
+                                tc05::mbar_wait_cluster(tc05::smem_u32(&full_bar[s]),
+                                                        (it / STAGES) & 1, WAIT_LIMIT));
+                if (!ok) break;
+                tc05::fence_after_sync();
+                const uint32_t off = s * (STAGE_BYTES / 16);
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)
+                        tc05::mma_f16_pair(d, desc_a + off + k * (ROWS ? 2048 / 16 : 32 / 16),
+                                           desc_b + off + k * (32 / 16), idesc, t0 > 0 || k > 0);
+                    tc05::mma_commit_pair(tc05::smem_u32(&empty_bar[s]));
+                    if (t0 + BK >= tile.t_end) tc05::mma_commit_pair(tc05::smem_u32(&acc_full[slot]));
+                }
+                __syncwarp();
+            }
+            ++acc_it;
+        }
+        if (!ok) abort_s = 1;
+        if (abort_s && leader && rank == 0) {  // nor does a product read on
+            tc05::mma_commit_pair(tc05::smem_u32(&quit_bar));
+            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
+        }
+    } else if (warp == 2) {
+        if (lane == 0) {
+            const uint32_t ready0 = tc05::map_rank(tc05::smem_u32(&ready_bar), 0),
+                           told1 = tc05::map_rank(tc05::smem_u32(&told_bar), 1),
+                           answer1 = tc05::map_rank(
+                               tc05::smem_u32(const_cast<int *>(&told_s)), 1);
+            auto ask = [&](uint32_t asked) -> int {
+                if (rank == 0) {
+                    int next = ring_ask(tiles, asked);
+                    if (next > 0) next /= 2;  // pairs
+                    // CTA 1 has read the answer before
+                    if (!tc05::mbar_wait_cluster(tc05::smem_u32(&ready_bar), asked & 1, kTileWait))
+                        next = -2;
+                    tc05::store_cluster(answer1, static_cast<uint32_t>(next));
+                    tc05::mbar_arrive_cluster(told1);
+                    return next;
+                }
+                tc05::mbar_arrive_cluster(ready0);
+                if (!tc05::mbar_wait_cluster(tc05::smem_u32(&told_bar), asked & 1, 2 * kTileWait))
+                    return -2;
+                return told_s;
+            };
+            ring_serve(tiles, abort_s, ring_depth((sh.t_size + BK - 1) / BK, STAGES), sh.unit,
+                       static_cast<int>(blockIdx.x / 2), make, ask);
+        }
+    } else if (warp >= 4) {
+        const int w = warp - 4;
+        const uint32_t buf = ring + STAGES * STAGE_BYTES;
+        constexpr int CHUNK = epilogue::cols(BN);
+        uint32_t acc_it = 0, chunk = 0;
+        for (uint32_t n = 0;; ++n) {
+            Tile tile;
+            bool ok = ring_take<true>(tiles, abort_s, n, tile);
+            const bool some = ok && tile.g >= 0;
+            const int slot = acc_it & 1;
+            if (some)
+                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
+                                             WAIT_LIMIT) || (abort_s = 1, false);
+            __syncwarp();
+            if (!epilogue::all_agree(ok)) break;
+            tc05::fence_after_sync();
+            const int live = min(BN, tile.c_end - tile.c0), m0 = tile.m0 + 128 * static_cast<int>(rank);
+            T *dst = out + static_cast<int64_t>(tile.c0) * sh.ldo + m0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
+                epilogue::store_chunk<T, CHUNK, false>(
+                    dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
+                    sh.m_size - m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
+                    {}, {});
+            if (some) {
+                tc05::fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    tc05::mbar_arrive_cluster(tc05::map_rank(tc05::smem_u32(&acc_empty[slot]), 0));
+                ++acc_it;
+            }
+        }
+    }
+    __syncwarp();
+    tc05::fence_before_sync();
+    __syncthreads();
+    tc05::cluster_sync();  // nothing of the other CTA reaches here any more
+    tc05::fence_after_sync();
+    if (tid == 0 && abort_s) atomicExch(status, 1);
+    if (warp == 0) tc05::tmem_dealloc_pair(tmem, COLS);
+}
+
+// maps: boxes of 64 values x 128 (forward) or 64 (ROWS) rows of the matrices, x 64 rows of the operand
+template <typename T, bool ROWS>
+int pair_launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
+                const Shape &shape, cudaStream_t s) {
+    static bool configured[64] = {};
+    int dev = 0;
+    PA_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 64 && !configured[dev]) {
+        PA_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<T, ROWS>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
+        configured[dev] = true;
+    }
+    int *status = const_cast<int *>(gemm_status_address());
+    PA_REQUIRE(status != nullptr, "status word not found");
+    const int64_t most = (static_cast<int64_t>(shape.rows) / pair::BN + shape.n_groups + 2) *
+                         ((shape.m_size + pair::BM - 1) / pair::BM);
+    PA_REQUIRE(most <= 0x3fffffff, "too many rows for one call");
+    Shape sh = shape;
+    sh.unit = tiles_per_unit(2 * most, (sh.t_size + pair::BK - 1) / pair::BK);
+    const unsigned grid = 2 * static_cast<unsigned>((most + sh.unit - 1) / sh.unit);
+    pair_kernel<T, ROWS><<<grid, pair::THREADS, pair::SMEM, s>>>(out, a, b, offsets, sh, status);
+    count_launch();
+    PA_CUDA_TRY(cudaGetLastError());
+    return PA_OK;
+}
+
+template int pair_launch<__half, false>(__half *, const CUtensorMap &, const CUtensorMap &,
+                                        const int64_t *, const Shape &, cudaStream_t);
+template int pair_launch<__half, true>(__half *, const CUtensorMap &, const CUtensorMap &,
+                                       const int64_t *, const Shape &, cudaStream_t);
+template int pair_launch<__nv_bfloat16, false>(__nv_bfloat16 *, const CUtensorMap &,
+                                               const CUtensorMap &, const int64_t *, const Shape &,
+                                               cudaStream_t);
+template int pair_launch<__nv_bfloat16, true>(__nv_bfloat16 *, const CUtensorMap &,
+                                              const CUtensorMap &, const int64_t *, const Shape &,
+                                              cudaStream_t);
+
+}  // namespace grouped
+}  // namespace pa

@@ -4,9 +4,21 @@
 
 #include "grouped.cuh"
 #include "tc05.cuh"
+#include "tmap.cuh"
 
 namespace pa {
 namespace grouped {
+
+// of the tensor-core products
+struct Shape {
+    int rows, n_groups;
+    int m_size;       // of D: contiguous axis
+    int c_size;       // MATRICES: rows of one matrix
+    int t_size;       // FORWARD, ROWS: summed axis
+    int unit;         // tiles a CTA takes at a time
+    int64_t ldo;
+    int piece;        // bytes that result rows are stored in
+};
 
 struct Segments {
     int edge[PA_MAX_GROUPS + 3];   // first row of segment i, ascending
@@ -114,15 +126,41 @@ inline int tiles_per_unit(int64_t tiles, int slices) {
     return unit;
 }
 
-// One thread hands out tiles: make(index) is the tile, or has g == kNoTile for an index that the
-// offsets do not reach.
-template <typename Make>
-__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
-                                           Make make) {
+// Asks for the work of a CTA (or cluster) that has not started: the number of its first CTA, -1 if
+// there is none, -2 if no answer came.
+__device__ __forceinline__ int ring_ask(TileRing &r, uint32_t asked) {
     const uint32_t answer = tc05::smem_u32(&r.answer), bar = tc05::smem_u32(&r.answered);
-    int index = blockIdx.x;
+    tc05::mbar_expect_tx(bar, 16);
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+        "[%0], [%1];" ::"r"(answer), "r"(bar)
+        : "memory");
+    if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) return -2;
+    uint32_t more, next;
+    asm volatile(
+        "{\n"
+        ".reg .b128 h;\n"
+        ".reg .pred p;\n"
+        "ld.shared.b128 h, [%2];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "mov.u32 %1, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n"
+        "}\n"
+        : "=r"(more), "=r"(next)
+        : "r"(answer)
+        : "memory");
+    tc05::fence_proxy_async_smem();  // the answer has been read before the next one is written
+    return more ? static_cast<int>(next) : -1;
+}
+
+// One thread hands out tiles: make(index) is the tile, or has g == kNoTile for an index that the
+// offsets do not reach; ask(n) is the n-th answer.
+template <typename Make, typename Ask>
+__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
+                                           int index, Make make, Ask ask) {
     uint32_t n = 0;
-    for (uint32_t asked = 0;; ++asked) {
+    for (uint32_t asked = 0; !abort_s; ++asked) {
         for (int u = 0; u < unit && !abort_s; ++u) {
             const Tile tile = make(index * unit + u);
             if (tile.g == kNoTile) break;
@@ -137,35 +175,20 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
                 abort_s = 1;
         }
         if (abort_s) break;
-        tc05::mbar_expect_tx(bar, 16);
-        asm volatile(
-            "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
-            "[%0], [%1];" ::"r"(answer), "r"(bar)
-            : "memory");
-        if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) {
-            abort_s = 1;
-            break;
-        }
-        uint32_t more, next;
-        asm volatile(
-            "{\n"
-            ".reg .b128 h;\n"
-            ".reg .pred p;\n"
-            "ld.shared.b128 h, [%2];\n"
-            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
-            "selp.u32 %0, 1, 0, p;\n"
-            "mov.u32 %1, 0;\n"
-            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n"
-            "}\n"
-            : "=r"(more), "=r"(next)
-            : "r"(answer)
-            : "memory");
-        tc05::fence_proxy_async_smem();  // the answer has been read before the next one is written
-        if (!more) break;
-        index = static_cast<int>(next);
+        index = ask(asked);
+        if (index == -2) abort_s = 1;
+        if (index < 0) break;
     }
     r.a[n & 3] = make_int4(kNoTile, 0, 0, 0);
     tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));
+}
+
+// the same for the tiles of CTAs without a cluster
+template <typename Make>
+__device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
+                                           Make make) {
+    ring_serve(r, abort_s, depth, unit, static_cast<int>(blockIdx.x), make,
+               [&](uint32_t asked) { return ring_ask(r, asked); });
 }
 
 // A reader's side: the n-th tile of this CTA.  A thread for itself, or (WARP) a whole warp.
@@ -205,6 +228,11 @@ __device__ __forceinline__ int segs_find(const Segments &s, int n_groups, int ti
     }
     return lo;
 }
+
+// grouped_pair.cu
+template <typename T, bool ROWS>
+int pair_launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
+                const Shape &shape, cudaStream_t s);
 
 }  // namespace grouped
 }  // namespace pa
