@@ -30,7 +30,6 @@ constexpr int BM = 128, BK = 64;
 constexpr int THREADS = 256;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
-enum { FORWARD = 0, ROWS = 1, MATRICES = 2 };
 __host__ __device__ constexpr int b_bytes(int bn) { return bn * BK * 2; }
 __host__ __device__ constexpr int stages(int bn) {
     return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : 10;
@@ -49,7 +48,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     using namespace mma;
     constexpr int STAGES = stages(BN), B_BYTES = b_bytes(BN), STAGE_BYTES = A_BYTES + B_BYTES;
     constexpr int BOX = BN < 64 ? BN : 64, BOX_BYTES = BOX * BK * 2;  // of B
-    constexpr bool A_MN = MODE != FORWARD, B_MN = MODE == MATRICES;
+    constexpr bool A_MN = MODE != kForward, B_MN = MODE == kMatrices;
     constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // TMEM columns: a power of two
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
@@ -86,14 +85,14 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 
     const int m_tiles = (sh.m_size + BM - 1) / BM;
     const int c_tiles = (sh.c_size + BN - 1) / BN;
-    const int row_tiles = MODE == MATRICES ? sh.n_groups * c_tiles : segs.tiles[sh.n_groups + 2];
+    const int row_tiles = MODE == kMatrices ? sh.n_groups * c_tiles : segs.tiles[sh.n_groups + 2];
     auto make = [&](int index) {
         Tile r;
         const int row = index / m_tiles;
         r.g = kNoTile;
         if (row >= row_tiles) return r;
         r.m0 = (index - row * m_tiles) * BM;
-        if (MODE == MATRICES) {
+        if (MODE == kMatrices) {
             r.g = row / c_tiles;
             r.c0 = (row - r.g * c_tiles) * BN;
             r.c_end = sh.c_size;
@@ -127,22 +126,22 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 const uint32_t bar = tc05::smem_u32(&full_bar[s]);
                 if (leader) {
                     tc05::mbar_expect_tx(bar, A_BYTES + boxes * BOX_BYTES);
-                    if (MODE == FORWARD) {
+                    if (MODE == kForward) {
                         tc05::tma_load_3d(a, &map_a, t0, tile.m0, tile.g, bar);
-                    } else if (MODE == ROWS) {
+                    } else if (MODE == kRows) {
                         tc05::tma_load_3d(a, &map_a, tile.m0, t0, tile.g, bar);
                         tc05::tma_load_3d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, tile.g, bar);
                     } else {
                         tc05::tma_load_2d(a, &map_a, tile.m0, t0, bar);
                         tc05::tma_load_2d(a + A_BYTES / 2, &map_a, tile.m0 + 64, t0, bar);
                     }
-                    if (MODE != MATRICES && boxes * BOX == BN) {
+                    if (MODE != kMatrices && boxes * BOX == BN) {
                         tc05::tma_load_2d(b, &map_b, t0, tile.c0, bar);
                     } else {
                         for (int j = 0; j < boxes; ++j)
                             tc05::tma_load_2d(b + j * BOX_BYTES, &map_tail,
-                                              MODE == MATRICES ? tile.c0 + BOX * j : t0,
-                                              MODE == MATRICES ? t0 : tile.c0 + BOX * j, bar);
+                                              MODE == kMatrices ? tile.c0 + BOX * j : t0,
+                                              MODE == kMatrices ? t0 : tile.c0 + BOX * j, bar);
                     }
                 }
                 __syncwarp();
@@ -183,8 +182,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     break;
                 }
                 const uint32_t a = ring + s * STAGE_BYTES, off = s * (STAGE_BYTES / 16);
-                const int live = MODE == MATRICES ? min(BK, tile.t_end - t0) : BK;
-                if (MODE == MATRICES && live % 16 != 0) {
+                const int live = MODE == kMatrices ? min(BK, tile.t_end - t0) : BK;
+                if (MODE == kMatrices && live % 16 != 0) {
                     // rows of the next group up to the end of the last k step: 128 bytes each
                     const int dead = 16 - live % 16;
                     for (int i = lane; i < dead * 8 * (2 + (cols + 63) / 64); i += 32) {
@@ -221,7 +220,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         }
     } else if (warp == 2) {
         if (lane == 0) {
-            const int sum = MODE == MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
+            const int sum = MODE == kMatrices ? sh.rows / sh.n_groups : sh.t_size;  // on average
             ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), sh.unit,
                        make);
         }
@@ -244,7 +243,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             tc05::fence_after_sync();
             const int live = min(BN, tile.c_end - tile.c0);
             const int64_t first =
-                (MODE == MATRICES ? static_cast<int64_t>(tile.g) * sh.c_size : 0) + tile.c0;
+                (MODE == kMatrices ? static_cast<int64_t>(tile.g) * sh.c_size : 0) + tile.c0;
             T *dst = out + first * sh.ldo + tile.m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
@@ -319,7 +318,7 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
                        int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw,
                        int64_t ldo, cudaStream_t s) {
     CUtensorMap a, b, tail;
-    const bool fwd = MODE == mma::FORWARD;
+    const bool fwd = MODE == kForward;
     int rc = map_matrices<T>(&a, w, fwd ? d_sum : d_out, fwd ? d_out : d_sum, n_groups,
                              ldw, fwd ? 128 : 64);
     if (rc != PA_OK) return rc;
@@ -330,7 +329,7 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
                    tiles_per_unit(most, (d_sum + mma::BK - 1) / mma::BK), ldo,
                    epilogue::piece_of(out, ldo, d_out)};
     if (BN == 256 && d_out > 128)  // pairs of CTAs have 256 neighbours of a result row
-        return pair_launch<T, MODE == mma::ROWS>(out, a, tail, offsets, sh, s);
+        return pair_launch<T, MODE>(out, a, tail, offsets, sh, s);
     b = tail;
     if (BN > 64 && (rc = map_rows<T>(&b, in, d_sum, rows, ldi, BN)) != PA_OK) return rc;
     return launch<T, MODE, BN>(out, a, b, tail, offsets, sh, most, s);
@@ -360,9 +359,9 @@ int rows_mma(void *out, const void *in, const void *w, const int64_t *offsets, i
     T *o = static_cast<T *>(out);
     const T *i = static_cast<const T *>(in), *m = static_cast<const T *>(w);
     if (transposed)
-        return rows_mma_mode<T, mma::ROWS>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
+        return rows_mma_mode<T, kRows>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
                                            ldo, s);
-    return rows_mma_mode<T, mma::FORWARD>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
+    return rows_mma_mode<T, kForward>(o, i, m, offsets, rows, n_groups, d_sum, d_out, ldi, ldw,
                                           ldo, s);
 }
 
@@ -381,7 +380,8 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0,
                    tiles_per_unit(most, static_cast<int>((each + mma::BK - 1) / mma::BK)), d,
                    epilogue::piece_of(dw, d, d)};
-    return launch<T, mma::MATRICES, BN>(dw, a, b, b, offsets, sh, most, s);
+    if (BN == 256 && d > 128) return pair_launch<T, kMatrices>(dw, a, b, offsets, sh, s);
+    return launch<T, kMatrices, BN>(dw, a, b, b, offsets, sh, most, s);
 }
 
 template <typename T>

@@ -1,11 +1,14 @@
-// Forward and gradient of the rows of grouped_mma.cu for large groups, by pairs of CTAs: a tile of 256 x
+// The products of grouped_mma.cu for large groups, by pairs of CTAs: a tile of 256 x
 // 256, 128 lanes of each CTA's TMEM.  Each CTA brings its 128 rows of A and half of B, and one MMA
 // (cta_group::2) reads both halves: 32 KB a slice and CTA instead of 48 for the same products.  What
 // bounds the single CTA is the traffic through shared memory (12 KB written and 12 KB read for
 // products that take 128 cycles, at 128 bytes a cycle), and, in a long step, the power it takes.
 //
 // CTA 0 issues the products and asks for tiles; it hands the answers to CTA 1.  Copies of both arrive
-// on CTA 0's barriers, commits on both CTAs'.  Otherwise as grouped_mma.cu.
+// on CTA 0's barriers, commits on both CTAs'.  In the gradient of the matrices the rows behind the end
+// of a group are cleared by the CTA that holds them: in such a last slice, and only there (an
+// arrival that publishes a CTA's stores to the other takes about 1 us), CTA 1's copies arrive on a
+// barrier of its own, and it tells CTA 0 when it has cleared.  Otherwise as grouped_mma.cu.
 #include "epilogue.cuh"
 #include "grouped.cuh"
 #include "segments.cuh"
@@ -26,15 +29,17 @@ constexpr uint32_t COLS = 512;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 }  // namespace pair
 
-template <typename T, bool ROWS>
+template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             const __grid_constant__ CUtensorMap map_b, const int64_t *__restrict__ offsets, Shape sh,
             int *__restrict__ status) {
     using namespace pair;
+    constexpr bool MATRICES = MODE == kMatrices, A_MN = MODE != kForward, B_MN = MATRICES;
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
-        ready_bar, told_bar, quit_bar;
+        ready_bar, told_bar, quit_bar, tail_bar[MATRICES ? STAGES : 1],
+        other_bar[MATRICES ? STAGES : 1];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int told_s;  // CTA 1: the answer that CTA 0 got
     __shared__ volatile int abort_s;
@@ -52,6 +57,10 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         for (int s = 0; s < 2; ++s) {
             tc05::mbar_init(tc05::smem_u32(&acc_full[s]), 1);
             tc05::mbar_init(tc05::smem_u32(&acc_empty[s]), 8);
+        }
+        for (int s = 0; MATRICES && s < STAGES; ++s) {
+            tc05::mbar_init(tc05::smem_u32(&tail_bar[s]), 1);
+            tc05::mbar_init(tc05::smem_u32(&other_bar[s]), 1);
         }
         tc05::mbar_init(tc05::smem_u32(&ready_bar), 1);
         tc05::mbar_init(tc05::smem_u32(&told_bar), 1);
@@ -71,13 +80,22 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     const uint32_t tmem = tmem_slot;
 
     const int m_tiles = (sh.m_size + BM - 1) / BM;
-    const int row_tiles = segs.tiles[sh.n_groups + 2];
+    const int c_tiles = (sh.c_size + BN - 1) / BN;
+    const int row_tiles = MATRICES ? sh.n_groups * c_tiles : segs.tiles[sh.n_groups + 2];
     auto make = [&](int index) {
         Tile r;
         const int row = index / m_tiles;
         r.g = kNoTile;
         if (row >= row_tiles) return r;
         r.m0 = (index - row * m_tiles) * BM;
+        if (MATRICES) {
+            r.g = row / c_tiles;
+            r.c0 = (row - r.g * c_tiles) * BN;
+            r.c_end = sh.c_size;
+            r.t0 = segs.edge[r.g + 1];
+            r.t_end = segs.edge[r.g + 2];
+            return r;
+        }
         const int seg = segs_find(segs, sh.n_groups, row);
         r.g = seg >= 1 && seg <= sh.n_groups ? seg - 1 : -1;
         r.c0 = segs.edge[seg] + (row - segs.tiles[seg]) * BN;
@@ -98,7 +116,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             const int half = columns(tile) / 2, boxes = (half + 63) / 64;
             const int m = tile.m0 + 128 * static_cast<int>(rank);
             const int c = tile.c0 + half * static_cast<int>(rank);
-            for (int t0 = 0; t0 < tile.t_end; t0 += BK, ++it) {
+            for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES)
                     ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
@@ -106,58 +124,110 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 if (!ok) break;
                 const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
                 const uint32_t bar = tc05::map_rank(tc05::smem_u32(&full_bar[s]), 0);
-                if (leader) {
-                    if (rank == 0)
-                        tc05::mbar_expect_tx(tc05::smem_u32(&full_bar[s]),
-                                             2 * (A_BYTES + boxes * BOX_BYTES));
-                    if (ROWS) {
+                const int bytes = A_BYTES + boxes * BOX_BYTES;
+                if (leader && MATRICES && (tile.t_end - t0) % 16 != 0 && tile.t_end - t0 < BK) {
+                    const uint32_t own = tc05::smem_u32(rank == 0 ? &full_bar[s] : &tail_bar[s]);
+                    tc05::mbar_expect_tx(own, bytes);
+                    tc05::tma_load_2d(a, &map_a, m, t0, own);
+                    tc05::tma_load_2d(a + A_BYTES / 2, &map_a, m + 64, t0, own);
+                    for (int j = 0; j < boxes; ++j)
+                        tc05::tma_load_2d(b + j * BOX_BYTES, &map_b, c + 64 * j, t0, own);
+                } else if (leader) {
+                    if (rank == 0) tc05::mbar_expect_tx(tc05::smem_u32(&full_bar[s]), 2 * bytes);
+                    if (MODE == kForward) {
+                        tc05::tma_load_3d_pair(a, &map_a, t0, m, tile.g, bar);
+                    } else if (MODE == kRows) {
                         tc05::tma_load_3d_pair(a, &map_a, m, t0, tile.g, bar);
                         tc05::tma_load_3d_pair(a + A_BYTES / 2, &map_a, m + 64, t0, tile.g, bar);
                     } else {
-                        tc05::tma_load_3d_pair(a, &map_a, t0, m, tile.g, bar);
+                        tc05::tma_load_2d_pair(a, &map_a, m, t0, bar);
+                        tc05::tma_load_2d_pair(a + A_BYTES / 2, &map_a, m + 64, t0, bar);
                     }
                     for (int j = 0; j < boxes; ++j)
-                        tc05::tma_load_2d_pair(b + j * BOX_BYTES, &map_b, t0, c + 64 * j, bar);
+                        tc05::tma_load_2d_pair(b + j * BOX_BYTES, &map_b,
+                                               MATRICES ? c + 64 * j : t0,
+                                               MATRICES ? t0 : c + 64 * j, bar);
                 }
                 __syncwarp();
             }
         }
         if (!ok) abort_s = 1;
-        if (abort_s && rank == 0) {  // no copy is left in flight behind the pair
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+        if (abort_s) {  // no copy is left in flight behind the pair
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; rank == 0 && i < it; ++i)
                 tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
                                         WAIT_LIMIT);
         }
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
         uint32_t it = 0, acc_it = 0;
+        uint32_t tails = 0;  // bit s: phase of stage s's barriers for last slices
         bool ok = true;
-        const uint64_t desc_a = ROWS ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
+        const uint64_t desc_a = A_MN ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
                                      : tc05::smem_desc_sw128(ring);
-        const uint64_t desc_b = tc05::smem_desc_sw128(ring + A_BYTES);
+        const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, BOX_BYTES)
+                                     : tc05::smem_desc_sw128(ring + A_BYTES);
         Tile tile;
         for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
-            if (rank != 0 || tile.g < 0) continue;  // CTA 0 issues for both
+            if (tile.g < 0 || tile.t0 >= tile.t_end) continue;
+            const int boxes = (columns(tile) / 2 + 63) / 64;
+            // clears the rows of the next group up to the end of the last k step: 128 bytes each
+            auto clear = [&](int s, int live) {
+                const int dead = 16 - live % 16;
+                for (int i = lane; i < dead * 8 * (2 + boxes); i += 32) {
+                    const int chunk = i / (dead * 8), rest = i - chunk * dead * 8;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                     ring + s * STAGE_BYTES + chunk * BOX_BYTES + live * 128 + rest * 16),
+                                 "r"(0)
+                                 : "memory");
+                }
+                tc05::fence_proxy_async_smem();
+                __syncwarp();
+            };
+            if (rank != 0) {  // CTA 0 issues for both
+                const int slices = (tile.t_end - tile.t0 + BK - 1) / BK;
+                const int live = tile.t_end - tile.t0 - (slices - 1) * BK;
+                it += slices;
+                if (!MATRICES || live % 16 == 0) continue;
+                const int s = (it - 1) % STAGES;
+                ok = tc05::mbar_wait_warp(tc05::smem_u32(&tail_bar[s]), (tails >> s) & 1, WAIT_LIMIT);
+                tails ^= 1u << s;
+                if (!ok) break;
+                clear(s, live);
+                if (lane == 0)
+                    tc05::mbar_arrive_cluster(tc05::map_rank(tc05::smem_u32(&other_bar[s]), 0));
+                continue;
+            }
             const int slot = acc_it & 1;
             if (acc_it >= 2)
                 ok = __all_sync(0xffffffffu,
                                 tc05::mbar_wait_cluster(tc05::smem_u32(&acc_empty[slot]),
                                                         (acc_it / 2 - 1) & 1, WAIT_LIMIT));
             const uint32_t d = tmem + slot * BN;
-            const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), ROWS, false, BM, columns(tile));
-            for (int t0 = 0; ok && t0 < tile.t_end; t0 += BK, ++it) {
+            const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, columns(tile));
+            for (int t0 = tile.t0; ok && t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
                 ok = __all_sync(0xffffffffu,
                                 tc05::mbar_wait_cluster(tc05::smem_u32(&full_bar[s]),
                                                         (it / STAGES) & 1, WAIT_LIMIT));
                 if (!ok) break;
+                const int live = MATRICES ? min(BK, tile.t_end - t0) : BK;
+                if (MATRICES && live % 16 != 0) {
+                    clear(s, live);
+                    ok = __all_sync(0xffffffffu,
+                                    tc05::mbar_wait_cluster(tc05::smem_u32(&other_bar[s]),
+                                                            (tails >> s) & 1, WAIT_LIMIT));
+                    tails ^= 1u << s;
+                    if (!ok) break;
+                }
                 tc05::fence_after_sync();
                 const uint32_t off = s * (STAGE_BYTES / 16);
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
-                        tc05::mma_f16_pair(d, desc_a + off + k * (ROWS ? 2048 / 16 : 32 / 16),
-                                           desc_b + off + k * (32 / 16), idesc, t0 > 0 || k > 0);
+                        if (16 * k < live)
+                            tc05::mma_f16_pair(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
+                                               desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16), idesc,
+                                               t0 > tile.t0 || k > 0);
                     tc05::mma_commit_pair(tc05::smem_u32(&empty_bar[s]));
                     if (t0 + BK >= tile.t_end) tc05::mma_commit_pair(tc05::smem_u32(&acc_full[slot]));
                 }
@@ -192,7 +262,8 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     return -2;
                 return told_s;
             };
-            ring_serve(tiles, abort_s, ring_depth((sh.t_size + BK - 1) / BK, STAGES), sh.unit,
+            const int sum = MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
+            ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), sh.unit,
                        static_cast<int>(blockIdx.x / 2), make, ask);
         }
     } else if (warp >= 4) {
@@ -203,7 +274,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         for (uint32_t n = 0;; ++n) {
             Tile tile;
             bool ok = ring_take<true>(tiles, abort_s, n, tile);
-            const bool some = ok && tile.g >= 0;
+            const bool some = ok && tile.t0 < tile.t_end;
             const int slot = acc_it & 1;
             if (some)
                 ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
@@ -212,7 +283,9 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
             const int live = min(BN, tile.c_end - tile.c0), m0 = tile.m0 + 128 * static_cast<int>(rank);
-            T *dst = out + static_cast<int64_t>(tile.c0) * sh.ldo + m0;
+            const int64_t first =
+                (MATRICES ? static_cast<int64_t>(tile.g) * sh.c_size : 0) + tile.c0;
+            T *dst = out + first * sh.ldo + m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
                 epilogue::store_chunk<T, CHUNK, false>(
@@ -237,42 +310,47 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     if (warp == 0) tc05::tmem_dealloc_pair(tmem, COLS);
 }
 
-// maps: boxes of 64 values x 128 (forward) or 64 (ROWS) rows of the matrices, x 64 rows of the operand
-template <typename T, bool ROWS>
+// maps: boxes of 64 values x 128 rows of the matrices (forward) or 64 rows (else), x 64 rows of the
+// other operand
+template <typename T, int MODE>
 int pair_launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
                 const Shape &shape, cudaStream_t s) {
     static bool configured[64] = {};
     int dev = 0;
     PA_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 64 && !configured[dev]) {
-        PA_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<T, ROWS>,
+        PA_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<T, MODE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
         configured[dev] = true;
     }
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
-    const int64_t most = (static_cast<int64_t>(shape.rows) / pair::BN + shape.n_groups + 2) *
-                         ((shape.m_size + pair::BM - 1) / pair::BM);
+    const int64_t m_tiles = (shape.m_size + pair::BM - 1) / pair::BM;
+    const int64_t most =
+        m_tiles * (MODE == kMatrices
+                       ? static_cast<int64_t>(shape.n_groups) * ((shape.c_size + pair::BN - 1) / pair::BN)
+                       : static_cast<int64_t>(shape.rows) / pair::BN + shape.n_groups + 2);
     PA_REQUIRE(most <= 0x3fffffff, "too many rows for one call");
     Shape sh = shape;
-    sh.unit = tiles_per_unit(2 * most, (sh.t_size + pair::BK - 1) / pair::BK);
+    const int sum = MODE == kMatrices ? sh.rows / sh.n_groups : sh.t_size;
+    sh.unit = tiles_per_unit(2 * most, (sum + pair::BK - 1) / pair::BK);
     const unsigned grid = 2 * static_cast<unsigned>((most + sh.unit - 1) / sh.unit);
-    pair_kernel<T, ROWS><<<grid, pair::THREADS, pair::SMEM, s>>>(out, a, b, offsets, sh, status);
+    pair_kernel<T, MODE><<<grid, pair::THREADS, pair::SMEM, s>>>(out, a, b, offsets, sh, status);
     count_launch();
     PA_CUDA_TRY(cudaGetLastError());
     return PA_OK;
 }
 
-template int pair_launch<__half, false>(__half *, const CUtensorMap &, const CUtensorMap &,
-                                        const int64_t *, const Shape &, cudaStream_t);
-template int pair_launch<__half, true>(__half *, const CUtensorMap &, const CUtensorMap &,
-                                       const int64_t *, const Shape &, cudaStream_t);
-template int pair_launch<__nv_bfloat16, false>(__nv_bfloat16 *, const CUtensorMap &,
-                                               const CUtensorMap &, const int64_t *, const Shape &,
-                                               cudaStream_t);
-template int pair_launch<__nv_bfloat16, true>(__nv_bfloat16 *, const CUtensorMap &,
-                                              const CUtensorMap &, const int64_t *, const Shape &,
-                                              cudaStream_t);
+#define PA_PAIR(T, MODE)                                                                        \
+    template int pair_launch<T, MODE>(T *, const CUtensorMap &, const CUtensorMap &,            \
+                                      const int64_t *, const Shape &, cudaStream_t);
+PA_PAIR(__half, kForward)
+PA_PAIR(__half, kRows)
+PA_PAIR(__half, kMatrices)
+PA_PAIR(__nv_bfloat16, kForward)
+PA_PAIR(__nv_bfloat16, kRows)
+PA_PAIR(__nv_bfloat16, kMatrices)
+#undef PA_PAIR
 
 }  // namespace grouped
 }  // namespace pa

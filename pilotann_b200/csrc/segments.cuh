@@ -9,12 +9,13 @@
 namespace pa {
 namespace grouped {
 
-// of the tensor-core products
+// the tensor-core products: y, dx, dw
+enum { kForward = 0, kRows = 1, kMatrices = 2 };
 struct Shape {
     int rows, n_groups;
     int m_size;       // of D: contiguous axis
-    int c_size;       // MATRICES: rows of one matrix
-    int t_size;       // FORWARD, ROWS: summed axis
+    int c_size;       // kMatrices: rows of one matrix
+    int t_size;       // kForward, kRows: summed axis
     int unit;         // tiles a CTA takes at a time
     int64_t ldo;
     int piece;        // bytes that result rows are stored in
@@ -230,7 +231,7 @@ __device__ __forceinline__ int segs_find(const Segments &s, int n_groups, int ti
 }
 
 // grouped_pair.cu
-template <typename T, bool ROWS>
+template <typename T, int MODE>
 int pair_launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_t *offsets,
                 const Shape &shape, cudaStream_t s);
 
