@@ -339,15 +339,20 @@ template <typename T, int MODE>
 static int rows_mma_mode(T *out, const T *in, const T *w, const int64_t *offsets, int64_t rows,
                          int n_groups, int d_sum, int d_out, int64_t ldi, int64_t ldw,
                          int64_t ldo, cudaStream_t s) {
-    const int64_t each = (rows + n_groups - 1) / n_groups;  // on average
-#define PA_GO(BN) \
-    return rows_mma_bn<T, MODE, BN>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldw, ldo, \
-                                   s)
-    if (each <= 16) PA_GO(16);
-    if (each <= 32) PA_GO(32);
-    if (each <= 64) PA_GO(64);
-    if (each <= 128) PA_GO(128);
+    // columns that a group fills on average, fewer where that leaves SMs without a tile
+    const int64_t each = (rows + n_groups - 1) / n_groups;
+    const int64_t m_tiles = (d_out + mma::BM - 1) / mma::BM, some = rows < n_groups ? rows : n_groups;
+    int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
+    while (bn > 32 && (rows / bn + some) * m_tiles < 148) bn /= 2;
+#define PA_GO(BN)                                                                             \
+    if (bn == BN)                                                                             \
+    return rows_mma_bn<T, MODE, BN>(out, in, w, offsets, rows, n_groups, d_sum, d_out, ldi, ldw, ldo, s)
+    PA_GO(16);
+    PA_GO(32);
+    PA_GO(64);
+    PA_GO(128);
     PA_GO(256);
+    return fail(PA_ERR_ARG, "no tile of %d columns", bn);
 #undef PA_GO
 }
 
