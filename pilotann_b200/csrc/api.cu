@@ -28,7 +28,7 @@ void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 }  // namespace pa
 
-// 104: refinement with the result list and wide CTAs, eight-warp traversal, chunks taken together
-extern "C" int pa_version(void) { return 104; }
+// 105: products of grouped rows, 4-bit tables
+extern "C" int pa_version(void) { return 105; }
 extern "C" const char *pa_last_error(void) { return pa::g_error; }
 extern "C" int64_t pa_launch_count(void) { return pa::g_launches.load(std::memory_order_relaxed); }

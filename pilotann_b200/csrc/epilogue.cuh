@@ -45,6 +45,15 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return r;
 }
 
+// v a b, without an overflow or underflow of a b that v would have undone
+__device__ __forceinline__ float by_both(float v, float a, float b) {
+    const float p = a * b;
+    return p >= 1.1754944e-38f && p <= 3.4028235e38f ? v * p : (v * a) * b;
+}
+
+// two of these multiply to a normal number (it costs a quarter of the stores to look at each product)
+__device__ __forceinline__ bool in_middle(float a) { return a >= 1.0842022e-19f && a <= 9.223372e18f; }
+
 // Bytes that result rows of `width` 16-bit values can be stored in: all rows start on as many, and are
 // whole pieces.
 inline int piece_of(const void *out, int64_t ld, int64_t width) {
@@ -82,10 +91,11 @@ __device__ __forceinline__ void store_rows(T *dst, int64_t ld, uint32_t buf, int
 
 // One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (`some` false: zeros instead), the
 // first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).  `m_left`: lanes that exist.
-// If SCALED, element (m, c) is multiplied by m_scale[i] c_scale[j] before it is rounded: i counts
+// With SCALES, element (m, c) is multiplied by m_scale[i] c_scale[j] before it is rounded (1: scales
+// that are in_middle, 2: any): i counts
 // the four lanes 32 w + 8 i + lane / 4 of this thread, j its columns 8 (j / 2) + 2 (lane % 4) + j % 2.
 // All 128 threads.
-template <typename T, int COLS, bool SCALED>
+template <typename T, int COLS, int SCALES>
 __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, bool some, int live,
                                             int m_left, int piece, uint32_t buf, int w, int lane,
                                             const float (&m_scale)[4],
@@ -105,20 +115,23 @@ __device__ __forceinline__ void store_chunk(T *dst, int64_t ld, uint32_t tmem, b
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) r[half][j] = 0;
     }
+    auto round = [&](auto scaled) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < COLS / 8; ++i)
+            for (int i = 0; i < COLS / 8; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float lo = __uint_as_float(r[half][4 * i + 2 * h]),
-                      hi = __uint_as_float(r[half][4 * i + 2 * h + 1]);
-                if (SCALED) {
-                    lo *= m_scale[2 * half + h] * c_scale[2 * i];
-                    hi *= m_scale[2 * half + h] * c_scale[2 * i + 1];
-                }
-                p[half][i][h] = pack2<T>(lo, hi);
-            }
+                for (int h = 0; h < 2; ++h)
+                    p[half][i][h] = pack2<T>(
+                        scaled(__uint_as_float(r[half][4 * i + 2 * h]), 2 * half + h, 2 * i),
+                        scaled(__uint_as_float(r[half][4 * i + 2 * h + 1]), 2 * half + h, 2 * i + 1));
+    };
+    if constexpr (SCALES == 0)
+        round([](float v, int, int) { return v; });
+    else if constexpr (SCALES == 1)
+        round([&](float v, int m, int c) { return v * (m_scale[m] * c_scale[c]); });
+    else
+        round([&](float v, int m, int c) { return by_both(v, m_scale[m], c_scale[c]); });
     // lane l names row l % 8 of matrix l / 8: column block l / 16, rows 8 (l / 8 % 2) on
     const uint32_t row = buf + (8 * (lane / 16) + lane % 8) * kPitch + (32 * w + 8 * (lane / 8 % 2)) * 2;
 #pragma unroll

@@ -13,6 +13,8 @@
 // quarter, take them to TMEM.  (tcgen05.cp from the issuing thread does the same, but each one, four
 // columns, kept the thread and the products behind it for 160 cycles: 12 of them on 8 products, which
 // take 96 each.  16384 x 4096 against 8192 rows took 458 us that way.)  nvfp4's row scales, powers of two, multiply the finished sum.
+#include <type_traits>
+
 #include "epilogue.cuh"
 #include "fp4.cuh"
 #include "grouped.cuh"
@@ -296,7 +298,9 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         bool ok = true;
         for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0) continue;
-            float t_row = 0.0f, q_row[NB] = {};
+            float t_row = 1.0f, q_row[NB];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) q_row[j] = 1.0f;
             if (METHOD == PA_NVFP4) {  // on their way while the first scales are written
                 if (tile.m0 + own < args.d_out)
                     t_row = __ldg(args.t_row_scale + tile.g * args.d_out + tile.m0 + own);
@@ -487,7 +491,8 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     if (METHOD == PA_NVFP4 && some) {
 #pragma unroll
                         for (int j = 0; j < CHUNK; ++j)
-                            r[j] = __float_as_uint(__uint_as_float(r[j]) * (mine * qs[c0 + j]));
+                            r[j] = __float_as_uint(epilogue::by_both(__uint_as_float(r[j]), mine,
+                                                                     qs[c0 + j]));
                     }
                     if (own < m_left) {
                         if (c0 + CHUNK <= live) {
@@ -502,24 +507,37 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                     }
                 }
             } else {
-                constexpr bool SCALED = METHOD == PA_NVFP4;  // zeros by zeros where there is no group
                 float m_scale[4] = {}, c_scale[CHUNK / 4] = {};
-                if (SCALED && some)
+                bool near = true;  // scales of this tile whose products need no second look
+                if (METHOD == PA_NVFP4 && some) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) m_scale[i] = ts[32 * w + 8 * i + lane / 4];
-                auto store = [&](auto *out) {
+                    near = epilogue::in_middle(ts[own]);
+                    for (int c = own; c < BN; c += 128) near = near && epilogue::in_middle(qs[c]);
+                    near = epilogue::all_agree(near);
+                }
+                auto store_scaled = [&](auto *out, auto scales) {
                     using O = typename std::remove_pointer<decltype(out)>::type;
+                    constexpr int SCALES = decltype(scales)::value;
 #pragma unroll 1
                     for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk) {
-                        if (SCALED && some)
+                        if (SCALES != 0 && some)
 #pragma unroll
                             for (int j = 0; j < CHUNK / 4; ++j)
                                 c_scale[j] = qs[c0 + 8 * (j / 2) + 2 * (lane % 4) + j % 2];
-                        epilogue::store_chunk<O, CHUNK, SCALED>(
+                        epilogue::store_chunk<O, CHUNK, SCALES>(
                             out + first + c0 * args.d_out, args.d_out, from + c0, some, live - c0,
                             m_left, args.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
                             m_scale, c_scale);
                     }
+                };
+                auto store = [&](auto *out) {
+                    if constexpr (METHOD == PA_MXFP4)
+                        store_scaled(out, std::integral_constant<int, 0>());
+                    else if (near)
+                        store_scaled(out, std::integral_constant<int, 1>());
+                    else
+                        store_scaled(out, std::integral_constant<int, 2>());
                 };
                 if (args.out_dtype == PA_BF16) store(static_cast<__nv_bfloat16 *>(args.out));
                 else store(static_cast<__half *>(args.out));
@@ -572,7 +590,7 @@ static int project_bn(Args args, const uint8_t *q_codes, const uint8_t *t_codes,
         return rc;
     const int64_t most = (static_cast<int64_t>(args.rows) / BN + args.n_groups + 2) *
                          ((args.d_out + mma::BM - 1) / mma::BM);
-    PA_REQUIRE(most <= 0x7fffffff, "too many rows for one call");
+    PA_REQUIRE(most <= 0x7fff0000, "too many rows for one call");
     args.unit = grouped::tiles_per_unit(most, (args.values + mma::BK - 1) / mma::BK);
     const unsigned grid = static_cast<unsigned>((most + args.unit - 1) / args.unit);
     project_kernel<METHOD, BN><<<grid, mma::threads(BN), mma::smem_bytes(BN), s>>>(map_t, map_q, tail,

@@ -247,7 +247,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             T *dst = out + first * sh.ldo + tile.m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
-                epilogue::store_chunk<T, CHUNK, false>(
+                epilogue::store_chunk<T, CHUNK, 0>(
                     dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
                     sh.m_size - tile.m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
                     lane, {}, {});
@@ -281,7 +281,7 @@ int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap
     }
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
-    PA_REQUIRE(most_tiles <= 0x7fffffff, "too many rows for one call");
+    PA_REQUIRE(most_tiles <= 0x7fff0000, "too many rows for one call");
     const unsigned grid = static_cast<unsigned>((most_tiles + sh.unit - 1) / sh.unit);
     mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, tail, offsets, sh,
                                                                             status);

@@ -288,7 +288,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             T *dst = out + first * sh.ldo + m0;
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
-                epilogue::store_chunk<T, CHUNK, false>(
+                epilogue::store_chunk<T, CHUNK, 0>(
                     dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
                     sh.m_size - m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
                     {}, {});

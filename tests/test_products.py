@@ -203,6 +203,64 @@ def test_grouped_products_and_gradients(dtype, groups, d, d_out):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("counts,d,d_out", [
+    ([1000, 0, 1, 3000, 257, 742], 512, 640),       # tiles of 256 x 256, many a CTA
+    ([2500, 77, 2423], 320, 1100),                  # both sides ragged
+    ([i % 3 for i in range(1024)], 72, 136),        # the most groups
+    ([0] * 1023 + [40], 264, 72),
+    ([20000], 24, 72),                              # a long sum, few tiles
+    ([5], 4096, 24),
+])
+def test_large_grouped_products(dtype, counts, d, d_out):
+    """Kernels for large groups, the largest number of groups and long sums; twice, with the same
+    bits."""
+    e, offsets = ext(), offsets_of(counts)
+    rows, n = sum(counts), len(counts)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.randn(rows, d, generator=g, device="cuda").to(dtype)
+    w = torch.randn(n, d_out, d, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(rows, d_out, generator=g, device="cuda").to(dtype)
+    want, size = grouped_plain(x, w, dy, offsets)
+    offsets = offsets.cuda()
+    y = e.project_grouped(x, w, offsets)
+    dx, dw = e.project_grouped_backward(dy, x, w, offsets)
+    for got, n_sum, i in ((y, d, 0), (dx, d_out, 1), (dw, max(counts), 2)):
+        assert off_by(got, want[i], size[i], n_sum) <= 0
+    again = e.project_grouped_backward(dy, x, w, offsets)
+    assert torch.equal(e.project_grouped(x, w, offsets), y)
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+
+
+@pytest.mark.gpu
+def test_fp32_sums_stay_exact_over_long_axes():
+    """65536 rows in one sum: the error of a sum kept in levels of 256 terms is that of about
+    2 * 16 roundings of random sign, 2^-24 each, of the size of the result (a single running sum
+    has 256 of them)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(65536, 40, generator=g, device="cuda")
+    dy = torch.randn(65536, 48, generator=g, device="cuda")
+    w = torch.zeros(1, 48, 40, device="cuda")
+    _, dw = ext().project_grouped_backward(dy, x, w, torch.tensor([0, 65536], device="cuda"),
+                                           want_query=False)
+    want = dy.double().T @ x.double()
+    assert (dw[0].double() - want).norm() / want.norm() < 32 * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("want", [(True, False), (False, True)])
+def test_gradient_of_one_side(want):
+    x = torch.randn(40, 64, device="cuda", dtype=BF16, requires_grad=want[0])
+    w = torch.randn(2, 32, 64, device="cuda", dtype=BF16, requires_grad=want[1])
+    offsets = torch.tensor([0, 20, 40], device="cuda")
+    dy = torch.randn(40, 32, device="cuda", dtype=BF16)
+    ext().project_grouped(x, w, offsets).backward(dy)
+    both = ext().project_grouped_backward(dy, x.detach(), w.detach(), offsets)
+    assert (x.grad is None) != want[0] and (w.grad is None) != want[1]
+    assert torch.equal(x.grad if want[0] else w.grad, both[0 if want[0] else 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shift", [0, 1, 8])
 def test_rows_of_wider_tensors(dtype, shift):
     """Rows start anywhere in wider ones: row strides and alignments other than the row's own."""
@@ -497,6 +555,68 @@ def test_fp4_scores_by_group(method, groups, d, d_out):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("method", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("up_q,up_t", [(40, 40), (-40, -40), (90, -90), (-100, 100), (0, -110)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_fp4_scores_of_large_and_small_values(method, up_q, up_t, out):
+    """Scales far from one, on both sides: what one side's scale takes away the other gives back."""
+    e = ext()
+    g = torch.Generator().manual_seed(12)
+    q = (torch.randn(33, 160, generator=g) * 2.0 ** up_q).cuda()
+    t = (torch.randn(200, 160, generator=g) * 2.0 ** up_t).cuda()
+    q[3], t[5] = 0.0, 0.0
+    codes, table = e.quantize_fp4(q, method), e.quantize_fp4(t, method)
+    a, b = e.dequantize_fp4(codes).double(), e.dequantize_fp4(table).double()
+    got = e.project_fp4(codes, table, dtype=out)
+    assert off_by(got, a @ b.T, a.abs() @ b.abs().T, 160) <= 0
+
+
+@pytest.mark.gpu
+def test_fp4_scores_of_extreme_row_scales():
+    """Row scales whose product leaves fp32's range: zeros stay zeros, the rest is what it is."""
+    e = ext()
+    q = torch.full((3, 32), 2.0 ** 120, device="cuda")
+    q[1] = 0.0
+    q[2] = 2.0 ** -120
+    t = torch.full((2, 32), 2.0 ** 120, device="cuda")
+    t[1] = 2.0 ** -120
+    got = e.project_fp4(e.quantize_fp4(q, "nvfp4"), e.quantize_fp4(t, "nvfp4"))
+    want = torch.tensor([[float("inf"), 32.0], [0.0, 0.0], [32.0, 0.0]])
+    # 2^120 and 2^-120 are not 6 times an E4M3 number: half a step of each side's scale and code
+    assert torch.equal(got.isinf().cpu(), want.isinf())
+    assert torch.allclose(got.cpu()[1:], want[1:], rtol=0.25) and torch.allclose(got[0, 1].cpu(), want[0, 1], rtol=0.25)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("method", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rows,d,d_out", [(5000, 544, 3000), (2, 2080, 40000), (1, 65536, 40),
+                                          (700, 512, 17)])
+def test_large_fp4_scores(method, rows, d, d_out):
+    """Many tiles a CTA, in units of several, and the longest rows."""
+    e = ext()
+    g = torch.Generator(device="cuda").manual_seed(d)
+    codes = e.quantize_fp4(torch.randn(rows, d, generator=g, device="cuda").to(BF16), method)
+    table = e.quantize_fp4(torch.randn(d_out, d, generator=g, device="cuda"), method)
+    a, b = e.dequantize_fp4(codes).double(), e.dequantize_fp4(table).double()
+    got = e.project_fp4(codes, table, dtype=BF16)
+    assert off_by(got, a @ b.T, a.abs() @ b.abs().T, d) <= 0
+    assert torch.equal(e.project_fp4(codes, table, dtype=BF16), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("method", ["mxfp4", "nvfp4"])
+def test_fp4_scores_of_the_most_groups(method):
+    e = ext()
+    counts = [i % 3 for i in range(1024)]
+    offsets, rows = offsets_of(counts), sum(counts)
+    q = torch.randn(rows, 96, device="cuda")
+    table = e.quantize_fp4(torch.randn(1024, 40, 96, device="cuda"), method)
+    a, b = e.dequantize_fp4(e.quantize_fp4(q, method)), e.dequantize_fp4(table)
+    want, size = grouped_plain(a, b, torch.zeros(rows, 40, device="cuda"), offsets)
+    assert off_by(e.project_fp4(q, table, offsets.cuda()), want[0], size[0], 96) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("method", ["mxfp4", "nvfp4"])
 def test_fp4_scores_of_nan_rows(method):
     """A NaN in a query or a table row makes its own scores NaN and no others."""
     e = ext()
@@ -635,6 +755,38 @@ assert len(got) == 2, got
 want = e.project_grouped_backward(dy, x, w, o)
 assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1])
 assert torch.equal(got[1], e.project_fp4(x, t, o))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_first_calls_in_a_capture():
+    """Nothing has to have run before a stream capture: a fresh process captures its first calls."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from pilotann_b200 import extension as e
+ids = torch.randint(4, (20000,), device="cuda")
+x = torch.randn(1500, 320, device="cuda").bfloat16()
+w = torch.randn(3, 304, 320, device="cuda").bfloat16()
+xf, wf = x.float(), w.float()
+xo, wo = x[:, :319].contiguous(), w[:, :, :319].contiguous()
+o = torch.tensor([0, 700, 700, 1500], device="cuda")
+dy = torch.randn(1500, 304, device="cuda").bfloat16()
+torch.cuda.synchronize()
+def step():
+    t = e.quantize_fp4(w, "nvfp4")
+    return [*e.group_rows(ids, 4), e.project_grouped(x, w, o), e.project_grouped(xf, wf, o),
+            e.project_grouped(xo, wo, o), *e.project_grouped_backward(dy, x, w, o),
+            e.project_fp4(x, t, o, dtype=torch.bfloat16), e.dequantize_fp4(t)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    held = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, step()))
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
