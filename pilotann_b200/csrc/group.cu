@@ -7,7 +7,7 @@
 // (rows of earlier groups) + (earlier blocks) + (earlier warps) + (earlier rows of the warp):
 // no counter is ever shared between rows whose order matters, and the result does not depend
 // on timing.  Up to kSingleRows rows: one launch of one CTA, bound by its latency (1024 ids, 64
-// groups: 4 us on the GPU, less than the call).  More: a histogram per block; the places of the
+// groups: 5 us on the GPU, less than the call).  More: a histogram per block; the places of the
 // blocks within each group, 32 groups a CTA, and the groups' sums; the pass that writes.
 // The passes read 8 bytes a row twice, the second time from L2, and write 8.
 #include "pa_common.cuh"
@@ -43,26 +43,28 @@ group_count_kernel(int32_t *__restrict__ block_counts, unsigned *__restrict__ do
         block_counts[blockIdx.x * static_cast<int64_t>(bins) + g] = count_s[g];
 }
 
-// exclusive prefix of v over the CTA's threads (all call it); *total receives the sum
-__device__ __forceinline__ int64_t cta_exclusive(int64_t v, int64_t *warp_sum_s, int64_t *total) {
+// exclusive prefix of v over the CTA's threads (all call it); *total receives the sum (32 bits: rows
+// < 2^31)
+__device__ __forceinline__ int32_t cta_exclusive(int32_t v, int32_t *warp_sum_s, int32_t *total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    int64_t x = v;
+    int32_t x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const int32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) warp_sum_s[w] = x;
     __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int i = 0; i < warps; ++i) {
-        const int64_t s = warp_sum_s[i];
-        if (i < w) before += s;
-        all += s;
+    int32_t sums = lane < warps ? warp_sum_s[lane] : 0;  // every warp adds them up for itself
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int32_t y = __shfl_up_sync(0xffffffffu, sums, o);
+        if (lane >= o) sums += y;
     }
+    *total = __shfl_sync(0xffffffffu, sums, 31);
+    const int32_t before = __shfl_sync(0xffffffffu, sums, w == 0 ? 0 : w - 1);
     __syncthreads();
-    *total = all;
-    return before + x - v;
+    return (w == 0 ? 0 : before) + x - v;
 }
 
 // Histograms of the blocks -> places of the blocks within their group; sums of the groups.  A lane
@@ -106,7 +108,7 @@ group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ totals, u
     }
     if (w == 0 && g < bins) totals[g] = carry;
     __shared__ bool last_s;
-    __shared__ int64_t warp_sum_s[32];
+    __shared__ int32_t warp_sum_s[32];
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
@@ -115,11 +117,11 @@ group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ totals, u
     }
     __syncthreads();
     if (!last_s) return;
-    int64_t base = 0;
+    int32_t base = 0;
     for (int g0 = 0; g0 < bins; g0 += 1024) {
         const int i = g0 + threadIdx.x;
-        int64_t total;
-        const int64_t at = cta_exclusive(i < bins ? __ldcg(totals + i) : 0, warp_sum_s, &total) + base;
+        int32_t total;
+        const int32_t at = cta_exclusive(i < bins ? __ldcg(totals + i) : 0, warp_sum_s, &total) + base;
         if (i < bins) offsets[i] = at;  // [n_groups]: where the ungrouped rows start
         base += total;
     }
@@ -133,7 +135,7 @@ group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
                      const int32_t *__restrict__ block_counts, const int64_t *__restrict__ ids,
                      int64_t rows, int n_groups) {
     extern __shared__ int32_t count_s[];  // [WARPS][n_groups + 1]
-    __shared__ int64_t warp_sum_s[32];
+    __shared__ int32_t warp_sum_s[32];
     constexpr int kThreads = 32 * WARPS, kEach = 8;
     const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t lo = (blockIdx.x * static_cast<int64_t>(WARPS) + w) * (32 * kEach) + lane;
@@ -148,26 +150,26 @@ group_scatter_kernel(int64_t *__restrict__ order, int64_t *__restrict__ offsets,
     for (int j = 0; j < kEach; ++j)
         if (g[j] >= 0) atomicAdd(&mine[g[j]], 1);
     __syncthreads();
-    // places: rows of earlier groups and blocks, then of earlier warps (32 bits: rows < 2^31)
-    int64_t base = 0;
+    // places: rows of earlier groups and blocks, then of earlier warps
+    int32_t base = 0;
     for (int g0 = 0; g0 < bins; g0 += kThreads) {
         const int i = g0 + threadIdx.x;
-        int64_t place = 0;
+        int32_t place = 0;
         if (block_counts != nullptr) {
             if (i < bins)
-                place = __ldg(offsets + i) +
+                place = static_cast<int32_t>(__ldg(offsets + i)) +
                         __ldg(block_counts + blockIdx.x * static_cast<int64_t>(bins) + i);
         } else {
             int32_t sum = 0;
             if (i < bins)
                 for (int k = 0; k < WARPS; ++k) sum += count_s[k * bins + i];
-            int64_t total;
+            int32_t total;
             place = cta_exclusive(sum, warp_sum_s, &total) + base;
             base += total;
             if (i < bins) offsets[i] = place;
         }
         if (i < bins) {
-            int32_t at = static_cast<int32_t>(place);
+            int32_t at = place;
 #pragma unroll
             for (int k = 0; k < WARPS; ++k) {
                 const int32_t c = count_s[k * bins + i];
