@@ -287,7 +287,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     } else if (warp == 2) {
         if (lane == 0)
             grouped::ring_serve(tiles, abort_s, grouped::ring_depth(n_stages, STAGES), args.unit,
-                                make);
+                                grouped::ring_ahead(n_stages), make);
     } else if (warp >= 8 && warp < 12) {
         // ---- scales to TMEM: lanes 32 (w % 4) on, for all the products of this CTA ----
         const uint32_t quarter = (32u * (warp & 3)) << 16;

@@ -32,7 +32,7 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_bytes(int bn) { return bn * BK * 2; }
 __host__ __device__ constexpr int stages(int bn) {
-    return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : 10;
+    return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : bn >= 32 ? 9 : 10;
 }
 __host__ __device__ constexpr int smem_bytes(int bn) {
     return stages(bn) * (A_BYTES + b_bytes(bn)) + epilogue::bytes(bn) + 1024;
@@ -78,6 +78,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     }
     if (warp == 0) tc05::tmem_alloc(tc05::smem_u32(&tmem_slot), COLS);
     segs_make<THREADS>(segs, offsets, sh.n_groups, sh.rows, BN);
+    if (MODE == kMatrices) segs_order(segs, sh.n_groups);
     tc05::fence_before_sync();
     __syncthreads();
     tc05::fence_after_sync();
@@ -93,8 +94,9 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         if (row >= row_tiles) return r;
         r.m0 = (index - row * m_tiles) * BM;
         if (MODE == kMatrices) {
-            r.g = row / c_tiles;
-            r.c0 = (row - r.g * c_tiles) * BN;
+            const int nth = row / c_tiles;
+            r.g = segs_group(segs, sh.n_groups, nth);
+            r.c0 = (row - nth * c_tiles) * BN;
             r.c_end = sh.c_size;
             r.t0 = segs.edge[r.g + 1];
             r.t_end = segs.edge[r.g + 2];
@@ -222,7 +224,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         if (lane == 0) {
             const int sum = MODE == kMatrices ? sh.rows / sh.n_groups : sh.t_size;  // on average
             ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), sh.unit,
-                       make);
+                       ring_ahead((sum + BK - 1) / BK), make);
         }
     } else if (warp >= 4) {
         const int w = warp - 4;

@@ -73,6 +73,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     }
     if (warp == 0) tc05::tmem_alloc_pair(tc05::smem_u32(&tmem_slot), COLS);
     segs_make<THREADS>(segs, offsets, sh.n_groups, sh.rows, BN);
+    if (MATRICES) segs_order(segs, sh.n_groups);
     tc05::fence_before_sync();
     __syncthreads();
     tc05::cluster_sync();  // the other CTA's barriers are there
@@ -89,8 +90,9 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         if (row >= row_tiles) return r;
         r.m0 = (index - row * m_tiles) * BM;
         if (MATRICES) {
-            r.g = row / c_tiles;
-            r.c0 = (row - r.g * c_tiles) * BN;
+            const int nth = row / c_tiles;
+            r.g = segs_group(segs, sh.n_groups, nth);
+            r.c0 = (row - nth * c_tiles) * BN;
             r.c_end = sh.c_size;
             r.t0 = segs.edge[r.g + 1];
             r.t_end = segs.edge[r.g + 2];
@@ -264,7 +266,8 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             };
             const int sum = MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
             ring_serve(tiles, abort_s, ring_depth((sum + BK - 1) / BK, STAGES), sh.unit,
-                       static_cast<int>(blockIdx.x / 2), make, ask);
+                       ring_ahead((sum + BK - 1) / BK), static_cast<int>(blockIdx.x / 2), make,
+                       ask);
         }
     } else if (warp >= 4) {
         const int w = warp - 4;

@@ -25,6 +25,7 @@ struct Segments {
     int edge[PA_MAX_GROUPS + 3];   // first row of segment i, ascending
     int tiles[PA_MAX_GROUPS + 3];  // row tiles before segment i
     int part[32];                  // of the prefix sums
+    int order[128];                // groups, most rows first
 };
 
 // inclusive prefix over the CTA's threads (all call it): maximum or sum; *all is over all of them
@@ -81,6 +82,27 @@ __device__ __forceinline__ void segs_make(Segments &s, const int64_t *offsets, i
     if (threadIdx.x == 0) s.tiles[segs] = carry;
 }
 
+// Groups by falling number of rows, for up to 128 of them (32 take 0.5 us): where a tile is summed
+// over the rows of its group, the long ones start first and the short ones fill the end (16384 rows in
+// 32 groups, the largest 1351: the SMs were done at 0.78 of the kernel's time on average).  All threads;
+// a barrier is still needed behind it.
+constexpr int kOrdered = 128;
+__device__ __forceinline__ void segs_order(Segments &s, int n_groups) {
+    const int g = threadIdx.x;
+    if (n_groups <= kOrdered && g < n_groups) {
+        const int mine = s.edge[g + 2] - s.edge[g + 1];
+        int before = 0;
+        for (int i = 0; i < n_groups; ++i) {
+            const int other = s.edge[i + 2] - s.edge[i + 1];
+            before += other > mine || (other == mine && i < g);
+        }
+        s.order[before] = g;
+    }
+}
+__device__ __forceinline__ int segs_group(const Segments &s, int n_groups, int i) {
+    return n_groups <= kOrdered ? s.order[i] : i;
+}
+
 // ---- tiles handed out while the kernel runs ----------------------------------------
 // The grid has a CTA per tile that the offsets could make; one CTA fits an SM.  A CTA works on its own
 // tile and then takes over the tile of a CTA that has not started (cluster launch control), until
@@ -118,6 +140,10 @@ __device__ __forceinline__ void ring_init(TileRing &r, int readers) {
     }
     tc05::mbar_init(tc05::smem_u32(&r.answered), 1);
 }
+
+// Whether tiles are so short that the next one is asked for before there is room for it: an answer
+// takes 1 us, 3 in a cluster, a slice about a quarter.
+__device__ __forceinline__ bool ring_ahead(int slices) { return slices <= 16; }
 
 // Tiles that a CTA takes at a time: enough for 16 slices (an answer takes as long as a few), as
 // long as every SM asks eight times.
@@ -159,27 +185,31 @@ __device__ __forceinline__ int ring_ask(TileRing &r, uint32_t asked) {
 // offsets do not reach; ask(n) is the n-th answer.
 template <typename Make, typename Ask>
 __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
-                                           int index, Make make, Ask ask) {
+                                           bool ahead, int index, Make make, Ask ask) {
     uint32_t n = 0;
+    auto room = [&]() {  // for one more: tile n - depth has been taken by all
+        const uint32_t old = n - depth;
+        if (n >= static_cast<uint32_t>(depth) &&
+            !tc05::mbar_wait_bounded(tc05::smem_u32(&r.empty[old & 3]), (old / 4) & 1, kTileWait))
+            abort_s = 1;
+    };
     for (uint32_t asked = 0; !abort_s; ++asked) {
         for (int u = 0; u < unit && !abort_s; ++u) {
             const Tile tile = make(index * unit + u);
             if (tile.g == kNoTile) break;
+            room();
             r.a[n & 3] = make_int4(tile.g, tile.m0, tile.c0, tile.c_end);
             r.b[n & 3] = make_int2(tile.t0, tile.t_end);
             tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));
             ++n;
-            // room for the next one: tile n - depth has been taken by all
-            const uint32_t old = n - depth;
-            if (n >= static_cast<uint32_t>(depth) &&
-                !tc05::mbar_wait_bounded(tc05::smem_u32(&r.empty[old & 3]), (old / 4) & 1, kTileWait))
-                abort_s = 1;
         }
+        if (!ahead) room();
         if (abort_s) break;
         index = ask(asked);
         if (index == -2) abort_s = 1;
         if (index < 0) break;
     }
+    if (ahead && !abort_s) room();
     r.a[n & 3] = make_int4(kNoTile, 0, 0, 0);
     tc05::mbar_arrive(tc05::smem_u32(&r.full[n & 3]));
 }
@@ -187,8 +217,8 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
 // the same for the tiles of CTAs without a cluster
 template <typename Make>
 __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
-                                           Make make) {
-    ring_serve(r, abort_s, depth, unit, static_cast<int>(blockIdx.x), make,
+                                           bool ahead, Make make) {
+    ring_serve(r, abort_s, depth, unit, ahead, static_cast<int>(blockIdx.x), make,
                [&](uint32_t asked) { return ring_ask(r, asked); });
 }
 
