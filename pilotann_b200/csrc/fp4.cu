@@ -300,6 +300,8 @@ extern "C" int pa_quantize_fp4(uint8_t *codes, uint8_t *scales, float *row_scale
     if (rows == 0) return PA_OK;
     PA_REQUIRE(codes && scales && x && (row_scale || method == PA_MXFP4), "null pointer");
     PA_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+    PA_REQUIRE(aligned_to(x, dtype == PA_F32 ? 4 : 2) && aligned_to(row_scale, 4),
+               "x and row_scale must be aligned to their values");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PA_F32)
         return fp4::quantize_launch<float>(codes, scales, row_scale, x, rows, d, ldx, method, s);
@@ -318,6 +320,8 @@ extern "C" int pa_dequantize_fp4(float *out, const uint8_t *codes, const uint8_t
     if (rows == 0) return PA_OK;
     PA_REQUIRE(out && codes && scales && (row_scale || method == PA_MXFP4), "null pointer");
     PA_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+    PA_REQUIRE(aligned_to(out, 4) && aligned_to(row_scale, 4),
+               "out and row_scale must be aligned to their values");
     const unsigned grid = static_cast<unsigned>((rows + fp4::kWarps - 1) / fp4::kWarps);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool vec = aligned16(out) && d % 4 == 0;

@@ -122,6 +122,9 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     constexpr int BUFS = scale_buffers(BN), ALL_COLS = ACC_COLS + BUFS * SCALE_COLS;
     constexpr uint32_t COLS = ALL_COLS <= 256 ? 256 : 512;
     static_assert(ALL_COLS <= 512, "TMEM has 512 columns");
+    static_assert(smem_bytes(BN) + sizeof(Segments) + sizeof(TileRing) + 1024 +
+                          (METHOD == PA_NVFP4 ? 8 * 4 * (BM + BN) : 4 * (BM + BN)) <= 227 * 1024,
+                  "shared memory of an SM");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], sc_full[SCALE_SLOTS],
         sc_empty[SCALE_SLOTS], tm_full[BUFS], tm_empty[BUFS], acc_full[2], acc_empty[2], quit_bar;
@@ -633,6 +636,9 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     PA_REQUIRE(out && query_codes && query_scales && codes && scales, "null pointer");
     PA_REQUIRE(method == PA_MXFP4 || (query_row_scale && row_scale), "nvfp4 needs row scales");
     PA_REQUIRE(aligned16(query_codes) && aligned16(codes), "codes must be 16-byte aligned");
+    PA_REQUIRE(aligned_to(out, out_dtype == PA_F32 ? 4 : 2) && aligned_to(query_row_scale, 4) &&
+                   aligned_to(row_scale, 4),
+               "out and row scales must be aligned to their values");
     int *status = const_cast<int *>(gemm_status_address());
     PA_REQUIRE(status != nullptr, "status word not found");
     const int values = static_cast<int>(fp4::padded(d));

@@ -542,6 +542,11 @@ int check(int64_t rows, int n_groups, int d, int d_out, int dtype) {
     return PA_OK;
 }
 
+bool aligned(int dtype, const void *a, const void *b, const void *c) {
+    const size_t size = dtype == PA_F32 ? 4 : 2;
+    return aligned_to(a, size) && aligned_to(b, size) && aligned_to(c, size);
+}
+
 // forward, or with `transposed` the gradient of the rows, of 16-bit values
 int rows_16(void *out, const void *in, int64_t ldi, const void *w, int64_t ldw,
             const int64_t *offsets, int64_t rows, int n_groups, int d_sum, int d_out, int64_t ldo,
@@ -575,6 +580,7 @@ extern "C" int pa_project_grouped(void *out, const void *query, const void *VT,
     PA_REQUIRE(ld_query >= d && ld_out >= d_out, "row strides must cover the rows");
     if (rows == 0) return PA_OK;
     PA_REQUIRE(out && query && VT && offsets, "null pointer");
+    PA_REQUIRE(grouped::aligned(dtype, out, query, VT), "operands must be aligned to their values");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PA_F32)
         return grouped::rows_f32(static_cast<float *>(out), static_cast<const float *>(query),
@@ -625,6 +631,9 @@ extern "C" int pa_project_grouped_backward(void *grad_query, void *grad_VT, cons
         return PA_OK;
     }
     PA_REQUIRE(grad && offsets && (!grad_query || VT) && (!grad_VT || query), "null pointer");
+    PA_REQUIRE(grouped::aligned(dtype, grad_query, grad_VT, grad) &&
+                   grouped::aligned(dtype, query, VT, nullptr),
+               "operands must be aligned to their values");
     if (dtype == PA_F32) {
         const float *dy = static_cast<const float *>(grad);
         if (grad_query)

@@ -50,6 +50,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     constexpr int BOX = BN < 64 ? BN : 64, BOX_BYTES = BOX * BK * 2;  // of B
     constexpr bool A_MN = MODE != kForward, B_MN = MODE == kMatrices;
     constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // TMEM columns: a power of two
+    static_assert(smem_bytes(BN) + sizeof(Segments) + sizeof(TileRing) + 512 <= 227 * 1024,
+                  "shared memory of an SM");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
         quit_bar;

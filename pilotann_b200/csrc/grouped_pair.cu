@@ -36,6 +36,8 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             int *__restrict__ status) {
     using namespace pair;
     constexpr bool MATRICES = MODE == kMatrices, A_MN = MODE != kForward, B_MN = MATRICES;
+    static_assert(SMEM + sizeof(Segments) + sizeof(TileRing) + 512 <= 227 * 1024,
+                  "shared memory of an SM");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
         ready_bar, told_bar, quit_bar, tail_bar[MATRICES ? STAGES : 1],

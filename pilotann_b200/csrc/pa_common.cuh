@@ -69,6 +69,10 @@ int refine_enqueue(int64_t *out_I, float *out_D, const int64_t *cand_I, const fl
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+inline bool aligned_to(const void *p, size_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
 // ---- constants with search semantics (upstream traverse_cuda.cu:7-15) ----
 constexpr int kBeams = PA_BEAMS;        // BEAM_WIDTH
 constexpr int kTeam = 8;                // TEAM_SIZE: lanes per distance

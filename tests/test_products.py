@@ -59,6 +59,10 @@ def test_c_entry_points_refuse_bad_arguments():
     refused(L.pa_project_fp4(0, 0, 0, 0, 0, 0, 0, 0, 4, 1, 8, 8, 7, 0, 0), b"dtype")
     refused(L.pa_project_fp4(16, 16, 16, 0, 16, 16, 0, 0, 4, 1, 8, 8, 0, 1, 0), b"row scales")
     refused(L.pa_project_grouped(16, 16, 16, 16, 4, 2, 9, 8, 9, 8, 1, 0, 0), b"workspace")
+    refused(L.pa_project_grouped(16, 17, 16, 16, 4, 2, 8, 8, 8, 8, 1, 0, 0), b"aligned")
+    refused(L.pa_project_grouped(18, 16, 16, 16, 4, 2, 8, 8, 8, 8, 0, 0, 0), b"aligned")
+    refused(L.pa_quantize_fp4(16, 16, 16, 18, 4, 8, 8, 0, 0, 0), b"aligned")
+    refused(L.pa_project_fp4(17, 16, 16, 0, 16, 16, 0, 0, 4, 1, 8, 8, 1, 0, 0), b"aligned")
     refused(L.pa_project_grouped_backward(16, 0, 16, 0, 16, 16, 4, 2, 8, 9, 9, 8, 8, 1, 0, 0),
             b"workspace")
     assert L.pa_project_grouped_workspace_bytes(16, 16, 4, 2, 8, 8, 8, 1) == 0
@@ -382,6 +386,38 @@ def test_offsets_that_do_not_ascend_stay_inside(bad, dtype):
     assert (out[:128] == 7).all() and (out[128 + rows:] == 7).all()
     ext().project_grouped_backward(x, x, w, offsets)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_rows(dtype):
+    e = ext()
+    x, w = torch.zeros(0, 72, device="cuda", dtype=dtype), torch.ones(3, 40, 72, device="cuda", dtype=dtype)
+    offsets = torch.zeros(4, dtype=torch.int64, device="cuda")
+    dy = torch.zeros(0, 40, device="cuda", dtype=dtype)
+    assert e.project_grouped(x, w, offsets).shape == (0, 40)
+    dx, dw = e.project_grouped_backward(dy, x, w, offsets)
+    assert dx.shape == (0, 72) and dw.shape == w.shape and not dw.any()
+    for method in ("mxfp4", "nvfp4"):
+        table = e.quantize_fp4(w, method)
+        assert e.project_fp4(x, table, offsets).shape == (0, 40)
+        none = e.quantize_fp4(x, method)
+        assert e.dequantize_fp4(none).shape == (0, 72)
+        assert e.project_fp4(w[0], none).shape == (40, 0)
+
+
+@pytest.mark.gpu
+def test_fp4_scores_past_2_31_elements():
+    """40000 queries against 65536 vectors: offsets into the scores need more than 32 bits."""
+    e = ext()
+    q = torch.randn(40_000, 32, device="cuda", dtype=BF16)
+    table = e.quantize_fp4(torch.randn(65_536, 32, device="cuda"), "nvfp4")
+    codes = e.quantize_fp4(q, "nvfp4")
+    got = e.project_fp4(codes, table, dtype=BF16)
+    a, b = e.dequantize_fp4(codes).double(), e.dequantize_fp4(table).double()
+    for lo in (0, 32_700, 39_900):
+        part = a[lo:lo + 100]
+        assert off_by(got[lo:lo + 100], part @ b.T, part.abs() @ b.abs().T, 32) <= 0
 
 
 @pytest.mark.gpu
