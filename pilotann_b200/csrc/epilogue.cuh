@@ -51,8 +51,10 @@ __device__ __forceinline__ float by_both(float v, float a, float b) {
     return p >= 1.1754944e-38f && p <= 3.4028235e38f ? v * p : (v * a) * b;
 }
 
-// two of these multiply to a normal number (it costs a quarter of the stores to look at each product)
-__device__ __forceinline__ bool in_middle(float a) { return a >= 1.0842022e-19f && a <= 9.223372e18f; }
+// two of these multiply to a normal number (looking at each product costs a quarter of the stores)
+__device__ __forceinline__ bool in_middle(float a) {
+    return a >= 1.0842022e-19f && a <= 9.223372e18f;  // 2^-63, 2^63
+}
 
 // Bytes that result rows of `width` 16-bit values can be stored in: all rows start on as many, and are
 // whole pieces.
@@ -90,7 +92,8 @@ __device__ __forceinline__ void store_rows(T *dst, int64_t ld, uint32_t buf, int
 }
 
 // One chunk: columns [c0, c0 + COLS) of the tile at `tmem` (`some` false: zeros instead), the
-// first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).  `m_left`: lanes that exist.
+// first `live` of them wanted (all of them if it is more).  dst: element (lane 0, column c0).
+// `m_left`: lanes that exist.
 // With SCALES, element (m, c) is multiplied by m_scale[i] c_scale[j] before it is rounded (1: scales
 // that are in_middle, 2: any): i counts
 // the four lanes 32 w + 8 i + lane / 4 of this thread, j its columns 8 (j / 2) + 2 (lane % 4) + j % 2.

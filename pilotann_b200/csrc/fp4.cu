@@ -83,8 +83,8 @@ template <typename T> __device__ __forceinline__ uint32_t top_bits(const Raw<T> 
 // v / step as codes.  fp32 values are divided.  16-bit ones have at most 11 significant bits and
 // step has four, so that a quotient is a border between two codes (a multiple of 1/4) exactly or at
 // least 2^-13 away from it: a product with the reciprocal, off by 2^-22 of its value, is rounded
-// to a multiple of 2^-14 by adding and subtracting 768, which lands on the border in the first case and stays
-// off it in the other, for two instructions a value.  (It loses the sign of what becomes 0.)
+// to a multiple of 2^-14 by adding and subtracting 768, which lands on the border in the first
+// case and stays off it in the other, for two instructions a value.  (It loses the sign of what becomes 0.)
 template <typename T>
 __device__ __forceinline__ uint32_t codes_by(float (&v)[8], float step) {
     if (sizeof(T) == 2 && step >= 1.1754944e-38f) {  // a reciprocal that does not overflow

@@ -9,7 +9,8 @@
 // on timing.  Up to kSingleRows rows: one launch of one CTA, bound by its latency (1024 ids, 64
 // groups: 5 us on the GPU, less than the call).  More: a histogram per block; the places of the
 // blocks within each group, 32 groups a CTA, and the groups' sums; the pass that writes.
-// The passes read 8 bytes a row twice, the second time from L2, and write 8.
+// The passes read 8 bytes a row twice, the second time from L2, and write 8.  1000000 ids, 1024 groups:
+// 26.6 us, 5 + 8 + 13, bound by the chain of the three and by stores of 8 bytes to 1024 places.
 #include "pa_common.cuh"
 
 namespace pa {
@@ -71,8 +72,8 @@ __device__ __forceinline__ int32_t cta_exclusive(int32_t v, int32_t *warp_sum_s,
 // has a group, a warp eight consecutive blocks, so that loads and stores are whole lines.  The CTA that
 // is done last adds up the groups.
 __global__ void __launch_bounds__(1024)
-group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ totals, unsigned *done, int32_t *__restrict__ block_counts, int n_blocks,
-                  int n_groups) {
+group_scan_kernel(int64_t *__restrict__ offsets, int32_t *__restrict__ totals, unsigned *done,
+                  int32_t *__restrict__ block_counts, int n_blocks, int n_groups) {
     __shared__ int32_t part_s[32][33];
     const int bins = n_groups + 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int g = blockIdx.x * 32 + lane;

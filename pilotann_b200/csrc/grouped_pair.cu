@@ -4,6 +4,9 @@
 // bounds the single CTA is the traffic through shared memory (12 KB written and 12 KB read for
 // products that take 128 cycles, at 128 bytes a cycle), and, in a long step, the power it takes.
 //
+// Measured: 65536 rows x 64 matrices of 1792 x 2048 (bf16): 320, 329 and 361 us alone (1500, 1460 and
+// 1330 TFLOP/s), a fifth more in a row, where power bounds them; 369, 369 and 418 by single CTAs.
+//
 // CTA 0 issues the products and asks for tiles; it hands the answers to CTA 1.  Copies of both arrive
 // on CTA 0's barriers, commits on both CTAs'.  In the gradient of the matrices the rows behind the end
 // of a group are cleared by the CTA that holds them: in such a last slice, and only there (an
