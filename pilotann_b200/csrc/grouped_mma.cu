@@ -55,6 +55,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;  // TMEM columns: a power of two
     static_assert(smem_bytes(BN) + sizeof(Segments) + sizeof(TileRing) + 512 <= 227 * 1024,
                   "shared memory of an SM");
+    static_assert(BK == kSlice, "parts of a sum are whole slices");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
         quit_bar;
@@ -162,64 +163,64 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         }
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
-        uint32_t it = 0, acc_it = 0;
+        uint32_t it = 0, slot = 0, phases = 0;  // bit s: of accumulator s
+        bool ok = true;
         // of the first stage; a descriptor counts 16 bytes, so others are sums
         const uint64_t desc_a = A_MN ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
                                      : tc05::smem_desc_sw128(ring);
         const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, 8192)
                                      : tc05::smem_desc_sw128(ring + A_BYTES);
         Tile tile;
-        for (uint32_t n = 0; ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
             if (tile.t0 >= tile.t_end) continue;
-            const int slot = acc_it & 1;
-            if (acc_it >= 2 && !tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[slot]), (acc_it / 2 - 1) & 1,
-                                                     WAIT_LIMIT)) {
-                abort_s = 1;
-                break;
-            }
-            tc05::fence_after_sync();
-            const uint32_t d = tmem + slot * BN;
             const int cols = min(BN, tile.c_end - tile.c0);
             const uint32_t idesc =
                 tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, (cols + 15) / 16 * 16);
-            for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
-                const int s = it % STAGES;
-                if (!tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1, WAIT_LIMIT)) {
-                    abort_s = 1;
-                    break;
-                }
-                const uint32_t a = ring + s * STAGE_BYTES, off = s * (STAGE_BYTES / 16);
-                const int live = MODE == kMatrices ? min(BK, tile.t_end - t0) : BK;
-                if (MODE == kMatrices && live % 16 != 0) {
-                    // rows of the next group up to the end of the last k step: 128 bytes each
-                    const int dead = 16 - live % 16;
-                    for (int i = lane; i < dead * 8 * (2 + (cols + 63) / 64); i += 32) {
-                        const int chunk = i / (dead * 8), rest = i - chunk * dead * 8;
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                         a + chunk * 8192 + live * 128 + rest * 16),
-                                     "r"(0)
-                                     : "memory");
-                    }
-                    tc05::fence_proxy_async_smem();
-                }
-                __syncwarp();
-                tc05::fence_after_sync();
-                if (leader) {
-#pragma unroll
-                    for (int k = 0; k < BK / 16; ++k) {
-                        if (16 * k < live) {
-                            tc05::mma_f16(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
-                                          desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16), idesc,
-                                          t0 > tile.t0 || k > 0);
+            for (int p0 = tile.t0; ok && p0 < tile.t_end; p0 += kPart) {
+                ok = tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[slot]), (phases >> slot & 1) ^ 1,
+                                          WAIT_LIMIT);
+                const uint32_t d = tmem + slot * BN;
+                const int p_end = part_end(p0, tile.t_end);
+                for (int t0 = p0; ok && t0 < p_end; t0 += BK, ++it) {
+                    const int s = it % STAGES;
+                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
+                                              WAIT_LIMIT);
+                    if (!ok) break;
+                    const uint32_t a = ring + s * STAGE_BYTES, off = s * (STAGE_BYTES / 16);
+                    const int live = MODE == kMatrices ? min(BK, p_end - t0) : BK;
+                    if (MODE == kMatrices && live % 16 != 0) {
+                        // rows of the next group up to the end of the last k step: 128 bytes each
+                        const int dead = 16 - live % 16;
+                        for (int i = lane; i < dead * 8 * (2 + (cols + 63) / 64); i += 32) {
+                            const int chunk = i / (dead * 8), rest = i - chunk * dead * 8;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                             a + chunk * 8192 + live * 128 + rest * 16),
+                                         "r"(0)
+                                         : "memory");
                         }
+                        tc05::fence_proxy_async_smem();
                     }
-                    tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
-                    if (t0 + BK >= tile.t_end) tc05::mma_commit(tc05::smem_u32(&acc_full[slot]));
+                    __syncwarp();
+                    tc05::fence_after_sync();
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) {
+                            if (16 * k < live) {
+                                tc05::mma_f16(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
+                                              desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16), idesc,
+                                              t0 > p0 || k > 0);
+                            }
+                        }
+                        tc05::mma_commit(tc05::smem_u32(&empty_bar[s]));
+                        if (t0 + BK >= p_end) tc05::mma_commit(tc05::smem_u32(&acc_full[slot]));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                phases ^= 1u << slot;
+                if (p0 == tile.t0) slot ^= 1;
             }
-            ++acc_it;
         }
+        if (!ok) abort_s = 1;
         __syncwarp();
         if (abort_s && leader) {  // nor does a product read on
             tc05::mma_commit(tc05::smem_u32(&quit_bar));
@@ -235,16 +236,16 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         const int w = warp - 4;
         const uint32_t buf = ring + STAGES * STAGE_BYTES;
         constexpr int CHUNK = epilogue::cols(BN);
-        uint32_t acc_it = 0, chunk = 0;
+        uint32_t slot = 0, phases = 0, chunk = 0;
         for (uint32_t n = 0;; ++n) {
             // the four warps must agree on what they do: they meet at barriers below
             Tile tile;
             bool ok = ring_take<true>(tiles, abort_s, n, tile);
             const bool some = ok && tile.t0 < tile.t_end;
-            const int slot = acc_it & 1;
+            const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)
-                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT) || (abort_s = 1, false);
+                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s,
+                                   [](uint64_t *bar) { tc05::mbar_arrive(tc05::smem_u32(bar)); });
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
@@ -255,14 +256,13 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
                 epilogue::store_chunk<T, CHUNK, 0>(
-                    dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
+                    dst + c0 * sh.ldo, sh.ldo, tmem + sum * BN + c0, some, live - c0,
                     sh.m_size - tile.m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w,
                     lane, {}, {});
             if (some) {
                 tc05::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&acc_empty[slot]));
-                ++acc_it;
+                if (lane == 0) tc05::mbar_arrive(tc05::smem_u32(&acc_empty[sum]));
             }
         }
     }

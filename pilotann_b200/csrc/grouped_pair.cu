@@ -41,6 +41,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     constexpr bool MATRICES = MODE == kMatrices, A_MN = MODE != kForward, B_MN = MATRICES;
     static_assert(SMEM + sizeof(Segments) + sizeof(TileRing) + 512 <= 227 * 1024,
                   "shared memory of an SM");
+    static_assert(BK == kSlice, "parts of a sum are whole slices");
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2],
         ready_bar, told_bar, quit_bar, tail_bar[MATRICES ? STAGES : 1],
@@ -166,7 +167,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         }
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
-        uint32_t it = 0, acc_it = 0;
+        uint32_t it = 0, slot = 0, phases = 0;  // bit s: of accumulator s
         uint32_t tails = 0;  // bit s: phase of stage s's barriers for last slices
         bool ok = true;
         const uint64_t desc_a = A_MN ? tc05::smem_desc_mn_sw128(ring, A_BYTES / 2)
@@ -204,43 +205,45 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     tc05::mbar_arrive_cluster(tc05::map_rank(tc05::smem_u32(&other_bar[s]), 0));
                 continue;
             }
-            const int slot = acc_it & 1;
-            if (acc_it >= 2)
+            const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, columns(tile));
+            for (int p0 = tile.t0; ok && p0 < tile.t_end; p0 += kPart) {
                 ok = __all_sync(0xffffffffu,
                                 tc05::mbar_wait_cluster(tc05::smem_u32(&acc_empty[slot]),
-                                                        (acc_it / 2 - 1) & 1, WAIT_LIMIT));
-            const uint32_t d = tmem + slot * BN;
-            const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, columns(tile));
-            for (int t0 = tile.t0; ok && t0 < tile.t_end; t0 += BK, ++it) {
-                const int s = it % STAGES;
-                ok = __all_sync(0xffffffffu,
-                                tc05::mbar_wait_cluster(tc05::smem_u32(&full_bar[s]),
-                                                        (it / STAGES) & 1, WAIT_LIMIT));
-                if (!ok) break;
-                const int live = MATRICES ? min(BK, tile.t_end - t0) : BK;
-                if (MATRICES && live % 16 != 0) {
-                    clear(s, live);
+                                                        (phases >> slot & 1) ^ 1, WAIT_LIMIT));
+                const uint32_t d = tmem + slot * BN;
+                const int p_end = part_end(p0, tile.t_end);
+                for (int t0 = p0; ok && t0 < p_end; t0 += BK, ++it) {
+                    const int s = it % STAGES;
                     ok = __all_sync(0xffffffffu,
-                                    tc05::mbar_wait_cluster(tc05::smem_u32(&other_bar[s]),
-                                                            (tails >> s) & 1, WAIT_LIMIT));
-                    tails ^= 1u << s;
+                                    tc05::mbar_wait_cluster(tc05::smem_u32(&full_bar[s]),
+                                                            (it / STAGES) & 1, WAIT_LIMIT));
                     if (!ok) break;
-                }
-                tc05::fence_after_sync();
-                const uint32_t off = s * (STAGE_BYTES / 16);
-                if (leader) {
+                    const int live = MATRICES ? min(BK, p_end - t0) : BK;
+                    if (MATRICES && live % 16 != 0) {
+                        clear(s, live);
+                        ok = __all_sync(0xffffffffu,
+                                        tc05::mbar_wait_cluster(tc05::smem_u32(&other_bar[s]),
+                                                                (tails >> s) & 1, WAIT_LIMIT));
+                        tails ^= 1u << s;
+                        if (!ok) break;
+                    }
+                    tc05::fence_after_sync();
+                    const uint32_t off = s * (STAGE_BYTES / 16);
+                    if (leader) {
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        if (16 * k < live)
-                            tc05::mma_f16_pair(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
-                                               desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16), idesc,
-                                               t0 > tile.t0 || k > 0);
-                    tc05::mma_commit_pair(tc05::smem_u32(&empty_bar[s]));
-                    if (t0 + BK >= tile.t_end) tc05::mma_commit_pair(tc05::smem_u32(&acc_full[slot]));
+                        for (int k = 0; k < BK / 16; ++k)
+                            if (16 * k < live)
+                                tc05::mma_f16_pair(d, desc_a + off + k * (A_MN ? 2048 / 16 : 32 / 16),
+                                                   desc_b + off + k * (B_MN ? 2048 / 16 : 32 / 16),
+                                                   idesc, t0 > p0 || k > 0);
+                        tc05::mma_commit_pair(tc05::smem_u32(&empty_bar[s]));
+                        if (t0 + BK >= p_end) tc05::mma_commit_pair(tc05::smem_u32(&acc_full[slot]));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                phases ^= 1u << slot;
+                if (p0 == tile.t0) slot ^= 1;
             }
-            ++acc_it;
         }
         if (!ok) abort_s = 1;
         if (abort_s && leader && rank == 0) {  // nor does a product read on
@@ -278,15 +281,17 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         const int w = warp - 4;
         const uint32_t buf = ring + STAGES * STAGE_BYTES;
         constexpr int CHUNK = epilogue::cols(BN);
-        uint32_t acc_it = 0, chunk = 0;
+        uint32_t slot = 0, phases = 0, chunk = 0;
+        auto emptied = [](uint64_t *bar) {
+            tc05::mbar_arrive_cluster(tc05::map_rank(tc05::smem_u32(bar), 0));
+        };
         for (uint32_t n = 0;; ++n) {
             Tile tile;
             bool ok = ring_take<true>(tiles, abort_s, n, tile);
             const bool some = ok && tile.t0 < tile.t_end;
-            const int slot = acc_it & 1;
+            const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)
-                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[slot]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT) || (abort_s = 1, false);
+                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s, emptied);
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
@@ -297,15 +302,13 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 #pragma unroll 1
             for (int c0 = 0; c0 < live; c0 += CHUNK, ++chunk)
                 epilogue::store_chunk<T, CHUNK, 0>(
-                    dst + c0 * sh.ldo, sh.ldo, tmem + slot * BN + c0, some, live - c0,
+                    dst + c0 * sh.ldo, sh.ldo, tmem + sum * BN + c0, some, live - c0,
                     sh.m_size - m0, sh.piece, buf + (chunk & 1) * CHUNK * epilogue::kPitch, w, lane,
                     {}, {});
             if (some) {
                 tc05::fence_before_sync();
                 __syncwarp();
-                if (lane == 0)
-                    tc05::mbar_arrive_cluster(tc05::map_rank(tc05::smem_u32(&acc_empty[slot]), 0));
-                ++acc_it;
+                if (lane == 0) emptied(&acc_empty[sum]);
             }
         }
     }
