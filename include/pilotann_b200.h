@@ -138,6 +138,11 @@ int pa_device_status(int reset);
  * router exactly.  No upstream counterpart. */
 int pa_selftest_bounded_wait(void *stream);
 
+/* Diagnostic: grouped and 4-bit products launched from now on, by any thread, give up after
+ * `polls` polls of the wait for a finished sum (0: at once; negative: the usual limit again), so
+ * that a test can see a kernel give up with copies and products on their way. */
+int pa_selftest_sum_polls(int polls);
+
 /* ---- visited-set pool -------------------------------------------------------
  * Device counterpart of upstream's `Bitmask` / `BitmaskPool`
  * (extension/inc/bitmask.hpp:12-45, 51-76; used at traverse_cpu.cpp:196-200 and

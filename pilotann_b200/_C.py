@@ -28,6 +28,7 @@ SYMBOLS = (
     "pa_group_rows_workspace_bytes", "pa_group_rows", "pa_project_grouped",
     "pa_project_grouped_backward", "pa_project_grouped_workspace_bytes",
     "pa_project_grouped_backward_workspace_bytes", "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4",
+    "pa_selftest_sum_polls",
 )
 
 PA_OUT_HANDOFF, PA_OUT_STAGE2, PA_OUT_TOPK = 0, 1, 2
@@ -139,8 +140,10 @@ def lib() -> ctypes.CDLL:
     L.pa_dequantize_fp4.argtypes = [P, P, P, P, c_int64, c_int, c_int, P]
     L.pa_project_fp4.argtypes = [P, P, P, P, P, P, P, P, c_int64, c_int, c_int, c_int64, c_int,
                                  c_int, P]
+    L.pa_selftest_sum_polls.argtypes = [c_int]
     for name in ("pa_group_rows", "pa_project_grouped", "pa_project_grouped_backward",
-                 "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4"):
+                 "pa_quantize_fp4", "pa_dequantize_fp4", "pa_project_fp4",
+                 "pa_selftest_sum_polls"):
         getattr(L, name).restype = c_int
     for name in ("pa_traverse_csr", "pa_pack_graph", "pa_traverse_packed", "pa_route",
                  "pa_project", "pa_stage_create", "pa_stage_search", "pa_stage_search_device",

@@ -35,12 +35,13 @@ using grouped::kNoTile;
 using grouped::Segments;
 using grouped::Tile;
 using grouped::TileRing;
+using grouped::wait_unless;
+using grouped::wait_warp;
 
 namespace mma {
 constexpr int BM = 128, BK = 256;        // values; 128 bytes of codes
 constexpr int A_BYTES = BM * BK / 2;
 constexpr int SCALE_SLOTS = 4;
-constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_blocks(int bn) { return bn > 128 ? 2 : 1; }
 // Loader warps of a block of 128 rows of scales: each has a piece of 16 bytes a row on its way,
 // about 1 us from DRAM, while a tile of short rows needs a piece every 0.6 us.
@@ -73,6 +74,7 @@ struct Args {
     int out_dtype;
     int piece;                           // bytes that 16-bit result rows are stored in
     int *status;
+    uint32_t polls;                      // limit of the wait for a sum
 };
 
 // Bytes [at, at + 16) of a row of `pitch` scale bytes, zero behind its end.  Only aligned 16-byte
@@ -194,6 +196,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         return r;
     };
 
+    uint32_t issued = 0;  // slices of codes, by warp 0
     if (warp == 0) {
         // ---- codes ----
         const bool leader = tc05::elect_one();
@@ -206,8 +209,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             for (int k = 0; k < n_stages; ++k, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES)
-                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
-                                              WAIT_LIMIT);
+                    ok = wait_warp(empty_bar[s], (it / STAGES - 1) & 1, abort_s);
                 if (!ok) break;
                 const uint32_t a = ring + s * STAGE_BYTES;
                 const uint32_t bar = tc05::smem_u32(&full_bar[s]);
@@ -226,11 +228,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             }
         }
         if (!ok) abort_s = 1;
-        if (abort_s) {  // no copy is left in flight behind the CTA
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
-                                        WAIT_LIMIT);
-        }
+        issued = it;
     } else if (warp == 1) {
         // ---- products: the warp runs together, one lane issues ----
         const bool leader = tc05::elect_one();
@@ -243,8 +241,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             if (tile.g < 0) continue;
             const int acc = acc_it & 1;
             if (acc_it >= 2)
-                ok = tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[acc]), (acc_it / 2 - 1) & 1,
-                                          WAIT_LIMIT);
+                ok = wait_warp(acc_empty[acc], (acc_it / 2 - 1) & 1, abort_s);
             const uint32_t d = tmem + acc * BN;
             const int cols = min(BN, tile.c_end - tile.c0);
             const uint32_t idesc0 = tc05::idesc_mxf4(METHOD == PA_MXFP4, (cols + 15) / 16 * 16);
@@ -252,13 +249,11 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             for (int k = 0; ok && k < n_stages; ++k, ++it) {
                 const int s = it % STAGES, buf = sg % BUFS;
                 if (k % GROUP == 0) {
-                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&tm_full[buf]), (sg / BUFS) & 1,
-                                              WAIT_LIMIT);
+                    ok = wait_warp(tm_full[buf], (sg / BUFS) & 1, abort_s);
                     sa = tmem + ACC_COLS + buf * SCALE_COLS;
                     sb = sa + 16;
                 }
-                ok = ok && tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
-                                                WAIT_LIMIT);
+                ok = ok && wait_warp(full_bar[s], (it / STAGES) & 1, abort_s);
                 if (!ok) break;
                 tc05::fence_after_sync();
                 const uint64_t a = desc_a + s * (STAGE_BYTES / 16), b = a + A_BYTES / 16;
@@ -288,10 +283,6 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             ++acc_it;
         }
         if (!ok) abort_s = 1;
-        if (abort_s && leader) {  // nor does a product read on
-            tc05::mma_commit(tc05::smem_u32(&quit_bar));
-            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
-        }
     } else if (warp == 2) {
         if (lane == 0)
             grouped::ring_serve(tiles, abort_s, grouped::ring_depth(n_stages, STAGES), args.unit,
@@ -319,9 +310,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             }
             for (int piece = 0; piece < n_pieces; ++piece, ++sg) {
                 const int slot = sg % SCALE_SLOTS, buf = sg % BUFS;
-                ok = __all_sync(0xffffffffu,
-                                tc05::mbar_wait_bounded(tc05::smem_u32(&sc_full[slot]),
-                                                        (sg / SCALE_SLOTS) & 1, WAIT_LIMIT));
+                ok = wait_warp(sc_full[slot], (sg / SCALE_SLOTS) & 1, abort_s);
                 if (!ok) break;
                 uint32_t r[1 + NB][16];
                 const uint32_t from = scale_ring + slot * SLOT_BYTES + 16 * lane;
@@ -335,9 +324,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
                                      : "r"(from + 2048 * j + 512 * w)
                                      : "memory");
                 if (sg >= BUFS)
-                    ok = __all_sync(0xffffffffu,
-                                    tc05::mbar_wait_bounded(tc05::smem_u32(&tm_empty[buf]),
-                                                            (sg / BUFS - 1) & 1, WAIT_LIMIT));
+                    ok = wait_warp(tm_empty[buf], (sg / BUFS - 1) & 1, abort_s);
                 if (!ok) break;
                 tc05::fence_after_sync();
                 const uint32_t to = tmem + ACC_COLS + buf * SCALE_COLS + quarter;
@@ -427,10 +414,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
 #pragma unroll
             for (int b = 0; b < 4; ++b) v[b] = scales_take(next[b], row[b], at, pitch);
             const int slot = sg % SCALE_SLOTS;
-            if (sg >= SCALE_SLOTS &&
-                !__all_sync(0xffffffffu,
-                            tc05::mbar_wait_bounded(tc05::smem_u32(&sc_empty[slot]),
-                                                    (sg / SCALE_SLOTS - 1) & 1, WAIT_LIMIT))) {
+            if (sg >= SCALE_SLOTS && !wait_warp(sc_empty[slot], (sg / SCALE_SLOTS - 1) & 1, abort_s)) {
                 abort_s = 1;
                 break;
             }
@@ -469,11 +453,9 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
             const float *ts = t_scale_s[acc_it % ROW_BUFS], *qs = q_scale_s[acc_it % ROW_BUFS];
             if (METHOD == PA_NVFP4 && some)
-                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&row_full[acc_it % ROW_BUFS]),
-                                             (acc_it / ROW_BUFS) & 1, WAIT_LIMIT) || (abort_s = 1, false);
-            if (some && ok)
-                ok = tc05::mbar_wait_bounded(tc05::smem_u32(&acc_full[acc]), (acc_it / 2) & 1,
-                                             WAIT_LIMIT) || (abort_s = 1, false);
+                ok = wait_unless(row_full[acc_it % ROW_BUFS], (acc_it / ROW_BUFS) & 1, abort_s);
+            if (some && ok) ok = wait_unless(acc_full[acc], (acc_it / 2) & 1, abort_s, args.polls);
+            if (some && !ok) abort_s = 1;
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
@@ -561,7 +543,10 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     __syncwarp();
     tc05::fence_before_sync();
     __syncthreads();
-    if (tid == 0 && abort_s) atomicExch(args.status, 1);
+    if (abort_s) {
+        grouped::wind_down<STAGES>(tiles, full_bar, issued, &quit_bar);
+        if (tid == 0) atomicExch(args.status, 1);
+    }
     if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
 }
 
@@ -650,7 +635,8 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     const int pitch = values / fp4::block_of(method);
     const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,
                          static_cast<int>(rows), n_groups, values, pitch, pitch, 1, out_dtype,
-                         epilogue::piece_of(out, d_out, d_out), status};
+                         epilogue::piece_of(out, d_out, d_out), status,
+                         grouped::sum_polls()};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return method == PA_MXFP4
                ? fp4::project_method<PA_MXFP4>(args, query_codes, codes, s)

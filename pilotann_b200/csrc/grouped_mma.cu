@@ -20,6 +20,8 @@
 // Measured: 128 rows x 64 matrices of 1024 x 2048 (bf16) 44 us, 5.3 TB/s, 81 % of the copy rate: the
 // rest is the start (4 us to the first slice) and SMs that the memory serves later than others.
 // Larger groups: grouped_pair.cu.
+#include <atomic>
+
 #include "epilogue.cuh"
 #include "grouped.cuh"
 #include "segments.cuh"
@@ -33,7 +35,6 @@ namespace mma {
 constexpr int BM = 128, BK = 64;
 constexpr int THREADS = 256;
 constexpr int A_BYTES = BM * BK * 2;
-constexpr uint32_t WAIT_LIMIT = 1u << 22;
 __host__ __device__ constexpr int b_bytes(int bn) { return bn * BK * 2; }
 __host__ __device__ constexpr int stages(int bn) {
     return bn >= 256 ? 4 : bn >= 128 ? 6 : bn >= 64 ? 8 : bn >= 32 ? 9 : 10;
@@ -117,6 +118,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         return r;
     };
 
+    uint32_t issued = 0;  // slices, by warp 0
     if (warp == 0) {
         const bool leader = tc05::elect_one();
         uint32_t it = 0;
@@ -127,8 +129,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES)
-                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
-                                              WAIT_LIMIT);
+                    ok = wait_warp(empty_bar[s], (it / STAGES - 1) & 1, abort_s);
                 if (!ok) break;
                 const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
                 const uint32_t bar = tc05::smem_u32(&full_bar[s]);
@@ -156,11 +157,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
         if (!ok) abort_s = 1;
-        if (abort_s) {  // no copy is left in flight behind the CTA
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
-                                        WAIT_LIMIT);
-        }
+        issued = it;
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
         uint32_t it = 0, slot = 0, phases = 0;  // bit s: of accumulator s
@@ -177,14 +174,12 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             const uint32_t idesc =
                 tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, (cols + 15) / 16 * 16);
             for (int p0 = tile.t0; ok && p0 < tile.t_end; p0 += kPart) {
-                ok = tc05::mbar_wait_warp(tc05::smem_u32(&acc_empty[slot]), (phases >> slot & 1) ^ 1,
-                                          WAIT_LIMIT);
+                ok = wait_warp(acc_empty[slot], (phases >> slot & 1) ^ 1, abort_s);
                 const uint32_t d = tmem + slot * BN;
                 const int p_end = part_end(p0, tile.t_end);
                 for (int t0 = p0; ok && t0 < p_end; t0 += BK, ++it) {
                     const int s = it % STAGES;
-                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&full_bar[s]), (it / STAGES) & 1,
-                                              WAIT_LIMIT);
+                    ok = wait_warp(full_bar[s], (it / STAGES) & 1, abort_s);
                     if (!ok) break;
                     const uint32_t a = ring + s * STAGE_BYTES, off = s * (STAGE_BYTES / 16);
                     const int live = MODE == kMatrices ? min(BK, p_end - t0) : BK;
@@ -221,11 +216,6 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
         if (!ok) abort_s = 1;
-        __syncwarp();
-        if (abort_s && leader) {  // nor does a product read on
-            tc05::mma_commit(tc05::smem_u32(&quit_bar));
-            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
-        }
     } else if (warp == 2) {
         if (lane == 0) {
             const int sum = MODE == kMatrices ? sh.rows / sh.n_groups : sh.t_size;  // on average
@@ -244,7 +234,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             const bool some = ok && tile.t0 < tile.t_end;
             const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)
-                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s,
+                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s, tiles,
+                                   sh.polls,
                                    [](uint64_t *bar) { tc05::mbar_arrive(tc05::smem_u32(bar)); });
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
@@ -269,11 +260,17 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     __syncwarp();
     tc05::fence_before_sync();
     __syncthreads();
-    if (tid == 0 && abort_s) atomicExch(status, 1);
+    if (abort_s) {
+        wind_down<STAGES>(tiles, full_bar, issued, &quit_bar);
+        if (tid == 0) atomicExch(status, 1);
+    }
     if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
 }
 
 // ---- host -------------------------------------------------------------------------
+static std::atomic<uint32_t> g_sum_polls{kTileWait};
+uint32_t sum_polls() { return g_sum_polls.load(std::memory_order_relaxed); }
+
 template <typename T, int MODE, int BN>
 int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &tail,
            const int64_t *offsets, const Shape &sh, int64_t most_tiles, cudaStream_t s) {
@@ -334,7 +331,7 @@ static int rows_mma_bn(T *out, const T *in, const T *w, const int64_t *offsets, 
     const int64_t most = (rows / BN + n_groups + 2) * ((d_out + 127) / 128);
     const Shape sh{static_cast<int>(rows), n_groups, d_out, 0, d_sum,
                    tiles_per_unit(most, (d_sum + mma::BK - 1) / mma::BK), ldo,
-                   epilogue::piece_of(out, ldo, d_out)};
+                   epilogue::piece_of(out, ldo, d_out), sum_polls()};
     if (BN == 256 && d_out > 128)  // pairs of CTAs have 256 neighbours of a result row
         return pair_launch<T, MODE>(out, a, tail, offsets, sh, s);
     b = tail;
@@ -391,7 +388,7 @@ static int matrices_mma_bn(T *dw, const T *dy, const T *x, const int64_t *offset
     const int64_t each = (rows + n_groups - 1) / n_groups;
     const Shape sh{static_cast<int>(rows), n_groups, d, d_out, 0,
                    tiles_per_unit(most, static_cast<int>((each + mma::BK - 1) / mma::BK)), d,
-                   epilogue::piece_of(dw, d, d)};
+                   epilogue::piece_of(dw, d, d), sum_polls()};
     if (BN == 256 && d > 128) return pair_launch<T, kMatrices>(dw, a, b, offsets, sh, s);
     return launch<T, kMatrices, BN>(dw, a, b, b, offsets, sh, most, s);
 }
@@ -419,3 +416,9 @@ template int matrices_mma<__nv_bfloat16>(void *, const void *, const void *, con
 
 }  // namespace grouped
 }  // namespace pa
+
+extern "C" int pa_selftest_sum_polls(int polls) {
+    pa::grouped::g_sum_polls.store(polls < 0 ? pa::grouped::kTileWait : static_cast<uint32_t>(polls),
+                                   std::memory_order_relaxed);
+    return PA_OK;
+}

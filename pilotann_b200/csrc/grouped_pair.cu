@@ -29,7 +29,6 @@ constexpr int BOX_BYTES = 64 * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int SMEM = STAGES * STAGE_BYTES + epilogue::bytes(BN) + 1024;
 constexpr uint32_t COLS = 512;
-constexpr uint32_t WAIT_LIMIT = 1u << 22;
 }  // namespace pair
 
 template <typename T, int MODE>
@@ -49,6 +48,9 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int told_s;  // CTA 1: the answer that CTA 0 got
     __shared__ volatile int abort_s;
+    // what a pair that gives up has to wait for: slices, and bytes that each brought to CTA 0's barrier
+    __shared__ uint32_t issued_s, bytes_s[STAGES];
+    __shared__ uint32_t tails_s;  // bit s: phase that stage s's next last slice is copied in
     __shared__ Segments segs;
     __shared__ TileRing tiles;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,7 +119,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
 
     if (warp == 0) {
         const bool leader = tc05::elect_one();
-        uint32_t it = 0;
+        uint32_t it = 0, tails = 0;
         bool ok = true;
         Tile tile;
         for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
@@ -127,13 +129,15 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES)
-                    ok = tc05::mbar_wait_warp(tc05::smem_u32(&empty_bar[s]), (it / STAGES - 1) & 1,
-                                              WAIT_LIMIT);
+                    ok = wait_warp(empty_bar[s], (it / STAGES - 1) & 1, abort_s);
                 if (!ok) break;
                 const uint32_t a = ring + s * STAGE_BYTES, b = a + A_BYTES;
                 const uint32_t bar = tc05::map_rank(tc05::smem_u32(&full_bar[s]), 0);
                 const int bytes = A_BYTES + boxes * BOX_BYTES;
-                if (leader && MATRICES && (tile.t_end - t0) % 16 != 0 && tile.t_end - t0 < BK) {
+                const bool tail = MATRICES && (tile.t_end - t0) % 16 != 0 && tile.t_end - t0 < BK;
+                if (tail) tails ^= 1u << s;
+                if (leader) bytes_s[s] = tail ? 0 : bytes;
+                if (leader && tail) {
                     const uint32_t own = tc05::smem_u32(rank == 0 ? &full_bar[s] : &tail_bar[s]);
                     tc05::mbar_expect_tx(own, bytes);
                     tc05::tma_load_2d(a, &map_a, m, t0, own);
@@ -160,10 +164,9 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
         if (!ok) abort_s = 1;
-        if (abort_s) {  // no copy is left in flight behind the pair
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; rank == 0 && i < it; ++i)
-                tc05::mbar_wait_bounded(tc05::smem_u32(&full_bar[i % STAGES]), (i / STAGES) & 1,
-                                        WAIT_LIMIT);
+        if (lane == 0) {
+            issued_s = it;
+            tails_s = tails;
         }
     } else if (warp == 1) {
         const bool leader = tc05::elect_one();
@@ -197,7 +200,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                 it += slices;
                 if (!MATRICES || live % 16 == 0) continue;
                 const int s = (it - 1) % STAGES;
-                ok = tc05::mbar_wait_warp(tc05::smem_u32(&tail_bar[s]), (tails >> s) & 1, WAIT_LIMIT);
+                ok = wait_warp(tail_bar[s], (tails >> s) & 1, abort_s);
                 tails ^= 1u << s;
                 if (!ok) break;
                 clear(s, live);
@@ -207,23 +210,17 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
             const uint32_t idesc = tc05::idesc_f16(is_bf16<T>(), A_MN, B_MN, BM, columns(tile));
             for (int p0 = tile.t0; ok && p0 < tile.t_end; p0 += kPart) {
-                ok = __all_sync(0xffffffffu,
-                                tc05::mbar_wait_cluster(tc05::smem_u32(&acc_empty[slot]),
-                                                        (phases >> slot & 1) ^ 1, WAIT_LIMIT));
+                ok = wait_warp<true>(acc_empty[slot], (phases >> slot & 1) ^ 1, abort_s);
                 const uint32_t d = tmem + slot * BN;
                 const int p_end = part_end(p0, tile.t_end);
                 for (int t0 = p0; ok && t0 < p_end; t0 += BK, ++it) {
                     const int s = it % STAGES;
-                    ok = __all_sync(0xffffffffu,
-                                    tc05::mbar_wait_cluster(tc05::smem_u32(&full_bar[s]),
-                                                            (it / STAGES) & 1, WAIT_LIMIT));
+                    ok = wait_warp<true>(full_bar[s], (it / STAGES) & 1, abort_s);
                     if (!ok) break;
                     const int live = MATRICES ? min(BK, p_end - t0) : BK;
                     if (MATRICES && live % 16 != 0) {
                         clear(s, live);
-                        ok = __all_sync(0xffffffffu,
-                                        tc05::mbar_wait_cluster(tc05::smem_u32(&other_bar[s]),
-                                                                (tails >> s) & 1, WAIT_LIMIT));
+                        ok = wait_warp<true>(other_bar[s], (tails >> s) & 1, abort_s);
                         tails ^= 1u << s;
                         if (!ok) break;
                     }
@@ -246,10 +243,6 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             }
         }
         if (!ok) abort_s = 1;
-        if (abort_s && leader && rank == 0) {  // nor does a product read on
-            tc05::mma_commit_pair(tc05::smem_u32(&quit_bar));
-            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, WAIT_LIMIT);
-        }
     } else if (warp == 2) {
         if (lane == 0) {
             const uint32_t ready0 = tc05::map_rank(tc05::smem_u32(&ready_bar), 0),
@@ -261,15 +254,13 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                     int next = ring_ask(tiles, asked);
                     if (next > 0) next /= 2;  // pairs
                     // CTA 1 has read the answer before
-                    if (!tc05::mbar_wait_cluster(tc05::smem_u32(&ready_bar), asked & 1, kTileWait))
-                        next = -2;
+                    if (!wait_moving<true>(ready_bar, asked & 1, abort_s, tiles.moved)) next = -2;
                     tc05::store_cluster(answer1, static_cast<uint32_t>(next));
                     tc05::mbar_arrive_cluster(told1);
                     return next;
                 }
                 tc05::mbar_arrive_cluster(ready0);
-                if (!tc05::mbar_wait_cluster(tc05::smem_u32(&told_bar), asked & 1, 2 * kTileWait))
-                    return -2;
+                if (!wait_moving<true>(told_bar, asked & 1, abort_s, tiles.moved)) return -2;
                 return told_s;
             };
             const int sum = MATRICES ? sh.rows / sh.n_groups : sh.t_size;  // on average
@@ -291,7 +282,8 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             const bool some = ok && tile.t0 < tile.t_end;
             const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)
-                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s, emptied);
+                ok = sum_parts<BN>(tile, acc_full, acc_empty, slot, phases, tmem, w, abort_s, tiles,
+                                   sh.polls, emptied);
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
             tc05::fence_after_sync();
@@ -315,9 +307,51 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     __syncwarp();
     tc05::fence_before_sync();
     __syncthreads();
-    tc05::cluster_sync();  // nothing of the other CTA reaches here any more
+    if (tid == 0 && abort_s)  // one that gives up takes the other along
+        tc05::store_cluster(
+            tc05::map_rank(tc05::smem_u32(const_cast<int *>(&abort_s)), rank ^ 1), 1);
+    __syncwarp();
+    tc05::cluster_sync();  // nothing of the other CTA reaches here any more, unless it gave up
     tc05::fence_after_sync();
-    if (tid == 0 && abort_s) atomicExch(status, 1);
+    if (abort_s) {
+        // what either has started lands before either ends
+        if (warp == 0 && lane == 0) {
+            const uint32_t mine = issued_s;
+            if (rank == 0) {
+                const uint32_t other = tc05::load_cluster(tc05::map_rank(tc05::smem_u32(&issued_s), 1));
+                const uint32_t top = max(mine, other);
+                for (uint32_t i = top > STAGES ? top - STAGES : 0; i < top; ++i) {
+                    const int s = i % STAGES;
+                    const uint32_t bar = tc05::smem_u32(&full_bar[s]);
+                    if (i < mine) {
+                        if (i >= other && bytes_s[s] != 0)  // CTA 1's half does not come
+                            tc05::mbar_complete_tx(bar, bytes_s[s]);
+                    } else {  // it comes alone
+                        const uint32_t bytes =
+                            tc05::load_cluster(tc05::map_rank(tc05::smem_u32(&bytes_s[s]), 1));
+                        if (bytes == 0) continue;
+                        tc05::mbar_expect_tx(bar, bytes);
+                    }
+                    tc05::mbar_wait_bounded(bar, (i / STAGES) & 1, kTileWait);
+                }
+            } else if (MATRICES) {
+                for (uint32_t i = mine > STAGES ? mine - STAGES : 0; i < mine; ++i)
+                    if (bytes_s[i % STAGES] == 0)
+                        tc05::mbar_wait_bounded(tc05::smem_u32(&tail_bar[i % STAGES]),
+                                                (tails_s >> (i % STAGES) & 1) ^ 1, kTileWait);
+            }
+        }
+        __syncwarp();
+        if (warp == 1 && tc05::elect_one()) {  // the lane that issues; both get an arrival
+            if (rank == 0) tc05::mma_commit_pair(tc05::smem_u32(&quit_bar));
+            tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, kTileWait);
+        }
+        if (tid == 64 && tiles.due)
+            tc05::mbar_wait_bounded(tc05::smem_u32(&tiles.answered), tiles.due - 1, kTileWait);
+        if (tid == 0) atomicExch(status, 1);
+        __syncthreads();
+        tc05::cluster_sync();
+    }
     if (warp == 0) tc05::tmem_dealloc_pair(tmem, COLS);
 }
 

@@ -19,6 +19,7 @@ struct Shape {
     int unit;         // tiles a CTA takes at a time
     int64_t ldo;
     int piece;        // bytes that result rows are stored in
+    uint32_t polls;   // limit of the wait for a sum
 };
 
 struct Segments {
@@ -117,13 +118,57 @@ struct Tile {
     int t0, t_end;    // summed axis
 };
 constexpr int kNoTile = -2;
-constexpr uint32_t kTileWait = 1u << 22;
+
+// ---- waits -----------------------------------------------------------------------------
+// A wait polls an mbarrier, 4 us a poll while nothing happens, and gives up after kTileWait of them (2 s)
+// or once another warp of the CTA has (quit).  No wait spans more than kPart terms of a sum, but the one
+// for room in the ring of tiles: a tile sums up to 2^31 rows (9 s).  That one starts again whenever
+// the warps that store have moved on.  A CTA that gives up waits for what it has started
+// (wind_down), frees its TMEM, sets the status word and returns.
+constexpr uint32_t kTileWait = 1u << 19;
+
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_unless(uint64_t &bar, uint32_t parity, const volatile int &quit,
+                                            uint32_t limit = kTileWait) {
+    const uint32_t at = tc05::smem_u32(&bar);
+    for (uint32_t i = 0; i < limit; ++i) {
+        if (CLUSTER ? tc05::mbar_try_wait_cluster(at, parity) : tc05::mbar_try_wait(at, parity))
+            return true;
+        if (quit) return false;
+    }
+    return false;
+}
+// the same answer in all lanes of the (converged) warp
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_warp(uint64_t &bar, uint32_t parity, const volatile int &quit,
+                                          uint32_t limit = kTileWait) {
+    return __all_sync(0xffffffffu, wait_unless<CLUSTER>(bar, parity, quit, limit));
+}
+// starts again whenever `moved` changes
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_moving(uint64_t &bar, uint32_t parity, const volatile int &quit,
+                                            const volatile uint32_t &moved) {
+    const uint32_t at = tc05::smem_u32(&bar);
+    uint32_t seen = moved;
+    for (uint32_t i = 0; i < kTileWait; ++i) {
+        if (CLUSTER ? tc05::mbar_try_wait_cluster(at, parity) : tc05::mbar_try_wait(at, parity))
+            return true;
+        if (quit) return false;
+        const uint32_t now = moved;
+        if (now != seen) i = 0, seen = now;
+    }
+    return false;
+}
+// the limit of the wait for a sum that launches get (grouped_mma.cu)
+uint32_t sum_polls();
 
 struct TileRing {
     __align__(16) uint4 answer;
     __align__(16) int4 a[4];
     int2 b[4];
     __align__(8) uint64_t full[4], empty[4], answered;
+    volatile uint32_t moved;  // counts what the first of the warps that store has done
+    volatile int due;         // 1 + phase of an answer that was given up
 };
 
 // Tiles known ahead of the slowest reader, for tiles of `slices` slices and a ring of `stages`: the
@@ -139,6 +184,8 @@ __device__ __forceinline__ void ring_init(TileRing &r, int readers) {
         tc05::mbar_init(tc05::smem_u32(&r.empty[i]), readers);
     }
     tc05::mbar_init(tc05::smem_u32(&r.answered), 1);
+    r.moved = 0;
+    r.due = 0;
 }
 
 // Whether tiles are so short that the next one is asked for before there is room for it: an answer
@@ -162,7 +209,10 @@ __device__ __forceinline__ int ring_ask(TileRing &r, uint32_t asked) {
         "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
         "[%0], [%1];" ::"r"(answer), "r"(bar)
         : "memory");
-    if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) return -2;
+    if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) {
+        r.due = 1 + (asked & 1);
+        return -2;
+    }
     uint32_t more, next;
     asm volatile(
         "{\n"
@@ -190,7 +240,7 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
     auto room = [&]() {  // for one more: tile n - depth has been taken by all
         const uint32_t old = n - depth;
         if (n >= static_cast<uint32_t>(depth) &&
-            !tc05::mbar_wait_bounded(tc05::smem_u32(&r.empty[old & 3]), (old / 4) & 1, kTileWait))
+            !wait_moving(r.empty[old & 3], (old / 4) & 1, abort_s, r.moved))
             abort_s = 1;
     };
     for (uint32_t asked = 0; !abort_s; ++asked) {
@@ -227,8 +277,7 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
 template <bool WARP>
 __device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, uint32_t n, Tile &tile) {
     const int slot = n & 3;
-    bool ok = tc05::mbar_wait_bounded(tc05::smem_u32(&r.full[slot]), (n / 4) & 1, kTileWait) &&
-              !abort_s;
+    bool ok = wait_unless(r.full[slot], (n / 4) & 1, abort_s) && !abort_s;
     if (WARP) ok = __all_sync(0xffffffffu, ok);  // lanes that gave up must not leave others behind
     if (!ok) {
         abort_s = 1;
@@ -255,8 +304,8 @@ __device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, ui
 // positive terms came out 4.3e-4 too small after 65536 terms and 6.9e-3 after 2^20, where half a step
 // of fp16 is 4.9e-4.  So a sum is multiplied in parts of 8192 terms (5e-5).  The first part stays
 // where it is; the others go to the other accumulator, one after another, and the warps that store
-// add each to the first, rounding to the nearest, while the products wait, about 1 us a part (one
-// group of 65536 rows, 2048 x 2048: 372 us without parts, 378 with).  Sums of one part are as before:
+// add each to the first, rounding to the nearest, while the products wait, about 2 us a part (one
+// group of 65536 rows, 2048 x 2048: 377 us without parts, 390 with).  Sums of one part are as before:
 // the accumulators take turns, and one is stored while the other is filled.
 constexpr int kSlice = 64;  // terms
 constexpr int kPart = 128 * kSlice;
@@ -269,15 +318,17 @@ __device__ __forceinline__ int part_end(int p0, int t_end) {
 template <int BN, typename Emptied>
 __device__ __forceinline__ bool sum_parts(const Tile &tile, uint64_t *full, uint64_t *empty,
                                           uint32_t &slot, uint32_t &phases, uint32_t tmem, int w,
-                                          volatile int &abort_s, Emptied emptied) {
+                                          volatile int &abort_s, TileRing &ring, uint32_t polls,
+                                          Emptied emptied) {
     constexpr int N = BN < 32 ? 1 : 2;  // 16 columns each
     const uint32_t lanes = tmem + ((32u * w) << 16), sum = lanes + slot * BN;
     const int cols = min(BN, tile.c_end - tile.c0);
     for (int t = 0; t < tile.t_end - tile.t0; t += kPart) {
-        if (!tc05::mbar_wait_warp(tc05::smem_u32(&full[slot]), phases >> slot & 1, kTileWait)) {
+        if (!wait_warp(full[slot], phases >> slot & 1, abort_s, polls)) {
             abort_s = 1;
             return false;
         }
+        if (w == 0 && (threadIdx.x & 31) == 0) ring.moved = ring.moved + 1;
         phases ^= 1u << slot;
         if (t == 0) {
             slot ^= 1;
@@ -308,6 +359,24 @@ __device__ __forceinline__ bool sum_parts(const Tile &tile, uint64_t *full, uint
         if ((threadIdx.x & 31) == 0) emptied(&empty[slot]);
     }
     return true;
+}
+
+// A CTA that gives up, behind a barrier behind which none of its warps starts anything: waits for the
+// copies (`issued` by warp 0, in slices), the products (of warp 1) and the answer that are still on
+// their way, so that none of them reaches memory that is no longer this CTA's.  All threads.
+template <int STAGES>
+__device__ __noinline__ void wind_down(TileRing &r, uint64_t *full, uint32_t issued, uint64_t *quit) {
+    const int warp = threadIdx.x >> 5;
+    if (warp == 0)
+        for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+            tc05::mbar_wait_bounded(tc05::smem_u32(&full[i % STAGES]), (i / STAGES) & 1, kTileWait);
+    if (warp == 1 && tc05::elect_one()) {  // the lane that issues
+        tc05::mma_commit(tc05::smem_u32(quit));
+        tc05::mbar_wait_bounded(tc05::smem_u32(quit), 0, kTileWait);
+    }
+    if (threadIdx.x == 64 && r.due)
+        tc05::mbar_wait_bounded(tc05::smem_u32(&r.answered), r.due - 1, kTileWait);
+    __syncthreads();
 }
 
 // the segment that has row tile `tile`
