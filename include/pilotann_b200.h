@@ -127,7 +127,8 @@ int pa_project(float *out, const float *query, const float *VT, int64_t batch,
 
 /* Synchronises the current device and returns 0, or 1 if a tensor-core kernel of
  * this library gave up on a bounded wait since the last reset (its output is
- * then undefined), or PA_ERR_CUDA.  No upstream counterpart. */
+ * then undefined; of grouped and 4-bit products NaN), or PA_ERR_CUDA.  No upstream
+ * counterpart. */
 int pa_device_status(int reset);
 
 /* Diagnostic for the bounded waits: launches one thread that polls 16 times on an
@@ -333,7 +334,9 @@ int pa_search_reduced_noalloc(int64_t *output_I, float *output_D,
 /* ---- products of grouped rows, 4-bit tables -----------------------------------
  * No counterpart upstream.  Rows that were sent to routers (pa_route) put in group
  * order, every row times the matrix of its own group with the gradients, and tables
- * held in four bits a value.  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
+ * held in four bits a value.  A product whose bounded wait runs out fills its result with NaN;
+ * from then on the products on that device return PA_ERR_CUDA until
+ * pa_device_status(1).  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
  * [1, PA_MAX_GROUPS], a row has at most PA_MAX_WIDTH values, at most PA_MAX_ROWS rows. */
 #define PA_F32 0
 #define PA_BF16 1

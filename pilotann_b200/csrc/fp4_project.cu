@@ -35,7 +35,6 @@ using grouped::kNoTile;
 using grouped::Segments;
 using grouped::Tile;
 using grouped::TileRing;
-using grouped::wait_unless;
 using grouped::wait_warp;
 
 namespace mma {
@@ -453,8 +452,8 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
             const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
             const float *ts = t_scale_s[acc_it % ROW_BUFS], *qs = q_scale_s[acc_it % ROW_BUFS];
             if (METHOD == PA_NVFP4 && some)
-                ok = wait_unless(row_full[acc_it % ROW_BUFS], (acc_it / ROW_BUFS) & 1, abort_s);
-            if (some && ok) ok = wait_unless(acc_full[acc], (acc_it / 2) & 1, abort_s, args.polls);
+                ok = wait_warp(row_full[acc_it % ROW_BUFS], (acc_it / ROW_BUFS) & 1, abort_s);
+            if (some && ok) ok = wait_warp(acc_full[acc], (acc_it / 2) & 1, abort_s, args.polls);
             if (some && !ok) abort_s = 1;
             __syncwarp();
             if (!epilogue::all_agree(ok)) break;
@@ -545,7 +544,14 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
     __syncthreads();
     if (abort_s) {
         grouped::wind_down<STAGES>(tiles, full_bar, issued, &quit_bar);
-        if (tid == 0) atomicExch(args.status, 1);
+        if (args.out_dtype == PA_F32)
+            grouped::gave_up(static_cast<float *>(args.out), args.rows, args.d_out, args.d_out, args.status);
+        else if (args.out_dtype == PA_BF16)
+            grouped::gave_up(static_cast<__nv_bfloat16 *>(args.out), args.rows, args.d_out, args.d_out,
+                             args.status);
+        else
+            grouped::gave_up(static_cast<__half *>(args.out), args.rows, args.d_out, args.d_out,
+                             args.status);
     }
     if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
 }
@@ -629,8 +635,10 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     PA_REQUIRE(aligned_to(out, out_dtype == PA_F32 ? 4 : 2) && aligned_to(query_row_scale, 4) &&
                    aligned_to(row_scale, 4),
                "out and row scales must be aligned to their values");
-    int *status = const_cast<int *>(gemm_status_address());
-    PA_REQUIRE(status != nullptr, "status word not found");
+    const int rc = product_check();
+    if (rc != PA_OK) return rc;
+    int *status = product_status_address();
+    if (status == nullptr) return fail(PA_ERR_CUDA, "no host memory for the status of products");
     const int values = static_cast<int>(fp4::padded(d));
     const int pitch = values / fp4::block_of(method);
     const fp4::Args args{out, query_scales, scales, query_row_scale, row_scale, offsets, d_out,

@@ -583,6 +583,7 @@ extern "C" int pa_project_grouped(void *out, const void *query, const void *VT,
     if (rows == 0) return PA_OK;
     PA_REQUIRE(out && query && VT && offsets, "null pointer");
     PA_REQUIRE(grouped::aligned(dtype, out, query, VT), "operands must be aligned to their values");
+    if ((rc = product_check()) != PA_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PA_F32)
         return grouped::rows_f32(static_cast<float *>(out), static_cast<const float *>(query),
@@ -636,6 +637,7 @@ extern "C" int pa_project_grouped_backward(void *grad_query, void *grad_VT, cons
     PA_REQUIRE(grouped::aligned(dtype, grad_query, grad_VT, grad) &&
                    grouped::aligned(dtype, query, VT, nullptr),
                "operands must be aligned to their values");
+    if ((rc = product_check()) != PA_OK) return rc;
     if (dtype == PA_F32) {
         const float *dy = static_cast<const float *>(grad);
         if (grad_query)

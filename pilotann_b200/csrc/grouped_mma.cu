@@ -262,7 +262,8 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
     __syncthreads();
     if (abort_s) {
         wind_down<STAGES>(tiles, full_bar, issued, &quit_bar);
-        if (tid == 0) atomicExch(status, 1);
+        gave_up(out, MODE == kMatrices ? static_cast<int64_t>(sh.n_groups) * sh.c_size : sh.rows,
+                sh.m_size, sh.ldo, status);
     }
     if (warp == 0) tc05::tmem_dealloc(tmem, COLS);
 }
@@ -283,8 +284,8 @@ int launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap
                                          mma::smem_bytes(BN)));
         configured[dev] = true;
     }
-    int *status = const_cast<int *>(gemm_status_address());
-    PA_REQUIRE(status != nullptr, "status word not found");
+    int *status = product_status_address();
+    if (status == nullptr) return fail(PA_ERR_CUDA, "no host memory for the status of products");
     PA_REQUIRE(most_tiles <= 0x7fff0000, "too many rows for one call");
     const unsigned grid = static_cast<unsigned>((most_tiles + sh.unit - 1) / sh.unit);
     mma_kernel<T, MODE, BN><<<grid, mma::THREADS, mma::smem_bytes(BN), s>>>(out, a, b, tail, offsets, sh,

@@ -251,7 +251,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
                                tc05::smem_u32(const_cast<int *>(&told_s)), 1);
             auto ask = [&](uint32_t asked) -> int {
                 if (rank == 0) {
-                    int next = ring_ask(tiles, asked);
+                    int next = ring_ask(tiles);
                     if (next > 0) next /= 2;  // pairs
                     // CTA 1 has read the answer before
                     if (!wait_moving<true>(ready_bar, asked & 1, abort_s, tiles.moved)) next = -2;
@@ -346,9 +346,9 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
             if (rank == 0) tc05::mma_commit_pair(tc05::smem_u32(&quit_bar));
             tc05::mbar_wait_bounded(tc05::smem_u32(&quit_bar), 0, kTileWait);
         }
-        if (tid == 64 && tiles.due)
-            tc05::mbar_wait_bounded(tc05::smem_u32(&tiles.answered), tiles.due - 1, kTileWait);
-        if (tid == 0) atomicExch(status, 1);
+        if (tid == 64 && rank == 0) ring_close(tiles);
+        gave_up(out, MATRICES ? static_cast<int64_t>(sh.n_groups) * sh.c_size : sh.rows, sh.m_size,
+                sh.ldo, status);
         __syncthreads();
         tc05::cluster_sync();
     }
@@ -368,8 +368,8 @@ int pair_launch(T *out, const CUtensorMap &a, const CUtensorMap &b, const int64_
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
         configured[dev] = true;
     }
-    int *status = const_cast<int *>(gemm_status_address());
-    PA_REQUIRE(status != nullptr, "status word not found");
+    int *status = product_status_address();
+    if (status == nullptr) return fail(PA_ERR_CUDA, "no host memory for the status of products");
     const int64_t m_tiles = (shape.m_size + pair::BM - 1) / pair::BM;
     const int64_t most =
         m_tiles * (MODE == kMatrices

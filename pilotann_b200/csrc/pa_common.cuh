@@ -52,6 +52,11 @@ bool gemm_operands_ok(const float *A, const float *B, int K, int64_t lda, int64_
 int gemm_small_launch(float *out, const float *A, const float *B, int M, int N, int K, int64_t lda,
                       int64_t ldb, int64_t ldo, cudaStream_t stream);
 const int *gemm_status_address();
+// api.cu: where a product on the current device says that it gave up (nullptr: no such memory), what
+// it says, and the error of calls behind one
+int *product_status_address();
+int product_status(bool reset);
+int product_check();
 int project_launch(float *out, const float *query, const float *VT, int64_t batch, int d,
                    int d_out, int64_t ld_out, cudaStream_t stream);
 

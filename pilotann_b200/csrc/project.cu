@@ -494,5 +494,5 @@ extern "C" int pa_device_status(int reset) {
         const int zero = 0;
         cudaMemcpyToSymbol(pa::g_gemm_status, &zero, sizeof(int));
     }
-    return status;
+    return status | pa::product_status(reset != 0);
 }

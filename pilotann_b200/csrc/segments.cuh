@@ -123,26 +123,35 @@ constexpr int kNoTile = -2;
 // A wait polls an mbarrier, 4 us a poll while nothing happens, and gives up after kTileWait of them (2 s)
 // or once another warp of the CTA has (quit).  No wait spans more than kPart terms of a sum, but the one
 // for room in the ring of tiles: a tile sums up to 2^31 rows (9 s).  That one starts again whenever
-// the warps that store have moved on.  A CTA that gives up waits for what it has started
-// (wind_down), frees its TMEM, sets the status word and returns.
+// the warps that store have moved on.  A CTA that gives up waits for what it has started and
+// keeps the rest of the grid from starting (wind_down), fills the result with NaN, sets the status word,
+// frees its TMEM and returns.
 constexpr uint32_t kTileWait = 1u << 19;
 
+template <bool CLUSTER>
+__device__ __forceinline__ bool over(uint32_t bar, uint32_t parity) {
+    return CLUSTER ? tc05::mbar_try_wait_cluster(bar, parity) : tc05::mbar_try_wait(bar, parity);
+}
+// one thread
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait_unless(uint64_t &bar, uint32_t parity, const volatile int &quit,
-                                            uint32_t limit = kTileWait) {
+__device__ __forceinline__ bool wait_unless(uint64_t &bar, uint32_t parity, const volatile int &quit) {
     const uint32_t at = tc05::smem_u32(&bar);
-    for (uint32_t i = 0; i < limit; ++i) {
-        if (CLUSTER ? tc05::mbar_try_wait_cluster(at, parity) : tc05::mbar_try_wait(at, parity))
-            return true;
+    for (uint32_t i = 0; i < kTileWait; ++i) {
+        if (over<CLUSTER>(at, parity)) return true;
         if (quit) return false;
     }
     return false;
 }
-// the same answer in all lanes of the (converged) warp
+// a converged warp, with the same answer in all lanes: they leave the loop together
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_warp(uint64_t &bar, uint32_t parity, const volatile int &quit,
                                           uint32_t limit = kTileWait) {
-    return __all_sync(0xffffffffu, wait_unless<CLUSTER>(bar, parity, quit, limit));
+    const uint32_t at = tc05::smem_u32(&bar);
+    for (uint32_t i = 0; i < limit; ++i) {
+        if (__all_sync(0xffffffffu, over<CLUSTER>(at, parity))) return true;
+        if (__any_sync(0xffffffffu, quit)) return false;
+    }
+    return false;
 }
 // starts again whenever `moved` changes
 template <bool CLUSTER = false>
@@ -151,8 +160,7 @@ __device__ __forceinline__ bool wait_moving(uint64_t &bar, uint32_t parity, cons
     const uint32_t at = tc05::smem_u32(&bar);
     uint32_t seen = moved;
     for (uint32_t i = 0; i < kTileWait; ++i) {
-        if (CLUSTER ? tc05::mbar_try_wait_cluster(at, parity) : tc05::mbar_try_wait(at, parity))
-            return true;
+        if (over<CLUSTER>(at, parity)) return true;
         if (quit) return false;
         const uint32_t now = moved;
         if (now != seen) i = 0, seen = now;
@@ -168,7 +176,9 @@ struct TileRing {
     int2 b[4];
     __align__(8) uint64_t full[4], empty[4], answered;
     volatile uint32_t moved;  // counts what the first of the warps that store has done
-    volatile int due;         // 1 + phase of an answer that was given up
+    volatile uint32_t asked;  // how often launch control was asked
+    volatile int due;         // the last answer was given up
+    volatile int none;        // it said that there is nothing left
 };
 
 // Tiles known ahead of the slowest reader, for tiles of `slices` slices and a ring of `stages`: the
@@ -184,8 +194,8 @@ __device__ __forceinline__ void ring_init(TileRing &r, int readers) {
         tc05::mbar_init(tc05::smem_u32(&r.empty[i]), readers);
     }
     tc05::mbar_init(tc05::smem_u32(&r.answered), 1);
-    r.moved = 0;
-    r.due = 0;
+    r.moved = r.asked = 0;
+    r.due = r.none = 0;
 }
 
 // Whether tiles are so short that the next one is asked for before there is room for it: an answer
@@ -200,19 +210,8 @@ inline int tiles_per_unit(int64_t tiles, int slices) {
     return unit;
 }
 
-// Asks for the work of a CTA (or cluster) that has not started: the number of its first CTA, -1 if
-// there is none, -2 if no answer came.
-__device__ __forceinline__ int ring_ask(TileRing &r, uint32_t asked) {
-    const uint32_t answer = tc05::smem_u32(&r.answer), bar = tc05::smem_u32(&r.answered);
-    tc05::mbar_expect_tx(bar, 16);
-    asm volatile(
-        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
-        "[%0], [%1];" ::"r"(answer), "r"(bar)
-        : "memory");
-    if (!tc05::mbar_wait_bounded(bar, asked & 1, kTileWait)) {
-        r.due = 1 + (asked & 1);
-        return -2;
-    }
+// The answer that has come: the number of the first CTA that was taken over, -1 if there was none.
+__device__ __forceinline__ int ring_answer(TileRing &r) {
     uint32_t more, next;
     asm volatile(
         "{\n"
@@ -225,10 +224,39 @@ __device__ __forceinline__ int ring_ask(TileRing &r, uint32_t asked) {
         "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n"
         "}\n"
         : "=r"(more), "=r"(next)
-        : "r"(answer)
+        : "r"(tc05::smem_u32(&r.answer))
         : "memory");
     tc05::fence_proxy_async_smem();  // the answer has been read before the next one is written
+    if (!more) r.none = 1;
     return more ? static_cast<int>(next) : -1;
+}
+
+// Asks for the work of a CTA (or cluster) that has not started: the number of its first CTA, -1 if
+// there is none, -2 if no answer came.
+__device__ __forceinline__ int ring_ask(TileRing &r) {
+    const uint32_t bar = tc05::smem_u32(&r.answered), phase = r.asked & 1;
+    r.asked = r.asked + 1;
+    tc05::mbar_expect_tx(bar, 16);
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+        "[%0], [%1];" ::"r"(tc05::smem_u32(&r.answer)), "r"(bar)
+        : "memory");
+    if (!tc05::mbar_wait_bounded(bar, phase, kTileWait)) {
+        r.due = 1;
+        return -2;
+    }
+    return ring_answer(r);
+}
+
+// One thread of a CTA that gives up: takes over what has not started, to leave it at that.  Nothing may
+// be asked behind an answer that there is nothing left, nor before the last answer has come.
+__device__ __forceinline__ void ring_close(TileRing &r) {
+    if (r.due) {
+        if (!tc05::mbar_wait_bounded(tc05::smem_u32(&r.answered), (r.asked - 1) & 1, kTileWait)) return;
+        ring_answer(r);
+    }
+    while (!r.none)
+        if (ring_ask(r) < 0) break;
 }
 
 // One thread hands out tiles: make(index) is the tile, or has g == kNoTile for an index that the
@@ -269,7 +297,7 @@ template <typename Make>
 __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, int depth, int unit,
                                            bool ahead, Make make) {
     ring_serve(r, abort_s, depth, unit, ahead, static_cast<int>(blockIdx.x), make,
-               [&](uint32_t asked) { return ring_ask(r, asked); });
+               [&](uint32_t) { return ring_ask(r); });
 }
 
 // A reader's side: the n-th tile of this CTA.  A thread for itself, or (WARP) a whole warp.
@@ -277,8 +305,11 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
 template <bool WARP>
 __device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, uint32_t n, Tile &tile) {
     const int slot = n & 3;
-    bool ok = wait_unless(r.full[slot], (n / 4) & 1, abort_s) && !abort_s;
-    if (WARP) ok = __all_sync(0xffffffffu, ok);  // lanes that gave up must not leave others behind
+    bool ok;
+    if (WARP)
+        ok = __all_sync(0xffffffffu, wait_warp(r.full[slot], (n / 4) & 1, abort_s) && !abort_s);
+    else
+        ok = wait_unless(r.full[slot], (n / 4) & 1, abort_s) && !abort_s;
     if (!ok) {
         abort_s = 1;
         return false;
@@ -363,9 +394,10 @@ __device__ __forceinline__ bool sum_parts(const Tile &tile, uint64_t *full, uint
 
 // A CTA that gives up, behind a barrier behind which none of its warps starts anything: waits for the
 // copies (`issued` by warp 0, in slices), the products (of warp 1) and the answer that are still on
-// their way, so that none of them reaches memory that is no longer this CTA's.  All threads.
+// their way, so that none of them reaches memory that is no longer this CTA's, and keeps CTAs that have
+// not started from it.  All threads.
 template <int STAGES>
-__device__ __noinline__ void wind_down(TileRing &r, uint64_t *full, uint32_t issued, uint64_t *quit) {
+__device__ __forceinline__ void wind_down(TileRing &r, uint64_t *full, uint32_t issued, uint64_t *quit) {
     const int warp = threadIdx.x >> 5;
     if (warp == 0)
         for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
@@ -374,9 +406,21 @@ __device__ __noinline__ void wind_down(TileRing &r, uint64_t *full, uint32_t iss
         tc05::mma_commit(tc05::smem_u32(quit));
         tc05::mbar_wait_bounded(tc05::smem_u32(quit), 0, kTileWait);
     }
-    if (threadIdx.x == 64 && r.due)
-        tc05::mbar_wait_bounded(tc05::smem_u32(&r.answered), r.due - 1, kTileWait);
+    if (threadIdx.x == 64) ring_close(r);
     __syncthreads();
+}
+
+// A result of which tiles are missing becomes NaN, all of it: which tiles those are is not known of work
+// that was taken over last.  (CTAs that do not give up may still store theirs.)  All threads.
+template <typename T>
+__device__ __forceinline__ void gave_up(T *out, int64_t rows, int64_t width, int64_t ld, int *status) {
+    for (int64_t r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5)
+        for (int64_t m = threadIdx.x & 31; m < width; m += 32)
+            out[r * ld + m] = from_f32<T>(CUDART_NAN_F);
+    if (threadIdx.x == 0) {
+        *static_cast<volatile int *>(status) = 1;  // host memory
+        __threadfence_system();
+    }
 }
 
 // the segment that has row tile `tile`
