@@ -8,6 +8,7 @@ errors (``RuntimeError``) and streams follow :mod:`pilotann_b200.extension`.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _C
 
@@ -157,6 +158,15 @@ def _grouped_backward(grad, query, VT, offsets, want_query, want_VT):
     return dq, dw
 
 
+def _no_tangent(name: str, *tensors) -> None:
+    """Inside a ``forward_ad.dual_level``: a tangent would be dropped without a word."""
+    if forward_ad._current_level < 0:
+        return
+    for x in tensors:
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 class _ProjectGrouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, VT, offsets):
@@ -187,13 +197,15 @@ def project_grouped(query: torch.Tensor, VT: torch.Tensor, offsets: torch.Tensor
     read there: values that do not ascend give unspecified rows, never an access outside the
     tensors.
 
-    Differentiable in ``query`` and ``VT``; not while the stream is being captured into a CUDA
+    Differentiable in ``query`` and ``VT``, once and in reverse mode (a forward-mode tangent is
+    refused); not while the stream is being captured into a CUDA
     graph: autograd runs a leaf's accumulation on the stream of the oldest live graph of that
     leaf, and where that is an eager one the capture breaks, or the process.  In a capture
     call this under ``torch.no_grad()`` and :func:`project_grouped_backward` for the
     gradients."""
     _grouped_checks(query, VT, offsets)
     _row_stride("query", query)
+    _no_tangent("project_grouped", query, VT)
     if torch.is_grad_enabled() and (query.requires_grad or VT.requires_grad):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("project_grouped records no gradient in a stream capture: call it "
@@ -207,8 +219,10 @@ def project_grouped_backward(grad: torch.Tensor, query: torch.Tensor, VT: torch.
                              want_VT: bool = True):
     """Gradients of :func:`project_grouped`: ``(grad_query [rows, d], grad_VT [n_groups,
     d_out, d])``, ``None`` for one that is not wanted.  ``grad_query[i] = grad[i] @ VT[g]``,
-    ``grad_VT[g] = grad[g's rows].T @ query[g's rows]`` (zeros for a group without rows)."""
+    ``grad_VT[g] = grad[g's rows].T @ query[g's rows]`` (zeros for a group without rows).  They
+    have no gradient themselves."""
     _grouped_checks(query, VT, offsets)
+    _no_tangent("project_grouped_backward", grad, query, VT)
     _check("grad", grad, 2, (query.dtype,))
     _same_device(query, "grad", grad)
     _require(tuple(grad.shape) == (query.size(0), VT.size(1)), "grad.shape == (rows, d_out)")
@@ -272,7 +286,8 @@ def quantize_fp4(x: torch.Tensor, method: str = "mxfp4") -> Fp4Table:
     ``mxfp4``: blocks of 32 values, scale ``2 ** (floor(log2 max|v|) - 2)``; ``nvfp4``: blocks
     of 16, scale ``max|v| / (6 s)`` in E4M3 times the row's power of two ``s``, the least with
     ``max|v| <= 6 * 448 s``.  Values go to the nearest code, ties to the even one, above 6 to
-    6.  A block (``mxfp4``) or row (``nvfp4``) with NaN or infinity becomes NaN as a whole."""
+    6.  A block (``mxfp4``) or row (``nvfp4``) with NaN or infinity becomes NaN as a whole.  Codes
+    have no gradient, whether or not ``x`` wants one."""
     if method not in _METHOD:
         raise RuntimeError(f"unknown 4-bit method {method!r}: mxfp4 or nvfp4")
     dim = x.dim() if isinstance(x, torch.Tensor) else 2
@@ -328,7 +343,8 @@ def project_fp4(query, table: Fp4Table, offsets: torch.Tensor | None = None,
     being the query quantised by the table's method in the same call (or an :class:`Fp4Table`
     of rows), sums in float32, result rounded once to ``dtype``.  With ``offsets`` the table is
     ``[n_groups, d_out, d]`` and every row meets the table of its group, as in
-    :func:`project_grouped`; rows of no group give zeros."""
+    :func:`project_grouped`; rows of no group give zeros.  The scores have no gradient, whether or
+    not ``query`` wants one."""
     if not isinstance(table, Fp4Table):
         raise RuntimeError("table must be an Fp4Table")
     if dtype not in _DTYPE:
