@@ -84,18 +84,27 @@ template <typename T> __device__ __forceinline__ uint32_t top_bits(const Raw<T> 
 // step has four, so that a quotient is a border between two codes (a multiple of 1/4) exactly or at
 // least 2^-13 away from it: a product with the reciprocal, off by 2^-22 of its value, is rounded
 // to a multiple of 2^-14 by adding and subtracting 768, which lands on the border in the first
-// case and stays off it in the other, for two instructions a value.  (It loses the sign of what becomes 0.)
+// case and stays off it in the other, for two instructions a value.  The subtraction makes a +0 of what
+// becomes 0; signs come from the values, so that codes do not depend on their type.
+__device__ __forceinline__ uint32_t signs_of(const Raw<float> &) { return 0; }  // not lost
+template <typename T> __device__ __forceinline__ uint32_t signs_of(const Raw<T> &raw) {
+    // high bytes of the even and the odd values
+    const uint32_t a = __byte_perm(raw.w[0], raw.w[1], 0x7351),
+                   b = __byte_perm(raw.w[2], raw.w[3], 0x7351);
+    const uint32_t even = __byte_perm(a, b, 0x5410), odd = __byte_perm(a, b, 0x7632);
+    return (even >> 4 & 0x08080808u) | (odd & 0x80808080u);
+}
 template <typename T>
-__device__ __forceinline__ uint32_t codes_by(float (&v)[8], float step) {
+__device__ __forceinline__ uint32_t codes_by(float (&v)[8], float step, const Raw<T> &raw) {
     if (sizeof(T) == 2 && step >= 1.1754944e-38f) {  // a reciprocal that does not overflow
         float inv;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));  // step < 2^126
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(__fmaf_rn(v[j], inv, 768.0f), -768.0f);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = step > 0.0f ? __fdiv_rn(v[j], step) : 0.0f;
+        return codes_of(v) | signs_of(raw);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = step > 0.0f ? __fdiv_rn(v[j], step) : 0.0f;
     return codes_of(v);
 }
 
@@ -168,7 +177,7 @@ quantize_kernel(uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                 if (e == 255u) { byte = 255u; code = 0u; }
             } else {
                 byte = scale_of<T>(__fmul_rn(__uint_as_float(top), s_inv));
-                code = codes_by<T>(v, __fmul_rn(e4m3_value(byte), s));
+                code = codes_by(v, __fmul_rn(e4m3_value(byte), s), raw[c]);
                 if (!(s > 0.0f)) { byte = 0u; code = 0u; }  // NaN: the row's scale says it
             }
             if (at < dp) {

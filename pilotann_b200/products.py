@@ -286,8 +286,8 @@ def quantize_fp4(x: torch.Tensor, method: str = "mxfp4") -> Fp4Table:
     ``mxfp4``: blocks of 32 values, scale ``2 ** (floor(log2 max|v|) - 2)``; ``nvfp4``: blocks
     of 16, scale ``max|v| / (6 s)`` in E4M3 times the row's power of two ``s``, the least with
     ``max|v| <= 6 * 448 s``.  Values go to the nearest code, ties to the even one, above 6 to
-    6.  A block (``mxfp4``) or row (``nvfp4``) with NaN or infinity becomes NaN as a whole.  Codes
-    have no gradient, whether or not ``x`` wants one."""
+    6.  A block (``mxfp4``) or row (``nvfp4``) with NaN or infinity becomes NaN as a whole.  Equal
+    values give equal codes whatever their type.  Codes have no gradient, whether or not ``x`` wants one."""
     if method not in _METHOD:
         raise RuntimeError(f"unknown 4-bit method {method!r}: mxfp4 or nvfp4")
     dim = x.dim() if isinstance(x, torch.Tensor) else 2
