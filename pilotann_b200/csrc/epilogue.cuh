@@ -71,23 +71,22 @@ __device__ __forceinline__ void store_rows(T *dst, int64_t ld, uint32_t buf, int
     constexpr int kEach = sizeof(V) / 2, kThreadsPerRow = 128 / kEach;
     const int m = kEach * (tid % kThreadsPerRow);
     if (m >= m_left) return;
-    if constexpr (kThreadsPerRow <= kThreads) {
+    static_assert(kThreadsPerRow <= kThreads, "a row at a time at least");
 #pragma unroll 4
-        for (int c = tid / kThreadsPerRow; c < rows; c += kThreads / kThreadsPerRow) {
-            V v;
-            const uint32_t from = buf + c * kPitch + 2 * m;
-            if constexpr (sizeof(V) == 16)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
-            else if constexpr (sizeof(V) == 8)
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                             : "=r"(v.x), "=r"(v.y) : "r"(from) : "memory");
-            else if constexpr (sizeof(V) == 4)
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-            else
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-            *reinterpret_cast<V *>(dst + c * ld + m) = v;
-        }
+    for (int c = tid / kThreadsPerRow; c < rows; c += kThreads / kThreadsPerRow) {
+        V v;
+        const uint32_t from = buf + c * kPitch + 2 * m;
+        if constexpr (sizeof(V) == 16)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+        else if constexpr (sizeof(V) == 8)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                         : "=r"(v.x), "=r"(v.y) : "r"(from) : "memory");
+        else if constexpr (sizeof(V) == 4)
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+        else
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+        *reinterpret_cast<V *>(dst + c * ld + m) = v;
     }
 }
 

@@ -22,10 +22,6 @@ namespace fp4 {
 __host__ __device__ constexpr int block_of(int method) { return method == PA_MXFP4 ? 32 : 16; }
 __host__ __device__ constexpr int64_t padded(int64_t d) { return (d + 31) / 32 * 32; }
 
-__device__ __forceinline__ float load_f32(const float *p) { return *p; }
-__device__ __forceinline__ float load_f32(const __half *p) { return __half2float(*p); }
-__device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-
 // eight values -> eight codes, value i in bits [4 i, 4 i + 4); nearest, ties to even, largest 6
 __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
     uint32_t r;

@@ -30,7 +30,6 @@
 namespace pa {
 namespace fp4 {
 
-using grouped::from_f32;
 using grouped::kNoTile;
 using grouped::Segments;
 using grouped::Tile;
@@ -202,7 +201,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         uint32_t it = 0;
         bool ok = true;
         Tile tile;
-        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && grouped::ring_take(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0) continue;
             const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
             for (int k = 0; k < n_stages; ++k, ++it) {
@@ -236,7 +235,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         // of the first stage; a descriptor counts 16 bytes, so others are sums
         const uint64_t desc_a = tc05::smem_desc_sw128(ring);
         Tile tile;
-        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && grouped::ring_take(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0) continue;
             const int acc = acc_it & 1;
             if (acc_it >= 2)
@@ -294,7 +293,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         Tile tile;
         uint32_t sg = 0, n_some = 0;
         bool ok = true;
-        for (uint32_t n = 0; ok && grouped::ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && grouped::ring_take(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0) continue;
             float t_row = 1.0f, q_row[NB];
 #pragma unroll
@@ -376,7 +375,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         uint32_t n = 0;
         auto rows_of_tile = [&]() {  // skips tiles without a group; false at the end
             do {
-                if (!grouped::ring_take<true>(tiles, abort_s, n++, tile)) return false;
+                if (!grouped::ring_take(tiles, abort_s, n++, tile)) return false;
             } while (tile.g < 0);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -447,7 +446,7 @@ project_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant_
         for (;; ++n_tile) {
             // the four warps must agree on what they do: they meet at barriers below
             Tile tile;
-            bool ok = grouped::ring_take<true>(tiles, abort_s, n_tile, tile);
+            bool ok = grouped::ring_take(tiles, abort_s, n_tile, tile);
             const bool some = ok && tile.g >= 0;
             const int acc = acc_it & 1, live = min(BN, tile.c_end - tile.c0);
             const float *ts = t_scale_s[acc_it % ROW_BUFS], *qs = q_scale_s[acc_it % ROW_BUFS];

@@ -1,4 +1,4 @@
-// Conversions and the segments of grouped rows, shared by the products.
+// The segments of grouped rows, and what the products share.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -9,10 +9,6 @@
 namespace pa {
 namespace grouped {
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T> __device__ __forceinline__ T from_f32(float v);  // round to nearest even
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }

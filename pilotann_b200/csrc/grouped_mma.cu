@@ -124,7 +124,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         uint32_t it = 0;
         bool ok = true;
         Tile tile;
-        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && ring_take(tiles, abort_s, n, tile); ++n) {
             const int boxes = (min(BN, tile.c_end - tile.c0) + BOX - 1) / BOX;
             for (int t0 = tile.t0; t0 < tile.t_end; t0 += BK, ++it) {
                 const int s = it % STAGES;
@@ -168,7 +168,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, 8192)
                                      : tc05::smem_desc_sw128(ring + A_BYTES);
         Tile tile;
-        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && ring_take(tiles, abort_s, n, tile); ++n) {
             if (tile.t0 >= tile.t_end) continue;
             const int cols = min(BN, tile.c_end - tile.c0);
             const uint32_t idesc =
@@ -230,7 +230,7 @@ mma_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         for (uint32_t n = 0;; ++n) {
             // the four warps must agree on what they do: they meet at barriers below
             Tile tile;
-            bool ok = ring_take<true>(tiles, abort_s, n, tile);
+            bool ok = ring_take(tiles, abort_s, n, tile);
             const bool some = ok && tile.t0 < tile.t_end;
             const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)

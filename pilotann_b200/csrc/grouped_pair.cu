@@ -122,7 +122,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         uint32_t it = 0, tails = 0;
         bool ok = true;
         Tile tile;
-        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && ring_take(tiles, abort_s, n, tile); ++n) {
             const int half = columns(tile) / 2, boxes = (half + 63) / 64;
             const int m = tile.m0 + 128 * static_cast<int>(rank);
             const int c = tile.c0 + half * static_cast<int>(rank);
@@ -178,7 +178,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         const uint64_t desc_b = B_MN ? tc05::smem_desc_mn_sw128(ring + A_BYTES, BOX_BYTES)
                                      : tc05::smem_desc_sw128(ring + A_BYTES);
         Tile tile;
-        for (uint32_t n = 0; ok && ring_take<true>(tiles, abort_s, n, tile); ++n) {
+        for (uint32_t n = 0; ok && ring_take(tiles, abort_s, n, tile); ++n) {
             if (tile.g < 0 || tile.t0 >= tile.t_end) continue;
             const int boxes = (columns(tile) / 2 + 63) / 64;
             // clears the rows of the next group up to the end of the last k step: 128 bytes each
@@ -278,7 +278,7 @@ pair_kernel(T *__restrict__ out, const __grid_constant__ CUtensorMap map_a,
         };
         for (uint32_t n = 0;; ++n) {
             Tile tile;
-            bool ok = ring_take<true>(tiles, abort_s, n, tile);
+            bool ok = ring_take(tiles, abort_s, n, tile);
             const bool some = ok && tile.t0 < tile.t_end;
             const uint32_t sum = slot;  // the accumulator that the sum is in, in the end
             if (some)

@@ -300,33 +300,25 @@ __device__ __forceinline__ void ring_serve(TileRing &r, volatile int &abort_s, i
                [&](uint32_t) { return ring_ask(r); });
 }
 
-// A reader's side: the n-th tile of this CTA.  A thread for itself, or (WARP) a whole warp.
-// false: no more, or gave up.
-template <bool WARP>
+// A reader's side: the n-th tile of this CTA, for a (converged) warp.  false: no more, or gave up.
 __device__ __forceinline__ bool ring_take(TileRing &r, volatile int &abort_s, uint32_t n, Tile &tile) {
     const int slot = n & 3;
-    bool ok;
-    if (WARP)
-        ok = __all_sync(0xffffffffu, wait_warp(r.full[slot], (n / 4) & 1, abort_s) && !abort_s);
-    else
-        ok = wait_unless(r.full[slot], (n / 4) & 1, abort_s) && !abort_s;
-    if (!ok) {
+    // lanes that gave up must not leave others behind
+    if (!__all_sync(0xffffffffu, wait_warp(r.full[slot], (n / 4) & 1, abort_s) && !abort_s)) {
         abort_s = 1;
         return false;
     }
     const int4 a = r.a[slot];
     const int2 b = r.b[slot];
-    if (WARP) __syncwarp();
-    if (!WARP || (threadIdx.x & 31) == 0) tc05::mbar_arrive(tc05::smem_u32(&r.empty[slot]));
-    tile = Tile{a.x, a.y, a.z, a.w, b.x, b.y};
-    if (WARP) {  // one value for the warp
-        tile.g = __shfl_sync(0xffffffffu, tile.g, 0);
-        tile.m0 = __shfl_sync(0xffffffffu, tile.m0, 0);
-        tile.c0 = __shfl_sync(0xffffffffu, tile.c0, 0);
-        tile.c_end = __shfl_sync(0xffffffffu, tile.c_end, 0);
-        tile.t0 = __shfl_sync(0xffffffffu, tile.t0, 0);
-        tile.t_end = __shfl_sync(0xffffffffu, tile.t_end, 0);
-    }
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc05::mbar_arrive(tc05::smem_u32(&r.empty[slot]));
+    // one value for the warp
+    tile.g = __shfl_sync(0xffffffffu, a.x, 0);
+    tile.m0 = __shfl_sync(0xffffffffu, a.y, 0);
+    tile.c0 = __shfl_sync(0xffffffffu, a.z, 0);
+    tile.c_end = __shfl_sync(0xffffffffu, a.w, 0);
+    tile.t0 = __shfl_sync(0xffffffffu, b.x, 0);
+    tile.t_end = __shfl_sync(0xffffffffu, b.y, 0);
     return tile.g != kNoTile;
 }
 
