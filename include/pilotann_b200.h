@@ -336,7 +336,7 @@ int pa_search_reduced_noalloc(int64_t *output_I, float *output_D,
  * order, every row times the matrix of its own group with the gradients, and tables
  * held in four bits a value.  A product whose bounded wait runs out fills its result with NaN;
  * from then on the products on that device return PA_ERR_CUDA until
- * pa_device_status(1).  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
+ * pa_device_status(1).  Pointers are aligned to their values.  dtype: PA_F32, PA_BF16, PA_F16.  n_groups is in
  * [1, PA_MAX_GROUPS], a row has at most PA_MAX_WIDTH values, at most PA_MAX_ROWS rows. */
 #define PA_F32 0
 #define PA_BF16 1

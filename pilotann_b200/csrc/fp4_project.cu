@@ -632,8 +632,8 @@ extern "C" int pa_project_fp4(void *out, const uint8_t *query_codes, const uint8
     PA_REQUIRE(method == PA_MXFP4 || (query_row_scale && row_scale), "nvfp4 needs row scales");
     PA_REQUIRE(aligned16(query_codes) && aligned16(codes), "codes must be 16-byte aligned");
     PA_REQUIRE(aligned_to(out, out_dtype == PA_F32 ? 4 : 2) && aligned_to(query_row_scale, 4) &&
-                   aligned_to(row_scale, 4),
-               "out and row scales must be aligned to their values");
+                   aligned_to(row_scale, 4) && aligned_to(offsets, 8),
+               "out, row scales and offsets must be aligned to their values");
     const int rc = product_check();
     if (rc != PA_OK) return rc;
     int *status = product_status_address();

@@ -225,6 +225,9 @@ extern "C" int pa_group_rows(int64_t *order, int64_t *offsets, const int64_t *ro
     PA_REQUIRE(offsets && (rows == 0 || (order && router)), "null pointer");
     const bool single = rows <= group::kSingleRows;
     PA_REQUIRE(single || workspace, "workspace missing (pa_group_rows_workspace_bytes)");
+    PA_REQUIRE(aligned_to(order, 8) && aligned_to(offsets, 8) && aligned_to(router, 8) &&
+                   aligned_to(workspace, 4),
+               "order, offsets and router must be aligned to 8 bytes, workspace to 4");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (rows <= group::kBlockRows)
         return scatter_launch<group::kWarps>(order, offsets, nullptr, router, rows, n_groups, 1, s);

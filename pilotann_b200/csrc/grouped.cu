@@ -544,9 +544,9 @@ int check(int64_t rows, int n_groups, int d, int d_out, int dtype) {
     return PA_OK;
 }
 
-bool aligned(int dtype, const void *a, const void *b, const void *c) {
+bool aligned(int dtype, const int64_t *offsets, const void *a, const void *b, const void *c) {
     const size_t size = dtype == PA_F32 ? 4 : 2;
-    return aligned_to(a, size) && aligned_to(b, size) && aligned_to(c, size);
+    return aligned_to(a, size) && aligned_to(b, size) && aligned_to(c, size) && aligned_to(offsets, 8);
 }
 
 // forward, or with `transposed` the gradient of the rows, of 16-bit values
@@ -582,7 +582,7 @@ extern "C" int pa_project_grouped(void *out, const void *query, const void *VT,
     PA_REQUIRE(ld_query >= d && ld_out >= d_out, "row strides must cover the rows");
     if (rows == 0) return PA_OK;
     PA_REQUIRE(out && query && VT && offsets, "null pointer");
-    PA_REQUIRE(grouped::aligned(dtype, out, query, VT), "operands must be aligned to their values");
+    PA_REQUIRE(grouped::aligned(dtype, offsets, out, query, VT), "operands must be aligned to their values");
     if ((rc = product_check()) != PA_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == PA_F32)
@@ -634,8 +634,8 @@ extern "C" int pa_project_grouped_backward(void *grad_query, void *grad_VT, cons
         return PA_OK;
     }
     PA_REQUIRE(grad && offsets && (!grad_query || VT) && (!grad_VT || query), "null pointer");
-    PA_REQUIRE(grouped::aligned(dtype, grad_query, grad_VT, grad) &&
-                   grouped::aligned(dtype, query, VT, nullptr),
+    PA_REQUIRE(grouped::aligned(dtype, offsets, grad_query, grad_VT, grad) &&
+                   grouped::aligned(dtype, offsets, query, VT, nullptr),
                "operands must be aligned to their values");
     if ((rc = product_check()) != PA_OK) return rc;
     if (dtype == PA_F32) {
