@@ -77,7 +77,7 @@ void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 }  // namespace pa
 
-// 105: products of grouped rows, 4-bit tables
-extern "C" int pa_version(void) { return 105; }
+// 106: long sums in parts, products that give up are NaN and seen by the next call
+extern "C" int pa_version(void) { return 106; }
 extern "C" const char *pa_last_error(void) { return pa::g_error; }
 extern "C" int64_t pa_launch_count(void) { return pa::g_launches.load(std::memory_order_relaxed); }

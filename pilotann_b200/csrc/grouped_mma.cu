@@ -17,7 +17,7 @@
 // issues the MMAs, warps 4-7 store the tile before while the next is multiplied (two accumulators in
 // TMEM).  Every wait is bounded.
 //
-// Measured: 128 rows x 64 matrices of 1024 x 2048 (bf16) 44 us, 5.3 TB/s, 81 % of the copy rate: the
+// Measured: 128 rows x 64 matrices of 1024 x 2048 (bf16) 45 us, 5.2 TB/s, 79 % of the copy rate: the
 // rest is the start (4 us to the first slice) and SMs that the memory serves later than others.
 // Larger groups: grouped_pair.cu.
 #include <atomic>
